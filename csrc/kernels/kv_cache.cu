@@ -1,0 +1,258 @@
+// Paged cache of keys and values: quantised as it is written, read back in 16 or 32 bits (sm_100a).
+//
+// Pages are [num_pages, heads, page, D] in bf16, int8 or e4m3, so that the tokens of one head in one page lie together, which is
+// how attention reads them. 8-bit rows (one token of one head) have one fp32 scale each, [num_pages, heads, page]:
+//   int8   s = fl32(max|x| / 127), code = x / s to the nearest, halves to even
+//   e4m3   s = 2^k, the least with max|x| / s <= 448: x / s is then exact, and the only rounding is that to e4m3. A scale of
+//          max|x| / 448 would hold no more: e4m3 has the same three bits behind the leading one in every binade
+// A row whose largest magnitude is below 2^-100 is held as zeros with scale 0; one that has an infinity or a NaN gets the scale
+// NaN, so that reading it says so instead of giving numbers that never were.
+//
+// Bound by memory: each row is read and written once. D / 8 lanes share a row (8 elements each, the row's largest magnitude over
+// shuffles); neighbouring groups take neighbouring heads of a token, which lie together on the contiguous side.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "host_util.h"
+
+namespace tb {
+
+enum : int { KV_BF16 = 0, KV_INT8 = 1, KV_E4M3 = 2 };
+constexpr int KV_THREADS = 256;
+
+struct KvArgs {
+  const void* x[2];            // k, v [B, T, H, D] with strides (write)
+  long sb[2], st[2], sh[2];    // elements
+  void* y[2];                  // k, v [B, T, H, D] contiguous (read)
+  void* pages[2];
+  float* scales[2];
+  const int* table;            // [B, table_ld]
+  const int* start;            // [B]: position of token 0 (null: 0)
+  const int* counts;           // [B]: tokens that count (null: T)
+  long table_ld;
+  int B, T, H, page, pages_per_seq, num_pages;
+};
+
+// Address of a row in the pages, in rows; -1 where the position is outside the table or the table names no page of the pool.
+__device__ __forceinline__ long kv_row(const KvArgs& a, int b, int t, int h) {
+  const int first = a.start ? a.start[b] : 0;
+  if (first < 0) return -1;
+  const unsigned pos = (unsigned)first + (unsigned)t, slot = pos / (unsigned)a.page;   // below 2^32
+  if (slot >= (unsigned)a.pages_per_seq) return -1;
+  const int p = a.table[b * a.table_ld + slot];
+  if ((unsigned)p >= (unsigned)a.num_pages) return -1;
+  return ((long)p * a.H + h) * a.page + (pos - slot * (unsigned)a.page);
+}
+
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    Vec16<T> v;
+    v.load_nc(p);
+    v.get(f);
+  } else {
+    const float4 u = __ldg((const float4*)p), w = __ldg((const float4*)p + 1);
+    f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = w.x, f[5] = w.y, f[6] = w.z, f[7] = w.w;
+  }
+}
+
+// x / s to the nearest integer, halves to even, decided exactly: n is next to the quotient, x - n s is exact in one fma (s has
+// 24 bits, n 7, and the rest is smaller than s), and s / 2 is exact. A quotient in fp32 can round onto a half that x / s is not.
+__device__ __forceinline__ int kv_round(float x, float s, float inv) {
+  float n = rintf(x * inv);
+  const float r = fmaf(-n, s, x), h = 0.5f * s;
+  const bool odd = ((int)n & 1) != 0;
+  if (r > h || (r == h && odd)) n += 1.f;
+  else if (r < -h || (r == -h && odd)) n -= 1.f;
+  return (int)n;
+}
+
+template <typename T, int KIND, int D>
+__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvArgs a) {
+  constexpr int G = D / 8;
+  const int lane = threadIdx.x % G;
+  const unsigned r = blockIdx.x * (KV_THREADS / G) + threadIdx.x / G;
+  const int b = blockIdx.y;
+  const int t = (int)(r / (unsigned)a.H), h = (int)(r - (unsigned)t * a.H);
+  const int n = a.counts ? min(a.counts[b], a.T) : a.T;
+  const bool mine = t < n;
+  long row = -1;
+  float f[2][8];
+  if (mine) {
+    row = kv_row(a, b, t, h);
+    if (row < 0 && lane == 0) report_bad_index();
+#pragma unroll
+    for (int z = 0; z < 2; ++z) load8<T>((const T*)a.x[z] + b * a.sb[z] + t * a.st[z] + h * a.sh[z] + lane * 8, f[z]);
+  } else {
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[z][j] = 0.f;
+  }
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    if constexpr (KIND == KV_BF16) {
+      Vec16<bf16> v;
+      v.set(f[z]);
+      if (row >= 0) v.store((bf16*)a.pages[z] + row * D + lane * 8);
+    } else {
+      float big = 0.f;
+      bool wild = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        big = fmaxf(big, fabsf(f[z][j]));
+        wild |= (__float_as_uint(f[z][j]) & 0x7f800000u) == 0x7f800000u;
+      }
+      big = group_max<G>(wild ? __int_as_float(0x7f800000) : big);
+      wild = big > FLT_MAX;
+      const bool none = big < 7.888609052210118e-31f;   // 2^-100
+      float s, inv;
+      if (KIND == KV_INT8) {
+        s = __fdiv_rn(big, 127.f);
+        inv = __fdiv_rn(1.f, none ? 1.f : s);
+      } else {
+        // big = m 2^e with m in [1, 2); 448 = 1.75 x 2^8
+        const uint32_t u = __float_as_uint(big);
+        const int k = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u);
+        s = __int_as_float((k + 127) << 23);
+        inv = __int_as_float((127 - k) << 23);
+      }
+      uint32_t w[2] = {0u, 0u};
+      if (!none && !wild) {
+        if (KIND == KV_INT8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv_round(f[z][j], s, inv) & 0xffu) << (8 * (j & 3));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2)
+            w[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[z][j] * inv, f[z][j + 1] * inv), __NV_SATFINITE, __NV_E4M3)
+                         << (8 * (j & 3));
+        }
+      }
+      if (row >= 0) {
+        *(uint2*)((uint8_t*)a.pages[z] + row * D + lane * 8) = make_uint2(w[0], w[1]);
+        if (lane == 0) a.scales[z][row] = wild ? __int_as_float(0x7fffffff) : none ? 0.f : s;
+      }
+    }
+  }
+}
+
+template <typename T, int KIND, int D>
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvArgs a) {
+  constexpr int G = D / 8;
+  const int lane = threadIdx.x % G;
+  const unsigned r = blockIdx.x * (KV_THREADS / G) + threadIdx.x / G;
+  const int b = blockIdx.y;
+  const int t = (int)(r / (unsigned)a.H), h = (int)(r - (unsigned)t * a.H);
+  if (t >= a.T) return;
+  const int n = a.counts ? a.counts[b] : a.T;
+  long row = -1;
+  if (t < n) {
+    row = kv_row(a, b, t, h);
+    if (row < 0 && lane == 0) report_bad_index();
+  }
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    float f[8] = {};
+    if (row >= 0) {
+      if constexpr (KIND == KV_BF16) {
+        load8<bf16>((const bf16*)a.pages[z] + row * D + lane * 8, f);
+      } else {
+        const uint2 w = __ldg((const uint2*)((const uint8_t*)a.pages[z] + row * D + lane * 8));
+        const float s = __ldg(a.scales[z] + row);
+        const uint32_t ws[2] = {w.x, w.y};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint8_t byte = (uint8_t)(ws[j >> 2] >> (8 * (j & 3)));
+          if (KIND == KV_INT8) f[j] = (float)(int8_t)byte * s;
+          else f[j] = __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3))) * s;
+        }
+      }
+    }
+    T* y = (T*)a.y[z] + (((long)b * a.T + t) * a.H + h) * D + lane * 8;
+    if constexpr (sizeof(T) == 2) {
+      Vec16<T> v;
+      v.set(f);
+      v.store(y);
+    } else {
+      *(float4*)y = make_float4(f[0], f[1], f[2], f[3]);
+      *((float4*)y + 1) = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  }
+}
+
+template <typename T, int KIND>
+static int kv_launch(const KvArgs& a, int D, bool write, cudaStream_t st) {
+  const dim3 grid((unsigned)ceil_div((long)a.T * a.H, KV_THREADS / (D / 8)), (unsigned)a.B);
+  if (write) {
+    if (D == 64) kv_write_kernel<T, KIND, 64><<<grid, KV_THREADS, 0, st>>>(a);
+    else kv_write_kernel<T, KIND, 128><<<grid, KV_THREADS, 0, st>>>(a);
+  } else {
+    if (D == 64) kv_read_kernel<T, KIND, 64><<<grid, KV_THREADS, 0, st>>>(a);
+    else kv_read_kernel<T, KIND, 128><<<grid, KV_THREADS, 0, st>>>(a);
+  }
+  TB_CUDA_CHECK(cudaGetLastError());
+  return 0;
+}
+
+static int kv_check(const KvArgs& a, int D, int kind, int dtype) {
+  if (D != 64 && D != 128) TB_FAIL(TB_E_ARG, "kv cache: head dim 64 or 128");
+  if (kind < 0 || kind > 2 || (dtype != 0 && dtype != 1)) TB_FAIL(TB_E_ARG, "kv cache: pages in bf16, int8 or e4m3, rows in bf16 or fp32");
+  if (a.page <= 0 || a.num_pages < 0 || a.pages_per_seq < 0 || a.H <= 0) TB_FAIL(TB_E_ARG, "kv cache: bad sizes");
+  if (a.B > 65535 || (long)a.T * a.H > 0x7fffff00l) TB_FAIL(TB_E_TOO_LARGE, "kv cache: at most 65535 sequences and 2^31 rows a sequence in one call");
+  for (int z = 0; z < 2; ++z)
+    if (!a.pages[z] || ((uintptr_t)a.pages[z] & 15) || (kind != KV_BF16 && !a.scales[z])) TB_FAIL(TB_E_ARG, "kv cache: pages must be 16-byte aligned and 8-bit pages have scales");
+  if (!a.table) TB_FAIL(TB_E_ARG, "kv cache: no page table");
+  return 0;
+}
+
+template <typename T>
+static int kv_dispatch(const KvArgs& a, int D, int kind, bool write, cudaStream_t st) {
+  if (kind == KV_BF16) return kv_launch<T, KV_BF16>(a, D, write, st);
+  if (kind == KV_INT8) return kv_launch<T, KV_INT8>(a, D, write, st);
+  return kv_launch<T, KV_E4M3>(a, D, write, st);
+}
+
+}  // namespace tb
+using namespace tb;
+
+int tb_set_check_word_kv_cache(int* word) {
+  TB_CUDA_CHECK(set_check_word_this_tu(word));
+  return 0;
+}
+
+// k, v [B, T, H, D]: strides (batch, token, head) in elements, multiples of 16 bytes; rows t >= counts[b] are left out.
+TB_EXPORT int tb_kv_write(const void* k, const void* v, const long* strides, void* k_pages, void* v_pages, float* k_scales,
+                          float* v_scales, const int* table, long table_ld, const int* start, const int* counts, int B, int T,
+                          int H, int D, int page, int pages_per_seq, int num_pages, int kind, int dtype, cudaStream_t st) {
+  TB_ENSURE_DEVICE();
+  if (B <= 0 || T <= 0) return 0;
+  KvArgs a{{k, v}, {strides[0], strides[3]}, {strides[1], strides[4]}, {strides[2], strides[5]}, {nullptr, nullptr}, {k_pages, v_pages},
+           {k_scales, v_scales}, table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages};
+  if (int r = kv_check(a, D, kind, dtype)) return r;
+  const int N = dtype == 0 ? 8 : 4;
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] % N) TB_FAIL(TB_E_ARG, "kv cache: strides must be multiples of 16 bytes");
+  if (!k || !v || (((uintptr_t)k | (uintptr_t)v) & 15)) TB_FAIL(TB_E_ARG, "kv cache: k and v must be 16-byte aligned");
+  return dtype == 0 ? kv_dispatch<bf16>(a, D, kind, true, st) : kv_dispatch<float>(a, D, kind, true, st);
+}
+
+// yk, yv [B, T, H, D] contiguous: rows t >= counts[b] and rows that no page holds are zeros.
+TB_EXPORT int tb_kv_read(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales, void* yk, void* yv,
+                         const int* table, long table_ld, const int* start, const int* counts, int B, int T, int H, int D,
+                         int page, int pages_per_seq, int num_pages, int kind, int dtype, cudaStream_t st) {
+  TB_ENSURE_DEVICE();
+  if (B <= 0 || T <= 0) return 0;
+  KvArgs a{{nullptr, nullptr}, {0, 0}, {0, 0}, {0, 0}, {yk, yv}, {(void*)k_pages, (void*)v_pages}, {(float*)k_scales, (float*)v_scales},
+           table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages};
+  if (int r = kv_check(a, D, kind, dtype)) return r;
+  if (!yk || !yv || (((uintptr_t)yk | (uintptr_t)yv) & 15)) TB_FAIL(TB_E_ARG, "kv cache: outputs must be 16-byte aligned");
+  return dtype == 0 ? kv_dispatch<bf16>(a, D, kind, false, st) : kv_dispatch<float>(a, D, kind, false, st);
+}

@@ -1,0 +1,321 @@
+// Verification of drafted tokens against the target's probabilities, from given uniform numbers (sm_100a).
+//
+// Node 0 is the last confirmed token, nodes 1 .. n-1 are drafted; probs[b, i] is the target's distribution after node i.
+//   chain with the draft's distributions q: node i + 1 is accepted while u_i q_i(x) < p_i(x). After the first refusal the next token
+//     is drawn from max(p - q, 0), after the last node from p
+//   fixed candidates, a chain or a tree: the children of a node share its number u; in index order each takes an interval of length
+//     p(x) behind the one before, and the child whose interval holds u is accepted (a token that comes twice has its mass
+//     once). Where none does, the next token is drawn from p without the children's tokens
+// Either way the token that follows and the accepted ones are distributed as if they had been drawn from p one by one.
+//
+// The walk needs only p (and q) at the drafted tokens: T scalars, loaded at once. What is bound by memory is the row (or two) that
+// the next token is drawn from, by inversion: a cluster of eight CTAs shares a sequence's row, a warp sums one of 128 segments,
+// the sums meet over distributed shared memory, and the CTA whose segment holds u * total goes through it once more. All sums are
+// in 64 bits: a token next to a border of the cumulative sum is then the same whatever the order of adding.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "host_util.h"
+
+namespace tb {
+
+namespace cg = cooperative_groups;
+
+constexpr int VD_CLUSTER = 8;
+constexpr int VD_THREADS = 512;
+constexpr int VD_WARPS = VD_THREADS / 32;
+constexpr int VD_SEGMENTS = VD_CLUSTER * VD_WARPS;
+static_assert(VD_SEGMENTS == 128, "pick_range() takes four sums a lane");
+constexpr int VD_MAX_NODES = 1024;
+constexpr int VD_UNROLL = 8;
+
+struct VerifyArgs {
+  const void *probs, *draft;        // [B, T, V], [B, T - 1, V] or null
+  long pb, pt, db, dt;              // strides in elements
+  const long* tokens;               // [B, T]
+  const long* parents;              // [B or 1, T]; null: a chain
+  long parents_ld;
+  const float* uniforms;            // [B, T]
+  const int* counts;                // [B] or null
+  long *accepted, *path, *next;     // [B], [B, T], [B]
+  int B, T, V;
+};
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_scan_d(double v, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+__device__ __forceinline__ double mass_of(float p, float q) {
+  const double r = (double)p - (double)q;
+  return r > 0.0 ? r : 0.0;   // negative and NaN: none
+}
+
+// The mass of columns [c, c + 32 * n) that a warp's lanes hold, in order: lane l has c + l, c + 32 + l, ...
+struct Row {
+  const void *p, *q;          // q null: nothing is taken off
+  const uint32_t* out;        // bit per column from `base` on that is left out; null: none
+  int base;
+};
+template <typename T>
+__device__ __forceinline__ double mass_at(const Row& r, int c, int end) {
+  if (c >= end) return 0.0;
+  const float p = to_f<T>(((const T*)r.p)[c]);
+  const float q = r.q ? to_f<T>(((const T*)r.q)[c]) : 0.f;
+  const bool gone = r.out && ((r.out[(c - r.base) >> 5] >> ((c - r.base) & 31)) & 1u);
+  return gone ? 0.0 : mass_of(p, q);
+}
+template <typename T>
+__device__ __forceinline__ double sum_range(const Row& r, int c0, int end, int lane) {
+  double sum = 0.0;
+  int c = c0 + lane;
+  for (; c + 32 * (VD_UNROLL - 1) < end; c += 32 * VD_UNROLL) {
+    float p[VD_UNROLL], q[VD_UNROLL];
+#pragma unroll
+    for (int i = 0; i < VD_UNROLL; ++i) p[i] = to_f<T>(((const T*)r.p)[c + 32 * i]);
+    if (r.q) {
+#pragma unroll
+      for (int i = 0; i < VD_UNROLL; ++i) q[i] = to_f<T>(((const T*)r.q)[c + 32 * i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VD_UNROLL; ++i) q[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < VD_UNROLL; ++i) {
+      const int at = c + 32 * i - r.base;
+      const bool gone = r.out && ((r.out[at >> 5] >> (at & 31)) & 1u);
+      sum += gone ? 0.0 : mass_of(p[i], q[i]);
+    }
+  }
+  for (; c < end; c += 32) sum += mass_at<T>(r, c, end);
+  return warp_sum_d(sum);
+}
+
+// Of the masses of up to 128 consecutive ranges (lane l of a warp holds m[0..3] of ranges 4l .. 4l + 3): the range in which the running
+// sum passes `target` (`scale`: target * total) (rounding can leave none: then the last that has any mass; -1: no mass at all), and the sum
+// before it.
+__device__ __forceinline__ void pick_range(const double (&m)[4], double first, double& target, bool scale, int lane, int& hit, double& before) {
+  const double own = (m[0] + m[1]) + (m[2] + m[3]);
+  const double incl = warp_scan_d(own, lane);
+  double at = __shfl_up_sync(0xffffffffu, incl, 1);
+  at = first + (lane ? at : 0.0);
+  if (scale) target *= __shfl_sync(0xffffffffu, incl, 31);
+  int last = -1, over = -1;
+  double b_last = 0.0, b_over = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double next = at + m[i];
+    if (m[i] > 0.0) {
+      last = 4 * lane + i;
+      b_last = at;
+      if (over < 0 && next > target) {
+        over = last;
+        b_over = at;
+      }
+    }
+    at = next;
+  }
+  const unsigned some = __ballot_sync(0xffffffffu, last >= 0), past = __ballot_sync(0xffffffffu, over >= 0);
+  const int src = past ? __ffs(past) - 1 : some ? 31 - __clz(some) : 0;
+  hit = __shfl_sync(0xffffffffu, past ? over : last, src);
+  before = __shfl_sync(0xffffffffu, past ? b_over : b_last, src);
+}
+
+template <typename T>
+__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS) verify_kernel(const VerifyArgs a, int words) {
+  extern __shared__ uint32_t out_bits[];                 // this CTA's columns
+  __shared__ float mass[VD_MAX_NODES], dmass[VD_MAX_NODES];
+  __shared__ int parent[VD_MAX_NODES], token[VD_MAX_NODES];
+  __shared__ double seg[VD_WARPS], sub[VD_WARPS], s_target, s_before;
+  __shared__ int s_last, s_kids, s_hit;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), b = blockIdx.x / VD_CLUSTER;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = min(max(a.counts ? a.counts[b] : a.T, 1), a.T);
+  const T* probs = (const T*)a.probs + b * a.pb;
+  const T* draft = a.draft ? (const T*)a.draft + b * a.db : nullptr;
+  const long* par = a.parents ? a.parents + b * a.parents_ld : nullptr;
+  const float* u = a.uniforms + (long)b * a.T;
+
+  for (int i = tid; i < n; i += VD_THREADS) {
+    const long tk = a.tokens[(long)b * a.T + i];
+    const long pr = par ? par[i] : i - 1;
+    const bool ok = i > 0 && tk >= 0 && tk < a.V && pr >= 0 && pr < i;   // anything else is never accepted
+    if (i > 0 && !ok) report_bad_index();
+    parent[i] = ok ? (int)pr : -1;
+    token[i] = ok ? (int)tk : -1;
+    mass[i] = ok ? to_f<T>(probs[pr * a.pt + tk]) : 0.f;
+    dmass[i] = ok && draft ? to_f<T>(draft[pr * a.dt + tk]) : 0.f;
+  }
+  for (int i = tid; i < words; i += VD_THREADS) out_bits[i] = 0;
+  __syncthreads();
+  if (!draft && par) {   // a token that is drafted twice under one parent
+    for (int i = tid; i < n; i += VD_THREADS) {
+      bool twice = false;
+      for (int j = 1; j < i; ++j) twice |= parent[j] == parent[i] && token[j] == token[i];
+      if (twice) dmass[i] = 1.f;   // unused otherwise without a draft distribution: marks the mass as taken
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    int cur = 0, took = 0;
+    bool kids = false;
+    long* path = rank == 0 ? a.path + (long)b * a.T : nullptr;
+    if (path && lane == 0) path[0] = 0;
+    while (true) {
+      int step = -1;
+      kids = false;
+      if (draft) {
+        if (cur + 1 < n) {
+          kids = true;
+          if (parent[cur + 1] == cur && (double)u[cur] * (double)dmass[cur + 1] < (double)mass[cur + 1]) step = cur + 1;
+        }
+      } else {
+        double low = 0.0;
+        const double x = (double)u[cur];
+        for (int j0 = cur + 1; j0 < n; j0 += 32) {
+          const int j = j0 + lane;
+          unsigned hit = __ballot_sync(0xffffffffu, j < n && parent[j] == cur);
+          kids |= hit != 0;
+          while (hit) {
+            const int c = j0 + __ffs(hit) - 1;
+            hit &= hit - 1;
+            const double m = dmass[c] != 0.f ? 0.0 : mass_of(mass[c], 0.f);
+            if (step < 0 && low <= x && x < low + m) step = c;
+            low += m;
+          }
+          if (!par) break;   // a chain: the child is the next node
+        }
+      }
+      if (step < 0) break;
+      cur = step;
+      ++took;
+      if (path && lane == 0) path[took] = cur;
+    }
+    if (path)
+      for (int i = took + 1 + lane; i < a.T; i += 32) path[i] = -1;
+    if (lane == 0) {
+      s_last = cur;
+      s_kids = kids;
+      if (rank == 0) a.accepted[b] = took;
+    }
+  }
+  __syncthreads();
+
+  // segments: multiples of 32 columns, so that a segment's words of the bit map are its own
+  const int last = s_last;
+  const int len = (((a.V + VD_SEGMENTS - 1) / VD_SEGMENTS) + 31) & ~31;
+  const int base = rank * VD_WARPS * len;                // may lie behind the last column
+  Row row{probs + last * a.pt, draft && s_kids ? draft + last * a.dt : nullptr, nullptr, base};
+  if (!draft && s_kids) {
+    for (int i = tid + 1; i < n; i += VD_THREADS)
+      if (parent[i] == last && token[i] >= base && token[i] < base + VD_WARPS * len)
+        atomicOr(&out_bits[(token[i] - base) >> 5], 1u << ((token[i] - base) & 31));
+    row.out = out_bits;
+    __syncthreads();
+  }
+  double target = 0.0, at = 0.0;
+  int hit = -1;
+  for (int pass = 0; pass < 2; ++pass) {
+    const int c0 = min(base + warp * len, a.V), c1 = min(c0 + len, a.V);
+    const double s = sum_range<T>(row, c0, c1, lane);
+    if (lane == 0) seg[warp] = s;
+    cluster.sync();
+    if (warp == 0) {                                     // every CTA does the same with the same numbers
+      double m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = cluster.map_shared_rank(seg, (4 * lane + i) / VD_WARPS)[(4 * lane + i) % VD_WARPS];
+      target = (double)u[a.T - 1];
+      pick_range(m, 0.0, target, true, lane, hit, at);
+      if (lane == 0) {
+        s_hit = hit;
+        s_target = target;
+        s_before = at;
+      }
+    }
+    cluster.sync();                                      // nobody's sums are written again, or its CTA gone, while they are read
+    hit = s_hit;
+    if (hit >= 0) break;
+    row.q = nullptr;                                     // the draft covers all of p: draw from p itself
+    row.out = nullptr;
+  }
+  if (hit < 0) {
+    if (rank == 0 && tid == 0) a.next[b] = -1;
+    return;
+  }
+  if (hit / VD_WARPS != rank) return;
+  target = s_target;
+  at = s_before;
+  const int c0 = hit * len, c1 = min(c0 + len, a.V);
+  const int part = ((len / 32 + VD_WARPS - 1) / VD_WARPS) * 32;
+  {
+    const int s0 = min(c0 + warp * part, c1), s1 = min(s0 + part, c1);
+    const double s = sum_range<T>(row, s0, s1, lane);
+    if (lane == 0) sub[warp] = s;
+  }
+  __syncthreads();
+  if (warp) return;
+  {
+    double m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = 4 * lane + i < VD_WARPS ? sub[4 * lane + i] : 0.0;
+    const double first = at;
+    pick_range(m, first, target, false, lane, hit, at);
+    if (hit < 0) hit = 0;                                // not reached: the segment has mass
+  }
+  const int s0 = min(c0 + hit * part, c1), s1 = min(s0 + part, c1);
+  int found = -1;
+  for (int c = s0; c < s1; c += 32) {
+    const double m = mass_at<T>(row, c + lane, s1);
+    const double sum = at + warp_scan_d(m, lane);
+    const unsigned any = __ballot_sync(0xffffffffu, m > 0.0), over = __ballot_sync(0xffffffffu, m > 0.0 && sum > target);
+    if (over) {
+      found = c + __ffs(over) - 1;
+      break;
+    }
+    if (any) found = c + 31 - __clz(any);
+    at = __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) a.next[b] = found;
+}
+
+}  // namespace tb
+using namespace tb;
+
+int tb_set_check_word_verify(int* word) {
+  TB_CUDA_CHECK(set_check_word_this_tu(word));
+  return 0;
+}
+
+TB_EXPORT int tb_verify_draft(const void* probs, const void* draft, const long* tokens, const long* parents, const float* uniforms,
+                              const int* counts, long* accepted, long* path, long* next, long pb, long pt, long db, long dt,
+                              long parents_ld, int B, int T, int V, int dtype, cudaStream_t st) {
+  TB_ENSURE_DEVICE();
+  if (B <= 0) return 0;
+  if (T < 1 || T > VD_MAX_NODES || V < 1) TB_FAIL(TB_E_ARG, "verify: 1 to %d nodes and at least one token in the vocabulary", VD_MAX_NODES);
+  if (!probs || !tokens || !uniforms || !accepted || !path || !next) TB_FAIL(TB_E_ARG, "verify: null pointer");
+  if (dtype != 0 && dtype != 1) TB_FAIL(TB_E_ARG, "verify: bf16 or fp32");
+  if (B > 0x7fffffff / VD_CLUSTER || V > (1 << 22)) TB_FAIL(TB_E_TOO_LARGE, "verify: at most 2^22 tokens in the vocabulary");
+  VerifyArgs a{probs, draft, pb, pt, db, dt, tokens, parents, parents_ld, uniforms, counts, accepted, path, next, B, T, V};
+  const int len = (((V + VD_SEGMENTS - 1) / VD_SEGMENTS) + 31) & ~31;
+  const int words = VD_WARPS * len / 32;                 // 2 KB at V = 128 000, 64 KB at 2^22
+  const int bytes = words * 4;
+  static std::atomic<uint64_t> done16{0}, done32{0};
+  if (dtype == 0) {
+    if (int r = smem_opt_in(done16, verify_kernel<bf16>, 72 * 1024)) return r;
+    verify_kernel<bf16><<<B * VD_CLUSTER, VD_THREADS, bytes, st>>>(a, words);
+  } else {
+    if (int r = smem_opt_in(done32, verify_kernel<float>, 72 * 1024)) return r;
+    verify_kernel<float><<<B * VD_CLUSTER, VD_THREADS, bytes, st>>>(a, words);
+  }
+  TB_CUDA_CHECK(cudaGetLastError());
+  return 0;
+}

@@ -8,7 +8,7 @@ __version__ = "0.1.0"
 from . import core  # noqa: E402
 from .core import DType, Device, DeviceType, RuntimeConfig, Shape, TorshDistributedError, TorshError  # noqa: E402,F401
 from . import ops  # noqa: E402,F401
-from .ops import attention, elementwise, gemm, linear, multi_tensor, norm, softmax  # noqa: E402,F401
+from .ops import attention, elementwise, gemm, kv_cache, linear, multi_tensor, norm, rotary, softmax, speculative  # noqa: E402,F401
 from . import autograd, data, models, nn, optim, parallel, serialize  # noqa: E402,F401
 from . import parallel as distributed  # noqa: E402,F401
 from . import engine  # noqa: E402,F401

@@ -13,9 +13,12 @@ import torch.nn.functional as _tF
 
 from ..ops import attention as _attn
 from ..ops import elementwise as _ew
+from ..ops import kv_cache as _kv
 from ..ops import linear as _lin
 from ..ops import norm as _norm
+from ..ops import rotary as _rot
 from ..ops import softmax as _sm
+from ..ops import speculative as _spec
 
 # ---- kernel-backed -------------------------------------------------------------------------
 relu, sigmoid, tanh, silu, gelu, swiglu = _ew.relu, _ew.sigmoid, _ew.tanh, _ew.silu, _ew.gelu, _ew.swiglu
@@ -23,7 +26,10 @@ swish = silu
 softmax, log_softmax = _sm.softmax, _sm.log_softmax
 embedding_lookup = _ew.embedding
 rope = _ew.rope
+rotary, rotary_frequencies = _rot.rotary, _rot.rotary_frequencies
 flash_attention = _attn.flash_attention
+kv_cache_write, kv_cache_read, kv_cache_attention, tree_mask_of = _kv.kv_cache_write, _kv.kv_cache_read, _kv.kv_cache_attention, _kv.tree_mask_of
+verify_draft = _spec.verify_draft
 
 
 def linear(x, weight, bias=None):

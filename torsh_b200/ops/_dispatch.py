@@ -1,6 +1,7 @@
 """Shared helpers for the op wrappers: dtype codes, alignment checks, ctypes signatures."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -37,6 +38,14 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+_here = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which the device of ``t`` is current: a launch goes to that device's current stream whichever device the caller is on."""
+    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def fn(name: str, argtypes):
     """Fetch a launcher from the CUDA library and set its signature once."""
     f = _fns.get(name)
@@ -48,7 +57,7 @@ def fn(name: str, argtypes):
     return f
 
 
-_KERNELS_PER_CALL = {"tb_flash_attn_bwd": 3, "tb_lamb_multi": 2, "tb_bn_fwd": 3, "tb_bn_bwd": 2}
+_KERNELS_PER_CALL = {"tb_flash_attn_bwd": 3, "tb_lamb_multi": 2, "tb_bn_fwd": 3, "tb_bn_bwd": 2, "tb_cache_attention": 2}
 
 
 def call(name: str, argtypes, *args):
