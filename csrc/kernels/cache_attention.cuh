@@ -22,7 +22,7 @@ struct CacheAttnArgs {
   bf16* out;                   // [B, T, Hq, D] contiguous
   float *part_o, *part_ml;     // partial results: see slot_of()
   int* plan;                   // [0]: tiles of a CTA, [1 .. B]: tiles in front of each sequence
-  int B, T, Hq, Hkv, G, page, num_pages, row_tiles, grid;
+  int B, T, Hq, Hkv, G, page, page_tiles, page_shift, num_pages, row_tiles, grid;   // page_shift: log2 of a page's tiles, or -1
   int limit;                   // tokens of a sequence that the table can name, or fewer
   float scale_log2;
 };
@@ -109,12 +109,6 @@ __device__ __forceinline__ Deal deal_tiles(const CacheAttnArgs& a, int* scratch)
   d.b = found[0];
   d.before = found[1];
   return d;
-}
-
-// A page of the pool for tokens `pos` .. of sequence b; -1: there is none.
-__device__ __forceinline__ int page_of(const CacheAttnArgs& a, int b, int pos) {
-  const int p = __ldg(a.table + (long)b * a.table_ld + pos / a.page);
-  return (unsigned)p < (unsigned)a.num_pages ? p : -1;
 }
 
 __device__ __forceinline__ bool sees(const CacheAttnArgs& a, int b, int t, int pos, const SeqLen& s) {
