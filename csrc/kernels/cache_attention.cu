@@ -104,43 +104,6 @@ __device__ __forceinline__ void put_pair(bf16* row, int mb, int g, float y0, flo
   else row[column_of<false, MB>(mb, 0, g)] = __float2bfloat16(y0), row[column_of<false, MB>(mb, 1, g)] = __float2bfloat16(y1);
 }
 
-// A warp's walk over its tiles of the CTA's run: unit after unit, every CA_WARPS-th tile.
-struct Walk {
-  int b, hr, h, nt, tile, end, left;   // hr: head and row tile; [tile, end): tiles of the unit in this CTA; left: tiles of the run from `end` on
-  int head;                            // first tile of the unit in this CTA
-  SeqLen s;
-};
-__device__ __forceinline__ void walk_unit(const CacheAttnArgs& a, Walk& w, int first_tile, int run) {
-  w.head = first_tile;
-  w.end = min(w.nt, first_tile + run);
-  w.left = run - (w.end - first_tile);
-  w.h = a.row_tiles == 1 ? w.hr : w.hr / a.row_tiles;
-}
-__device__ __forceinline__ void walk_begin(const CacheAttnArgs& a, Walk& w, const Deal& d, int warp) {
-  w.b = d.b;
-  w.s = seq_len(a, d.b);
-  w.nt = (w.s.len + CA_TILE - 1) / CA_TILE;
-  const int in = d.first - d.before;
-  w.hr = in / w.nt;
-  walk_unit(a, w, in - w.hr * w.nt, d.last - d.first);
-  w.tile = w.head + warp;
-}
-// On to the next unit of the run; false: there is none.
-__device__ __forceinline__ bool walk_next(const CacheAttnArgs& a, Walk& w, int warp) {
-  if (w.left <= 0) return false;
-  if (++w.hr == a.Hkv * a.row_tiles) {
-    w.hr = 0;
-    do {
-      if (++w.b >= a.B) return false;
-      w.s = seq_len(a, w.b);
-      w.nt = (w.s.len + CA_TILE - 1) / CA_TILE;
-    } while (w.nt == 0);
-  }
-  walk_unit(a, w, 0, w.left);
-  w.tile = warp;
-  return true;
-}
-
 template <int D, int KIND, int NT>
 __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache_attn_kernel(const CacheAttnArgs a) {
   using S = CaShape<D, KIND, NT>;
@@ -156,27 +119,26 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
   const uint32_t ring_u = ca_smem(ring);
 
   const Deal deal = deal_tiles<CA_THREADS, CA_TILE, CA_WARPS>(a, scratch);
-  if (deal.first >= deal.last) return;
+  zero_empty<D, CA_THREADS>(a);
+  if (deal.first >= deal.last) {
+    if (threadIdx.x == 0) a.plan[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
 
   // the loading side runs STAGES - 1 tiles ahead, its page number one more
   Walk ld;
-  walk_begin(a, ld, deal, warp);
+  walk_begin<CA_TILE>(a, ld, deal, warp);
   bool more = true;
-  int pg = -1, slot_tile = 0;
+  long next_row = -1;
   auto seek = [&]() {
-    while (more && ld.tile >= ld.end) more = walk_next(a, ld, warp);
-    if (more) {
-      const int slot = a.page_shift >= 0 ? ld.tile >> a.page_shift : ld.tile / a.page_tiles;
-      slot_tile = ld.tile - slot * a.page_tiles;
-      const int p = __ldg(a.table + (long)ld.b * a.table_ld + slot);
-      pg = (unsigned)p < (unsigned)a.num_pages ? p : -1;
-    }
+    while (more && ld.tile >= ld.end) more = walk_next<CA_TILE>(a, ld, warp);
+    if (more) next_row = rows_at(a, ld.b, ld.h, ld.tile * CA_TILE);
   };
   auto load = [&](int stage) {
     if (more) {
-      const int live = pg < 0 ? 0 : min(ld.s.len - ld.tile * CA_TILE, CA_TILE);
-      if (pg < 0 && lane == 0) report_bad_index();
-      const long row = ((long)max(pg, 0) * a.Hkv + ld.h) * a.page + slot_tile * CA_TILE;
+      const int live = next_row < 0 ? 0 : min(ld.s.len - ld.tile * CA_TILE, CA_TILE);
+      if (next_row < 0 && lane == 0) report_bad_index();
+      const long row = max(next_row, 0l);
       const uint8_t* kp = (const uint8_t*)a.k_pages + row * S::ROW + lane * 16;
       const uint8_t* vp = (const uint8_t*)a.v_pages + row * S::ROW + lane * 16;
       const uint32_t dst = ring_u + stage * S::STAGE;
@@ -201,7 +163,8 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
   for (int i = 0; i < S::STAGES - 1; ++i) load(i);
 
   Walk w;
-  walk_begin(a, w, deal, warp);
+  walk_begin<CA_TILE>(a, w, deal, warp);
+  if (threadIdx.x == 0) a.plan[blockIdx.x] = make_int4(w.b, w.hr, w.head, deal.per);
   int stage = 0;
 
   while (true) {
@@ -516,10 +479,17 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
           const float4 z = ((const float4*)(smem + v * S::RING + scratch[36 + v] * S::STAGE))[i * 32 + lane];
           y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
         }
+        const int n = (p0 + i) / MB, j = (p0 + i) % MB;
         if (!whole) {
-          ((float4*)part)[(p0 + i) * 32 + lane] = y;
+          float* pr = part + (n * 8 + 2 * c) * D;
+          if (HALVES) {
+            *(float2*)(pr + column_of<HALVES, MB>(j, 0, g)) = make_float2(y.x, y.z);
+            *(float2*)(pr + D + column_of<HALVES, MB>(j, 0, g)) = make_float2(y.y, y.w);
+          } else {
+            pr[column_of<HALVES, MB>(j, 0, g)] = y.x, pr[column_of<HALVES, MB>(j, 1, g)] = y.z;
+            pr[D + column_of<HALVES, MB>(j, 0, g)] = y.y, pr[D + column_of<HALVES, MB>(j, 1, g)] = y.w;
+          }
         } else {
-          const int n = (p0 + i) / MB, j = (p0 + i) % MB;
           const float yy[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
@@ -538,72 +508,76 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
       }
     }
     __syncthreads();   // the stages and ml are free again
-    if (!walk_next(a, w, warp)) break;
+    if (!walk_next<CA_TILE>(a, w, warp)) break;
   }
   ca_wait<0>();
 }
 
-// Joins the parts of the units that the deal has cut, and writes the rows of sequences that see nothing. Block (unit, four blocks of
-// 16 columns and 8 rows); its warps share the parts, then the blocks.
+// Joins the parts of the units that the deal has cut. Blocks x look at the unit that CTA x began with: if that is its first cut, they
+// join it. `share` warps have a row between them, and its parts.
 constexpr int CJ_WARPS = 8;
-template <int D, bool HALVES, int NT>
-__global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const CacheAttnArgs a) {
-  constexpr int MB = D / 16, ROWS = 8 * NT, JB = 4;
-  __shared__ float4 buf[CJ_WARPS][JB][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int unit = blockIdx.x, n = blockIdx.y * JB / MB, j0 = blockIdx.y * JB % MB;
-  const int units = a.Hkv * a.row_tiles;
-  const int b = unit / units, hr = unit - b * units;
+template <int D>
+__global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const CacheAttnArgs a, int tile, int share) {
+  constexpr int N = D / 32;                            // columns of a lane
+  __shared__ float buf[CJ_WARPS][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 p = a.plan[blockIdx.x];
+  if (p.w == 0 || p.z == 0 || p.z > p.w) return;       // nothing; a unit's beginning; not its first cut
+  const int b = p.x, hr = p.y, per = p.w;
+  const int h = a.row_tiles == 1 ? hr : hr / a.row_tiles;
+  const int r = blockIdx.y * (CJ_WARPS / share) + warp / share, sub = warp % share;
+  const int row = (hr - h * a.row_tiles) * a.part_rows + r, t = row / a.G;
+  const bool mine = r < a.part_rows && t < a.T;
   const SeqLen s = seq_len(a, b);
-  const int nt = (s.len + CA_TILE - 1) / CA_TILE;
-  const int per = a.plan[0], first = a.plan[1 + b] + hr * nt;
-  const int c0 = nt ? first / per : 0, c1 = nt ? (first + nt - 1) / per : -1;
-  if (c0 == c1) return;                                // whole: written already
-  float4 y[JB];
+  const int nt = (s.len + tile - 1) / tile;
+  const int c0 = blockIdx.x - 1, c1 = (blockIdx.x * per - p.z + nt - 1) / per;
+  float top = -INFINITY, all = 0.f, y[N] = {};
+  if (mine) {
+    for (int k = c0 + lane; k <= c1; k += 32) {
+      const float2 z = *(const float2*)(a.part_ml + ((long)slot_of(k, k > c0) * a.part_rows + r) * 2);
+      const float now = fmaxf(top, z.x), ref = now == -INFINITY ? 0.f : now;
+      all = all * exp2f(top - ref) + z.y * exp2f(z.x - ref);
+      top = now;
+    }
+    const float now = warp_max(top), ref = now == -INFINITY ? 0.f : now;
+    all = warp_sum(all * exp2f(top - ref));
+#pragma unroll 4
+    for (int k = c0 + sub; k <= c1; k += share) {
+      const long at = (long)slot_of(k, k > c0) * a.part_rows + r;
+      const float f = exp2f(a.part_ml[at * 2] - ref);
+      const float* o = a.part_o + at * D + lane * N;
 #pragma unroll
-  for (int j = 0; j < JB; ++j) y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float top[2] = {-INFINITY, -INFINITY}, all[2] = {0.f, 0.f};
-  for (int k = c0; k <= c1; ++k) {
-    const float4 z = *(const float4*)(a.part_ml + ((long)slot_of(k, k > c0) * ROWS + n * 8 + 2 * c) * 2);
-    top[0] = fmaxf(top[0], z.x);
-    top[1] = fmaxf(top[1], z.z);
-  }
-  const float ref[2] = {top[0] == -INFINITY ? 0.f : top[0], top[1] == -INFINITY ? 0.f : top[1]};
-  for (int k = c0; k <= c1; ++k) {
-    const long slot = slot_of(k, k > c0);
-    const float4 z = *(const float4*)(a.part_ml + (slot * ROWS + n * 8 + 2 * c) * 2);
-    const float f[2] = {exp2f(z.x - ref[0]), exp2f(z.z - ref[1])};
-    all[0] += z.y * f[0];
-    all[1] += z.w * f[1];
-    if ((k - c0) % CJ_WARPS == warp) {
-#pragma unroll
-      for (int j = 0; j < JB; ++j) {
-        const float4 x = ((const float4*)(a.part_o + slot * ROWS * D))[(n * MB + j0 + j) * 32 + lane];
-        y[j].x += x.x * f[0], y[j].y += x.y * f[1], y[j].z += x.z * f[0], y[j].w += x.w * f[1];
+      for (int i = 0; i < N; i += 2) {
+        const float2 z = *(const float2*)(o + i);
+        y[i] += z.x * f, y[i + 1] += z.y * f;
       }
     }
   }
+  if (share > 1) {
 #pragma unroll
-  for (int j = 0; j < JB; ++j) buf[warp][j][lane] = y[j];
-  __syncthreads();
-  if (warp >= JB) return;
-  float4 z = buf[0][warp][lane];
+    for (int i = 0; i < N; ++i) buf[warp][lane * N + i] = y[i];
+    __syncthreads();
+    if (sub) return;
+    for (int v = 1; v < share; ++v)
 #pragma unroll
-  for (int v = 1; v < CJ_WARPS; ++v) {
-    const float4 x = buf[v][warp][lane];
-    z.x += x.x, z.y += x.y, z.z += x.z, z.w += x.w;
+      for (int i = 0; i < N; ++i) y[i] += buf[warp + v][lane * N + i];
   }
-  const float zz[4] = {z.x, z.y, z.z, z.w};
-  const int h = hr / a.row_tiles, row0 = (hr - h * a.row_tiles) * ROWS;
+  if (!mine) return;
+  const float norm = t < s.count && (all > 0.f || all != all) ? 1.f / all : 0.f;   // a row that sees nothing: zeros
+  bf16* op = a.out + (((long)b * a.T + t) * a.Hq + h * a.G + row - t * a.G) * D + lane * N;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = row0 + n * 8 + 2 * c + r, t = row / a.G;
-    if (t >= a.T) continue;
-    const float norm = t < s.count && (all[r] > 0.f || all[r] != all[r]) ? 1.f / all[r] : 0.f;
-    const bool live = t < s.count;
-    bf16* op = a.out + (((long)b * a.T + t) * a.Hq + h * a.G + row - t * a.G) * D;
-    put_pair<HALVES, MB>(op, j0 + warp, g, live ? zz[r] * norm : 0.f, live ? zz[2 + r] * norm : 0.f);
-  }
+  for (int i = 0; i < N; i += 2) *(uint32_t*)(op + i) = t < s.count ? pack2<false>(y[i] * norm, y[i + 1] * norm) : 0u;
+}
+
+int cache_attn_join(const CacheAttnArgs& a, int D, int tile, cudaStream_t st) {
+  // one sequence cuts few units into many parts, many sequences many units into few
+  const long units = (long)a.B * a.Hkv * a.row_tiles;
+  const int share = units * 8 >= a.grid ? 1 : CJ_WARPS;
+  const dim3 grid((unsigned)a.grid, (unsigned)((a.part_rows * share + CJ_WARPS - 1) / CJ_WARPS));
+  if (D == 64) cache_attn_join_kernel<64><<<grid, CJ_WARPS * 32, 0, st>>>(a, tile, share);
+  else cache_attn_join_kernel<128><<<grid, CJ_WARPS * 32, 0, st>>>(a, tile, share);
+  TB_CUDA_CHECK(cudaGetLastError());
+  return 0;
 }
 
 template <int D, int KIND, int NT>
@@ -614,10 +588,7 @@ static int cache_attn_launch(CacheAttnArgs& a, cudaStream_t st) {
   a.grid = S::OCC * sm_count();
   cache_attn_kernel<D, KIND, NT><<<a.grid, CA_THREADS, S::SMEM, st>>>(a);
   TB_CUDA_CHECK(cudaGetLastError());
-  const dim3 grid((unsigned)(a.B * a.Hkv * a.row_tiles), (unsigned)(S::BLOCKS / 4));
-  cache_attn_join_kernel<D, S::HALVES, NT><<<grid, CJ_WARPS * 32, 0, st>>>(a);
-  TB_CUDA_CHECK(cudaGetLastError());
-  return 0;
+  return cache_attn_join(a, D, CA_TILE, st);
 }
 
 template <int D, int KIND>
@@ -636,21 +607,26 @@ static int cache_attn_kind(CacheAttnArgs& a, int kind, int nt, cudaStream_t st) 
 // Blocks of 8 rows that a CTA takes: 1, 2 or 4.
 static int ca_row_blocks(long rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 constexpr int CA_MAX_OCC = 4;
+// Up to here the rows go to this file's kernel, beyond to the one on tcgen05.
+constexpr long CA_MAX_ROWS = 16;
+static long ca_slots(bool tc) { return 2l * (tc ? 1 : CA_MAX_OCC) * sm_count(); }
+// Rows of a slot of partial results: a multiple of 4, so that what follows stays aligned.
+static int ca_part_rows(long rows) { return rows > CA_MAX_ROWS ? (int)(rows < 128 ? (rows + 3) & ~3l : 128) : 8 * ca_row_blocks(rows); }
 
 }  // namespace tb
 using namespace tb;
 
+int tb_set_check_word_cache_attention_tc(int* word);
 int tb_set_check_word_cache_attention(int* word) {
   TB_CUDA_CHECK(set_check_word_this_tu(word));
-  return 0;
+  return tb_set_check_word_cache_attention_tc(word);
 }
 
 // Bytes of workspace that tb_cache_attention needs for these sizes.
 TB_EXPORT long tb_cache_attention_workspace(int B, int T, int Hq, int Hkv, int D) {
   if (ensure_device() || Hkv <= 0) return -1;
-  const int rows = 8 * ca_row_blocks((long)T * (Hq / Hkv));
-  const long slots = 2l * CA_MAX_OCC * sm_count();
-  return slots * rows * D * 4 + slots * rows * 8 + ((long)B + 1) * 4 + 256;
+  const long rows = (long)T * (Hq / Hkv), slots = ca_slots(rows > CA_MAX_ROWS);
+  return slots * ca_part_rows(rows) * (D * 4 + 8) + slots / 2 * 16;
 }
 
 // q [B, T, Hq, D] bf16 (strides in elements, multiples of 8; 16-byte aligned), out contiguous. ws: tb_cache_attention_workspace() bytes,
@@ -658,7 +634,7 @@ TB_EXPORT long tb_cache_attention_workspace(int B, int T, int Hq, int Hkv, int D
 TB_EXPORT int tb_cache_attention(const void* q, const long* q_strides, const void* k_pages, const void* v_pages, const float* k_scales,
                                  const float* v_scales, const int* table, long table_ld, const int* start, const int* counts,
                                  const uint8_t* mask, long mask_b, long mask_t, void* out, void* ws, int B, int T, int Hq, int Hkv,
-                                 int D, int page, int pages_per_seq, int num_pages, int max_len, int kind, float scale, cudaStream_t st) {
+                                 int D, int page, int pages_per_seq, int num_pages, int max_len, int kind, float scale, int* status, cudaStream_t st) {
   TB_ENSURE_DEVICE();
   if (B <= 0 || T <= 0 || Hq <= 0) return 0;
   if (!q || !out || !ws || !k_pages || !v_pages || !table || !start || (kind != CA_BF16 && (!k_scales || !v_scales)))
@@ -677,8 +653,10 @@ TB_EXPORT int tb_cache_attention(const void* q, const long* q_strides, const voi
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.page = page, a.num_pages = num_pages;
   a.scale_log2 = scale * 1.4426950408889634f;
   const long rows = (long)T * a.G;
+  const bool tc = rows > CA_MAX_ROWS;
   const int nt = ca_row_blocks(rows);
-  a.row_tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
+  const int per_tile = tc ? 128 : 8 * nt;
+  a.row_tiles = (int)((rows + per_tile - 1) / per_tile);
   a.page_tiles = page / CA_TILE;
   a.page_shift = (a.page_tiles & (a.page_tiles - 1)) ? -1 : __builtin_ctz((unsigned)a.page_tiles);
   const long held = (long)pages_per_seq * page;
@@ -686,9 +664,11 @@ TB_EXPORT int tb_cache_attention(const void* q, const long* q_strides, const voi
   const long tiles = ((long)a.limit + CA_TILE - 1) / CA_TILE * B * Hkv * a.row_tiles;
   if (rows > 0x7fffff00l || tiles > 0x7fff0000l || a.limit > 0x7fff0000l || (long)B * Hkv * a.row_tiles > 0x7fff0000l)
     TB_FAIL(TB_E_TOO_LARGE, "cache attention: too much for one call");
-  const long slots = 2l * CA_MAX_OCC * sm_count();
+  const long slots = ca_slots(tc);
+  a.part_rows = ca_part_rows(rows);
   a.part_o = (float*)ws;
-  a.part_ml = a.part_o + slots * 8 * nt * D;
-  a.plan = (int*)(a.part_ml + slots * 8 * nt * 2);
+  a.part_ml = a.part_o + slots * a.part_rows * D;
+  a.plan = (int4*)(a.part_ml + slots * a.part_rows * 2);
+  if (tc) return cache_attn_tc(a, D, kind, status, st);
   return D == 64 ? cache_attn_kind<64>(a, kind, nt, st) : cache_attn_kind<128>(a, kind, nt, st);
 }

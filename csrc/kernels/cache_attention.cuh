@@ -20,9 +20,10 @@ struct CacheAttnArgs {
   const uint8_t* mask;         // [B or 1, T, T]: mask[t, j] != 0: token t sees new token j (null: j <= t)
   long mask_b, mask_t, table_ld;
   bf16* out;                   // [B, T, Hq, D] contiguous
-  float *part_o, *part_ml;     // partial results: see slot_of()
-  int* plan;                   // [0]: tiles of a CTA, [1 .. B]: tiles in front of each sequence
+  float *part_o, *part_ml;     // partial results, [slot][row][D] and [slot][row] of (maximum, sum): see slot_of()
+  int4* plan;                  // of each CTA: the sequence, head and row tile, and tile that it begins with, and the tiles of a CTA (0: it has none)
   int B, T, Hq, Hkv, G, page, page_tiles, page_shift, num_pages, row_tiles, grid;   // page_shift: log2 of a page's tiles, or -1
+  int part_rows;               // rows of a slot of partial results
   int limit;                   // tokens of a sequence that the table can name, or fewer
   float scale_log2;
 };
@@ -43,7 +44,7 @@ __device__ __forceinline__ SeqLen seq_len(const CacheAttnArgs& a, int b) {
 // begins inside it and ends behind it to slot 2c + 1; whole units go straight to the output.
 __device__ __forceinline__ int slot_of(int cta, bool begins_before) { return 2 * cta + (begins_before ? 0 : 1); }
 
-// Sum of a value over the threads of a block in front of this one, and over all; scratch holds 33 ints.
+// Sum of a value over the threads of a block in front of this one, and over all; scratch holds 32 ints.
 template <int THREADS>
 __device__ __forceinline__ int block_prefix(int v, int* scratch, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -67,11 +68,12 @@ __device__ __forceinline__ int block_prefix(int v, int* scratch, int& total) {
 }
 
 // The deal: the tiles of all units in a row, `per` of them to each CTA, so that every CTA has the same share whatever the lengths.
-// Returns the CTA's first sequence and the tiles in front of it. CTA 0 leaves the plan for the kernel that joins the parts.
+// Returns the CTA's first sequence and the tiles in front of it.
 struct Deal {
   int per, first, last;   // tiles of a CTA; this CTA's tiles are [first, last)
   int b, before;          // the sequence that tile `first` is of, and the tiles in front of that sequence
 };
+// `scratch`: 36 ints of shared memory.
 template <int THREADS, int TILE, int ROUND>
 __device__ __forceinline__ Deal deal_tiles(const CacheAttnArgs& a, int* scratch) {
   Deal d;
@@ -83,17 +85,14 @@ __device__ __forceinline__ Deal deal_tiles(const CacheAttnArgs& a, int* scratch)
     int total;
     const int before = all + block_prefix<THREADS>(n, scratch, total);
     if (b0 == 0) keep_n = n, keep_before = before;
-    if (blockIdx.x == 0 && b < a.B) a.plan[1 + b] = before;
     all += total;
   }
   d.per = max((all + a.grid - 1) / a.grid, 1);
   d.per = (d.per + ROUND - 1) / ROUND * ROUND;
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = d.per;
   d.first = min((long)blockIdx.x * d.per, (long)all);
   d.last = min((long)d.first + d.per, (long)all);
   d.b = d.before = 0;
   if (d.first >= d.last) return d;
-  __shared__ int found[2];
   all = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
@@ -103,12 +102,68 @@ __device__ __forceinline__ Deal deal_tiles(const CacheAttnArgs& a, int* scratch)
       before = all + block_prefix<THREADS>(n, scratch, total);
       all += total;
     }
-    if (before <= d.first && d.first < before + n) found[0] = b, found[1] = before;
+    if (before <= d.first && d.first < before + n) scratch[34] = b, scratch[35] = before;
   }
   __syncthreads();
-  d.b = found[0];
-  d.before = found[1];
+  d.b = scratch[34];
+  d.before = scratch[35];
   return d;
+}
+
+// A walk over the tiles of the CTA's run: unit after unit, every STEP-th tile of each from the `offset`-th on.
+struct Walk {
+  int b, hr, h, nt, tile, end, left;   // hr: head and row tile; [tile, end): tiles of the unit in this CTA; left: tiles of the run from `end` on
+  int head;                            // first tile of the unit in this CTA
+  SeqLen s;
+};
+__device__ __forceinline__ void walk_unit(const CacheAttnArgs& a, Walk& w, int first_tile, int run) {
+  w.head = first_tile;
+  w.end = min(w.nt, first_tile + run);
+  w.left = run - (w.end - first_tile);
+  w.h = a.row_tiles == 1 ? w.hr : w.hr / a.row_tiles;
+}
+template <int TILE>
+__device__ __forceinline__ void walk_begin(const CacheAttnArgs& a, Walk& w, const Deal& d, int offset) {
+  w.b = d.b;
+  w.s = seq_len(a, d.b);
+  w.nt = (w.s.len + TILE - 1) / TILE;
+  const int in = d.first - d.before;
+  w.hr = in / w.nt;
+  walk_unit(a, w, in - w.hr * w.nt, d.last - d.first);
+  w.tile = w.head + offset;
+}
+// On to the next unit of the run; false: there is none.
+template <int TILE>
+__device__ __forceinline__ bool walk_next(const CacheAttnArgs& a, Walk& w, int offset) {
+  if (w.left <= 0) return false;
+  if (++w.hr == a.Hkv * a.row_tiles) {
+    w.hr = 0;
+    do {
+      if (++w.b >= a.B) return false;
+      w.s = seq_len(a, w.b);
+      w.nt = (w.s.len + TILE - 1) / TILE;
+    } while (w.nt == 0);
+  }
+  walk_unit(a, w, 0, w.left);
+  w.tile = offset;
+  return true;
+}
+
+// Rows of 16 tokens of a page, tokens `pos` .. of sequence b: the row of the first in the pool, -1 where the table names no page of it.
+__device__ __forceinline__ long rows_at(const CacheAttnArgs& a, int b, int h, int pos) {
+  const int tile = pos >> 4;
+  const int slot = a.page_shift >= 0 ? tile >> a.page_shift : tile / a.page_tiles;
+  const int p = __ldg(a.table + (long)b * a.table_ld + slot);
+  if ((unsigned)p >= (unsigned)a.num_pages) return -1;
+  return ((long)p * a.Hkv + h) * a.page + (tile - slot * a.page_tiles) * 16;
+}
+
+// Sequences that see nothing: their rows are zeros.
+template <int D, int THREADS>
+__device__ __forceinline__ void zero_empty(const CacheAttnArgs& a) {
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (seq_len(a, b).len == 0)
+      for (long i = threadIdx.x; i < (long)a.T * a.Hq * D / 8; i += THREADS) ((uint4*)(a.out + (long)b * a.T * a.Hq * D))[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 __device__ __forceinline__ bool sees(const CacheAttnArgs& a, int b, int t, int pos, const SeqLen& s) {
@@ -149,5 +204,10 @@ __device__ __forceinline__ void pairs_of(uint32_t t0, uint32_t t1, uint32_t (&r)
   halves_of<KIND>(lo, r[0], r[1]);
   halves_of<KIND>(hi, r[2], r[3]);
 }
+
+// Joins the units that the deal has cut; in cache_attention.cu.
+int cache_attn_join(const CacheAttnArgs& a, int D, int tile, cudaStream_t st);
+// The same attention for many rows, on tcgen05; in cache_attention_sm100.cu.
+int cache_attn_tc(CacheAttnArgs& a, int D, int kind, int* status, cudaStream_t st);
 
 }  // namespace tb

@@ -72,6 +72,17 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
   return warp_max(r);
 }
 
+// Quotients by a number that the host knows: a multiplication instead of a division, for numerators below 2^31.
+struct FastDiv {
+  unsigned d, m, s;
+  __host__ static FastDiv of(unsigned d) {
+    unsigned s = 0;
+    while (s < 32 && (1ull << s) < d) ++s;
+    return {d, (unsigned)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
 __host__ __device__ inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 }  // namespace tb

@@ -31,13 +31,16 @@ struct KvArgs {
   const int* counts;           // [B]: tokens that count (null: T)
   long table_ld;
   int B, T, H, page, pages_per_seq, num_pages;
+  FastDiv by_h, by_page;
 };
 
 // Address of a row in the pages, in rows; -1 where the position is outside the table or the table names no page of the pool.
 __device__ __forceinline__ long kv_row(const KvArgs& a, int b, int t, int h) {
   const int first = a.start ? a.start[b] : 0;
   if (first < 0) return -1;
-  const unsigned pos = (unsigned)first + (unsigned)t, slot = pos / (unsigned)a.page;   // below 2^32
+  const unsigned pos = (unsigned)first + (unsigned)t;
+  if (pos >= 0x80000000u) return -1;
+  const unsigned slot = a.by_page.div(pos);
   if (slot >= (unsigned)a.pages_per_seq) return -1;
   const int p = a.table[b * a.table_ld + slot];
   if ((unsigned)p >= (unsigned)a.num_pages) return -1;
@@ -74,123 +77,152 @@ __device__ __forceinline__ int kv_round(float x, float s, float inv) {
   return (int)n;
 }
 
+// Row r of a sequence: token r / H, head r % H. A thread has a few rows, a pass of the block apart, so that their loads are in flight together.
+constexpr int KV_WRITE_ROWS = 2, KV_READ_ROWS = 4;
+
 template <typename T, int KIND, int D>
 __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvArgs a) {
-  constexpr int G = D / 8;
+  constexpr int G = D / 8, PER = KV_THREADS / G, R = KV_WRITE_ROWS;
   const int lane = threadIdx.x % G;
-  const unsigned r = blockIdx.x * (KV_THREADS / G) + threadIdx.x / G;
+  const unsigned r0 = blockIdx.x * (PER * R) + threadIdx.x / G;
   const int b = blockIdx.y;
-  const int t = (int)(r / (unsigned)a.H), h = (int)(r - (unsigned)t * a.H);
   const int n = a.counts ? min(a.counts[b], a.T) : a.T;
-  const bool mine = t < n;
-  long row = -1;
-  float f[2][8];
-  if (mine) {
-    row = kv_row(a, b, t, h);
-    if (row < 0 && lane == 0) report_bad_index();
+  if ((int)(blockIdx.x * (PER * R) / (unsigned)a.H) >= n) return;
+  float f[R][2][8];
+  long row[R];
 #pragma unroll
-    for (int z = 0; z < 2; ++z) load8<T>((const T*)a.x[z] + b * a.sb[z] + t * a.st[z] + h * a.sh[z] + lane * 8, f[z]);
-  } else {
+  for (int i = 0; i < R; ++i) {
+    const unsigned r = r0 + i * PER;
+    const int t = (int)a.by_h.div(r), h = (int)(r - (unsigned)t * a.H);
+    row[i] = -1;
+    if (t < n) {
 #pragma unroll
-    for (int z = 0; z < 2; ++z)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[z][j] = 0.f;
-  }
-#pragma unroll
-  for (int z = 0; z < 2; ++z) {
-    if constexpr (KIND == KV_BF16) {
-      Vec16<bf16> v;
-      v.set(f[z]);
-      if (row >= 0) v.store((bf16*)a.pages[z] + row * D + lane * 8);
+      for (int z = 0; z < 2; ++z) load8<T>((const T*)a.x[z] + b * a.sb[z] + t * a.st[z] + h * a.sh[z] + lane * 8, f[i][z]);
+      row[i] = kv_row(a, b, t, h);
+      if (row[i] < 0 && lane == 0) report_bad_index();
     } else {
-      float big = 0.f;
-      bool wild = false;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        big = fmaxf(big, fabsf(f[z][j]));
-        wild |= (__float_as_uint(f[z][j]) & 0x7f800000u) == 0x7f800000u;
-      }
-      big = group_max<G>(wild ? __int_as_float(0x7f800000) : big);
-      wild = big > FLT_MAX;
-      const bool none = big < 7.888609052210118e-31f;   // 2^-100
-      float s, inv;
-      if (KIND == KV_INT8) {
-        s = __fdiv_rn(big, 127.f);
-        inv = __fdiv_rn(1.f, none ? 1.f : s);
-      } else {
-        // big = m 2^e with m in [1, 2); 448 = 1.75 x 2^8
-        const uint32_t u = __float_as_uint(big);
-        const int k = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u);
-        s = __int_as_float((k + 127) << 23);
-        inv = __int_as_float((127 - k) << 23);
-      }
-      uint32_t w[2] = {0u, 0u};
-      if (!none && !wild) {
-        if (KIND == KV_INT8) {
+      for (int z = 0; z < 2; ++z)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv_round(f[z][j], s, inv) & 0xffu) << (8 * (j & 3));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j += 2)
-            w[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[z][j] * inv, f[z][j + 1] * inv), __NV_SATFINITE, __NV_E4M3)
-                         << (8 * (j & 3));
-        }
-      }
-      if (row >= 0) {
-        *(uint2*)((uint8_t*)a.pages[z] + row * D + lane * 8) = make_uint2(w[0], w[1]);
-        if (lane == 0) a.scales[z][row] = wild ? __int_as_float(0x7fffffff) : none ? 0.f : s;
-      }
+        for (int j = 0; j < 8; ++j) f[i][z][j] = 0.f;
     }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      float (&x)[8] = f[i][z];
+      if constexpr (KIND == KV_BF16) {
+        Vec16<bf16> v;
+        v.set(x);
+        if (row[i] >= 0) v.store((bf16*)a.pages[z] + row[i] * D + lane * 8);
+      } else {
+        float big = 0.f;
+        bool wild = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          big = fmaxf(big, fabsf(x[j]));
+          wild |= (__float_as_uint(x[j]) & 0x7f800000u) == 0x7f800000u;
+        }
+        big = group_max<G>(wild ? __int_as_float(0x7f800000) : big);
+        wild = big > FLT_MAX;
+        const bool none = big < 7.888609052210118e-31f;   // 2^-100
+        float s, inv;
+        if (KIND == KV_INT8) {
+          s = __fdiv_rn(big, 127.f);
+          inv = __fdiv_rn(1.f, none ? 1.f : s);
+        } else {
+          // big = m 2^e with m in [1, 2); 448 = 1.75 x 2^8
+          const uint32_t u = __float_as_uint(big);
+          const int k = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u);
+          s = __int_as_float((k + 127) << 23);
+          inv = __int_as_float((127 - k) << 23);
+        }
+        uint32_t w[2] = {0u, 0u};
+        if (!none && !wild) {
+          if (KIND == KV_INT8) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv_round(x[j], s, inv) & 0xffu) << (8 * (j & 3));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+              w[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[j] * inv, x[j + 1] * inv), __NV_SATFINITE, __NV_E4M3)
+                           << (8 * (j & 3));
+          }
+        }
+        if (row[i] >= 0) {
+          *(uint2*)((uint8_t*)a.pages[z] + row[i] * D + lane * 8) = make_uint2(w[0], w[1]);
+          if (lane == 0) a.scales[z][row[i]] = wild ? __int_as_float(0x7fffffff) : none ? 0.f : s;
+        }
+      }
+    }
 }
 
 template <typename T, int KIND, int D>
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvArgs a) {
-  constexpr int G = D / 8;
+  constexpr int G = D / 8, PER = KV_THREADS / G, R = KV_READ_ROWS;
   const int lane = threadIdx.x % G;
-  const unsigned r = blockIdx.x * (KV_THREADS / G) + threadIdx.x / G;
+  const unsigned r0 = blockIdx.x * (PER * R) + threadIdx.x / G;
   const int b = blockIdx.y;
-  const int t = (int)(r / (unsigned)a.H), h = (int)(r - (unsigned)t * a.H);
-  if (t >= a.T) return;
   const int n = a.counts ? a.counts[b] : a.T;
-  long row = -1;
-  if (t < n) {
-    row = kv_row(a, b, t, h);
-    if (row < 0 && lane == 0) report_bad_index();
-  }
+  long row[R];
+  uint4 raw[R][2];
+  float sc[R][2];
 #pragma unroll
-  for (int z = 0; z < 2; ++z) {
-    float f[8] = {};
-    if (row >= 0) {
-      if constexpr (KIND == KV_BF16) {
-        load8<bf16>((const bf16*)a.pages[z] + row * D + lane * 8, f);
-      } else {
-        const uint2 w = __ldg((const uint2*)((const uint8_t*)a.pages[z] + row * D + lane * 8));
-        const float s = __ldg(a.scales[z] + row);
-        const uint32_t ws[2] = {w.x, w.y};
+  for (int i = 0; i < R; ++i) {
+    const unsigned r = r0 + i * PER;
+    const int t = (int)a.by_h.div(r), h = (int)(r - (unsigned)t * a.H);
+    row[i] = t < a.T && t < n ? kv_row(a, b, t, h) : -2;
+    if (row[i] == -1 && lane == 0) report_bad_index();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint8_t byte = (uint8_t)(ws[j >> 2] >> (8 * (j & 3)));
-          if (KIND == KV_INT8) f[j] = (float)(int8_t)byte * s;
-          else f[j] = __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3))) * s;
+    for (int z = 0; z < 2; ++z) {
+      raw[i][z] = make_uint4(0u, 0u, 0u, 0u);
+      sc[i][z] = 0.f;
+      if (row[i] >= 0) {
+        if constexpr (KIND == KV_BF16) {
+          raw[i][z] = __ldg((const uint4*)((const bf16*)a.pages[z] + row[i] * D + lane * 8));
+        } else {
+          const uint2 w = __ldg((const uint2*)((const uint8_t*)a.pages[z] + row[i] * D + lane * 8));
+          raw[i][z].x = w.x, raw[i][z].y = w.y;
+          sc[i][z] = __ldg(a.scales[z] + row[i]);
         }
       }
     }
-    T* y = (T*)a.y[z] + (((long)b * a.T + t) * a.H + h) * D + lane * 8;
-    if constexpr (sizeof(T) == 2) {
-      Vec16<T> v;
-      v.set(f);
-      v.store(y);
-    } else {
-      *(float4*)y = make_float4(f[0], f[1], f[2], f[3]);
-      *((float4*)y + 1) = make_float4(f[4], f[5], f[6], f[7]);
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const unsigned r = r0 + i * PER;
+    if (r >= (unsigned)a.T * (unsigned)a.H) break;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      float f[8];
+      const uint32_t ws[4] = {raw[i][z].x, raw[i][z].y, raw[i][z].z, raw[i][z].w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (KIND == KV_BF16) {
+          f[j] = __uint_as_float(j & 1 ? ws[j >> 1] & 0xffff0000u : ws[j >> 1] << 16);
+        } else {
+          const uint8_t byte = (uint8_t)(ws[j >> 2] >> (8 * (j & 3)));
+          if (KIND == KV_INT8) f[j] = (float)(int8_t)byte * sc[i][z];
+          else f[j] = __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3))) * sc[i][z];
+        }
+      }
+      T* y = (T*)a.y[z] + ((long)b * a.T * a.H + r) * D + lane * 8;
+      if constexpr (sizeof(T) == 2) {
+        Vec16<T> v;
+        v.set(f);
+        v.store(y);
+      } else {
+        *(float4*)y = make_float4(f[0], f[1], f[2], f[3]);
+        *((float4*)y + 1) = make_float4(f[4], f[5], f[6], f[7]);
+      }
     }
   }
 }
 
 template <typename T, int KIND>
 static int kv_launch(const KvArgs& a, int D, bool write, cudaStream_t st) {
-  const dim3 grid((unsigned)ceil_div((long)a.T * a.H, KV_THREADS / (D / 8)), (unsigned)a.B);
+  const dim3 grid((unsigned)ceil_div((long)a.T * a.H, KV_THREADS / (D / 8) * (write ? KV_WRITE_ROWS : KV_READ_ROWS)), (unsigned)a.B);
   if (write) {
     if (D == 64) kv_write_kernel<T, KIND, 64><<<grid, KV_THREADS, 0, st>>>(a);
     else kv_write_kernel<T, KIND, 128><<<grid, KV_THREADS, 0, st>>>(a);
@@ -235,7 +267,7 @@ TB_EXPORT int tb_kv_write(const void* k, const void* v, const long* strides, voi
   TB_ENSURE_DEVICE();
   if (B <= 0 || T <= 0) return 0;
   KvArgs a{{k, v}, {strides[0], strides[3]}, {strides[1], strides[4]}, {strides[2], strides[5]}, {nullptr, nullptr}, {k_pages, v_pages},
-           {k_scales, v_scales}, table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages};
+           {k_scales, v_scales}, table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages, FastDiv::of(H > 0 ? H : 1), FastDiv::of(page > 0 ? page : 1)};
   if (int r = kv_check(a, D, kind, dtype)) return r;
   const int N = dtype == 0 ? 8 : 4;
   for (int i = 0; i < 6; ++i)
@@ -251,7 +283,7 @@ TB_EXPORT int tb_kv_read(const void* k_pages, const void* v_pages, const float* 
   TB_ENSURE_DEVICE();
   if (B <= 0 || T <= 0) return 0;
   KvArgs a{{nullptr, nullptr}, {0, 0}, {0, 0}, {0, 0}, {yk, yv}, {(void*)k_pages, (void*)v_pages}, {(float*)k_scales, (float*)v_scales},
-           table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages};
+           table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages, FastDiv::of(H > 0 ? H : 1), FastDiv::of(page > 0 ? page : 1)};
   if (int r = kv_check(a, D, kind, dtype)) return r;
   if (!yk || !yv || (((uintptr_t)yk | (uintptr_t)yv) & 15)) TB_FAIL(TB_E_ARG, "kv cache: outputs must be 16-byte aligned");
   return dtype == 0 ? kv_dispatch<bf16>(a, D, kind, false, st) : kv_dispatch<float>(a, D, kind, false, st);

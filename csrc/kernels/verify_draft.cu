@@ -9,10 +9,12 @@
 // Either way the token that follows and the accepted ones are distributed as if they had been drawn from p one by one.
 //
 // The walk needs only p (and q) at the drafted tokens: T scalars, loaded at once. What is bound by memory is the row (or two) that
-// the next token is drawn from, by inversion: a cluster of eight CTAs shares a sequence's row, a warp sums one of 128 segments,
-// the sums meet over distributed shared memory, and the CTA whose segment holds u * total goes through it once more. All sums are
-// in 64 bits: a token next to a border of the cumulative sum is then the same whatever the order of adding.
+// the next token is drawn from, by inversion: a cluster of eight CTAs shares a sequence's row, a warp sums one segment and stores the
+// sum into the shared memory of all eight, and the CTA whose segment holds u * total goes through that once more (out of L2).
+// All sums are in 64 bits: a token next to a border of the cumulative sum is then the same whatever the order of adding.
 #include <cooperative_groups.h>
+
+#include <utility>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -22,11 +24,8 @@ namespace tb {
 namespace cg = cooperative_groups;
 
 constexpr int VD_CLUSTER = 8;
-constexpr int VD_THREADS = 512;
-constexpr int VD_WARPS = VD_THREADS / 32;
-constexpr int VD_SEGMENTS = VD_CLUSTER * VD_WARPS;
-static_assert(VD_SEGMENTS == 128, "pick_range() takes four sums a lane");
 constexpr int VD_MAX_NODES = 1024;
+constexpr int VD_MAX_CHUNKS = 64;
 constexpr int VD_UNROLL = 8;
 
 struct VerifyArgs {
@@ -75,7 +74,7 @@ __device__ __forceinline__ double mass_at(const Row& r, int c, int end) {
 }
 template <typename T>
 __device__ __forceinline__ double sum_range(const Row& r, int c0, int end, int lane) {
-  double sum = 0.0;
+  double part[4] = {0.0, 0.0, 0.0, 0.0}, sum = 0.0;
   int c = c0 + lane;
   for (; c + 32 * (VD_UNROLL - 1) < end; c += 32 * VD_UNROLL) {
     float p[VD_UNROLL], q[VD_UNROLL];
@@ -92,29 +91,32 @@ __device__ __forceinline__ double sum_range(const Row& r, int c0, int end, int l
     for (int i = 0; i < VD_UNROLL; ++i) {
       const int at = c + 32 * i - r.base;
       const bool gone = r.out && ((r.out[at >> 5] >> (at & 31)) & 1u);
-      sum += gone ? 0.0 : mass_of(p[i], q[i]);
+      part[i & 3] += gone ? 0.0 : mass_of(p[i], q[i]);
     }
   }
+  sum = (part[0] + part[1]) + (part[2] + part[3]);
   for (; c < end; c += 32) sum += mass_at<T>(r, c, end);
   return warp_sum_d(sum);
 }
 
-// Of the masses of up to 128 consecutive ranges (lane l of a warp holds m[0..3] of ranges 4l .. 4l + 3): the range in which the running
-// sum passes `target` (`scale`: target * total) (rounding can leave none: then the last that has any mass; -1: no mass at all), and the sum
+// Of the masses of 32 N consecutive ranges (lane l of a warp holds m[0 .. N-1] of ranges N l ..): the range in which the running sum,
+// `before` at the first, passes `target` (rounding can leave none: then the last that has any mass; -1: no mass at all), and the sum
 // before it.
-__device__ __forceinline__ void pick_range(const double (&m)[4], double first, double& target, bool scale, int lane, int& hit, double& before) {
-  const double own = (m[0] + m[1]) + (m[2] + m[3]);
+template <int N>
+__device__ __forceinline__ void pick_range(const double (&m)[N], double target, int lane, int& hit, double& before) {
+  double own = 0.0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) own += m[i];
   const double incl = warp_scan_d(own, lane);
   double at = __shfl_up_sync(0xffffffffu, incl, 1);
-  at = first + (lane ? at : 0.0);
-  if (scale) target *= __shfl_sync(0xffffffffu, incl, 31);
+  at = before + (lane ? at : 0.0);
   int last = -1, over = -1;
   double b_last = 0.0, b_over = 0.0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N; ++i) {
     const double next = at + m[i];
     if (m[i] > 0.0) {
-      last = 4 * lane + i;
+      last = N * lane + i;
       b_last = at;
       if (over < 0 && next > target) {
         over = last;
@@ -129,14 +131,17 @@ __device__ __forceinline__ void pick_range(const double (&m)[4], double first, d
   before = __shfl_sync(0xffffffffu, past ? b_over : b_last, src);
 }
 
-template <typename T>
-__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS) verify_kernel(const VerifyArgs a, int words) {
+template <typename T, int VD_WARPS>
+__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_WARPS * 32, VD_WARPS <= 8 ? 4 : 1) verify_kernel(const VerifyArgs a, int words) {
+  constexpr int VD_THREADS = VD_WARPS * 32, VD_SEGMENTS = VD_CLUSTER * VD_WARPS, PER_LANE = VD_SEGMENTS / 32;
   extern __shared__ uint32_t out_bits[];                 // this CTA's columns
   __shared__ float mass[VD_MAX_NODES], dmass[VD_MAX_NODES];
   __shared__ int parent[VD_MAX_NODES], token[VD_MAX_NODES];
-  __shared__ double seg[VD_WARPS], sub[VD_WARPS], s_target, s_before;
-  __shared__ int s_last, s_kids, s_hit;
+  __shared__ float num[VD_MAX_NODES];
+  __shared__ double seg[2][VD_SEGMENTS];
+  __shared__ int s_last, s_kids;
   cg::cluster_group cluster = cg::this_cluster();
+  auto started = cluster.barrier_arrive();               // waited for before the first store into another CTA
   const int rank = (int)cluster.block_rank(), b = blockIdx.x / VD_CLUSTER;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = min(max(a.counts ? a.counts[b] : a.T, 1), a.T);
@@ -144,6 +149,7 @@ __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS)
   const T* draft = a.draft ? (const T*)a.draft + b * a.db : nullptr;
   const long* par = a.parents ? a.parents + b * a.parents_ld : nullptr;
   const float* u = a.uniforms + (long)b * a.T;
+  const float last_u = u[a.T - 1];
 
   for (int i = tid; i < n; i += VD_THREADS) {
     const long tk = a.tokens[(long)b * a.T + i];
@@ -153,6 +159,7 @@ __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS)
     parent[i] = ok ? (int)pr : -1;
     token[i] = ok ? (int)tk : -1;
     mass[i] = ok ? to_f<T>(probs[pr * a.pt + tk]) : 0.f;
+    num[i] = u[i];
     dmass[i] = ok && draft ? to_f<T>(draft[pr * a.dt + tk]) : 0.f;
   }
   for (int i = tid; i < words; i += VD_THREADS) out_bits[i] = 0;
@@ -176,11 +183,11 @@ __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS)
       if (draft) {
         if (cur + 1 < n) {
           kids = true;
-          if (parent[cur + 1] == cur && (double)u[cur] * (double)dmass[cur + 1] < (double)mass[cur + 1]) step = cur + 1;
+          if (parent[cur + 1] == cur && (double)num[cur] * (double)dmass[cur + 1] < (double)mass[cur + 1]) step = cur + 1;
         }
       } else {
         double low = 0.0;
-        const double x = (double)u[cur];
+        const double x = (double)num[cur];
         for (int j0 = cur + 1; j0 < n; j0 += 32) {
           const int j = j0 + lane;
           unsigned hit = __ballot_sync(0xffffffffu, j < n && parent[j] == cur);
@@ -227,22 +234,16 @@ __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS)
   for (int pass = 0; pass < 2; ++pass) {
     const int c0 = min(base + warp * len, a.V), c1 = min(c0 + len, a.V);
     const double s = sum_range<T>(row, c0, c1, lane);
-    if (lane == 0) seg[warp] = s;
+    if (!pass) cluster.barrier_wait(std::move(started));
+    // each pass has sums of its own: nobody's are written again while they are read
+    if (lane < VD_CLUSTER) cluster.map_shared_rank(seg[pass], lane)[rank * VD_WARPS + warp] = s;
     cluster.sync();
-    if (warp == 0) {                                     // every CTA does the same with the same numbers
-      double m[4];
+    double m[PER_LANE], own = 0.0;                       // every warp does the same with the same numbers
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m[i] = cluster.map_shared_rank(seg, (4 * lane + i) / VD_WARPS)[(4 * lane + i) % VD_WARPS];
-      target = (double)u[a.T - 1];
-      pick_range(m, 0.0, target, true, lane, hit, at);
-      if (lane == 0) {
-        s_hit = hit;
-        s_target = target;
-        s_before = at;
-      }
-    }
-    cluster.sync();                                      // nobody's sums are written again, or its CTA gone, while they are read
-    hit = s_hit;
+    for (int i = 0; i < PER_LANE; ++i) own += m[i] = seg[pass][PER_LANE * lane + i];
+    at = 0.0;
+    target = (double)last_u * warp_sum_d(own);
+    pick_range<PER_LANE>(m, target, lane, hit, at);
     if (hit >= 0) break;
     row.q = nullptr;                                     // the draft covers all of p: draw from p itself
     row.out = nullptr;
@@ -252,39 +253,54 @@ __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS)
     return;
   }
   if (hit / VD_WARPS != rank) return;
-  target = s_target;
-  at = s_before;
-  const int c0 = hit * len, c1 = min(c0 + len, a.V);
-  const int part = ((len / 32 + VD_WARPS - 1) / VD_WARPS) * 32;
-  {
-    const int s0 = min(c0 + warp * part, c1), s1 = min(s0 + part, c1);
-    const double s = sum_range<T>(row, s0, s1, lane);
-    if (lane == 0) sub[warp] = s;
+  // the segment in chunks of 256 columns: the warps sum them, then one takes the chunk, eight neighbouring columns to a lane
+  __shared__ double chunk[VD_MAX_CHUNKS];
+  const int c0 = hit * len, c1 = min(c0 + len, a.V), wide = max(256, ((len / 32 + VD_MAX_CHUNKS - 1) / VD_MAX_CHUNKS) * 32);
+  const int chunks = (c1 - c0 + wide - 1) / wide;
+  for (int k = warp; k < VD_MAX_CHUNKS; k += VD_WARPS) {
+    const double s = k < chunks ? sum_range<T>(row, c0 + k * wide, min(c0 + (k + 1) * wide, c1), lane) : 0.0;
+    if (lane == 0) chunk[k] = s;
   }
   __syncthreads();
   if (warp) return;
   {
-    double m[4];
+    double m[VD_MAX_CHUNKS / 32];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = 4 * lane + i < VD_WARPS ? sub[4 * lane + i] : 0.0;
-    const double first = at;
-    pick_range(m, first, target, false, lane, hit, at);
+    for (int i = 0; i < VD_MAX_CHUNKS / 32; ++i) m[i] = chunk[VD_MAX_CHUNKS / 32 * lane + i];
+    pick_range<VD_MAX_CHUNKS / 32>(m, target, lane, hit, at);
     if (hit < 0) hit = 0;                                // not reached: the segment has mass
   }
-  const int s0 = min(c0 + hit * part, c1), s1 = min(s0 + part, c1);
   int found = -1;
-  for (int c = s0; c < s1; c += 32) {
-    const double m = mass_at<T>(row, c + lane, s1);
-    const double sum = at + warp_scan_d(m, lane);
-    const unsigned any = __ballot_sync(0xffffffffu, m > 0.0), over = __ballot_sync(0xffffffffu, m > 0.0 && sum > target);
-    if (over) {
-      found = c + __ffs(over) - 1;
-      break;
-    }
-    if (any) found = c + 31 - __clz(any);
-    at = __shfl_sync(0xffffffffu, sum, 31);
+  const int e1 = min(c0 + (hit + 1) * wide, c1);
+  for (int e0 = c0 + hit * wide; e0 < e1; e0 += 256) {
+    double m[8], next = at, own = 0.0;
+    int col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) own += m[i] = mass_at<T>(row, e0 + 8 * lane + i, e1);
+    next = at + warp_sum_d(own);
+    pick_range<8>(m, target, lane, col, at);
+    if (col >= 0) found = e0 + col;
+    if (next > target) break;
+    at = next;
   }
   if (lane == 0) a.next[b] = found;
+}
+
+template <typename T, int WARPS>
+static int verify_sized(const VerifyArgs& a, cudaStream_t st) {
+  const int segments = VD_CLUSTER * WARPS;
+  const int len = (((a.V + segments - 1) / segments) + 31) & ~31;
+  const int words = WARPS * len / 32;                    // a bit for each of a CTA's columns: 2 KB at V = 128 000, 64 KB at 2^22
+  static std::atomic<uint64_t> done{0};
+  if (int r = smem_opt_in(done, verify_kernel<T, WARPS>, 72 * 1024)) return r;
+  verify_kernel<T, WARPS><<<a.B * VD_CLUSTER, WARPS * 32, words * 4, st>>>(a, words);
+  TB_CUDA_CHECK(cudaGetLastError());
+  return 0;
+}
+// Few sequences: as many threads as a CTA has, so that a row is loaded in one go. Many: CTAs of which four fit an SM.
+template <typename T>
+static int verify_launch(const VerifyArgs& a, cudaStream_t st) {
+  return a.B * VD_CLUSTER <= sm_count() ? verify_sized<T, 32>(a, st) : verify_sized<T, 8>(a, st);
 }
 
 }  // namespace tb
@@ -305,17 +321,5 @@ TB_EXPORT int tb_verify_draft(const void* probs, const void* draft, const long* 
   if (dtype != 0 && dtype != 1) TB_FAIL(TB_E_ARG, "verify: bf16 or fp32");
   if (B > 0x7fffffff / VD_CLUSTER || V > (1 << 22)) TB_FAIL(TB_E_TOO_LARGE, "verify: at most 2^22 tokens in the vocabulary");
   VerifyArgs a{probs, draft, pb, pt, db, dt, tokens, parents, parents_ld, uniforms, counts, accepted, path, next, B, T, V};
-  const int len = (((V + VD_SEGMENTS - 1) / VD_SEGMENTS) + 31) & ~31;
-  const int words = VD_WARPS * len / 32;                 // 2 KB at V = 128 000, 64 KB at 2^22
-  const int bytes = words * 4;
-  static std::atomic<uint64_t> done16{0}, done32{0};
-  if (dtype == 0) {
-    if (int r = smem_opt_in(done16, verify_kernel<bf16>, 72 * 1024)) return r;
-    verify_kernel<bf16><<<B * VD_CLUSTER, VD_THREADS, bytes, st>>>(a, words);
-  } else {
-    if (int r = smem_opt_in(done32, verify_kernel<float>, 72 * 1024)) return r;
-    verify_kernel<float><<<B * VD_CLUSTER, VD_THREADS, bytes, st>>>(a, words);
-  }
-  TB_CUDA_CHECK(cudaGetLastError());
-  return 0;
+  return dtype == 0 ? verify_launch<bf16>(a, st) : verify_launch<float>(a, st);
 }

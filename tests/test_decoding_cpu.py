@@ -159,7 +159,7 @@ def _attention_args():
     (dict(k_scales=None), ValueError), (dict(v_scales=torch.ones(5, 2, 8)), ValueError), (dict(k_scales=torch.ones(5, 2, 16).double()), ValueError),
     (dict(page_table=torch.zeros(3, 2, dtype=torch.int32)), ValueError), (dict(page_table=torch.zeros(2, 2)), ValueError),
     (dict(start=torch.zeros(3, dtype=torch.int32)), ValueError), (dict(start=torch.zeros(2)), ValueError), (dict(counts=torch.zeros(1, dtype=torch.int32)), ValueError),
-    (dict(tree_mask=torch.ones(3, 3)), ValueError), (dict(tree_mask=torch.ones(2, 2, dtype=torch.bool)), ValueError), (dict(max_len=-1), ValueError),
+    (dict(tree_mask=torch.ones(3, 3)), ValueError), (dict(tree_mask=torch.ones(2, 2, dtype=torch.bool)), ValueError), (dict(max_len=-1), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=math.nan), ValueError),
     (dict(q=torch.zeros(2, 3, 4, 64, requires_grad=True)), RuntimeError),
     (dict(k_pages=torch.zeros(5, 2, 16, 64).to(torch.uint8), v_pages=torch.zeros(5, 2, 16, 64).to(torch.uint8)), TypeError),
     (dict(k_pages=torch.zeros(5, 2, 16, 64).bfloat16(), v_pages=torch.zeros(5, 2, 16, 64).bfloat16()), ValueError),

@@ -266,7 +266,9 @@ def _random_tree(T, seed):
 
 SHAPES = [(1, 1, 1, 1, 64, 16, [0]), (2, 1, 4, 4, 128, 16, [15, 16]), (3, 1, 8, 2, 128, 32, [17, 1, 700]), (5, 1, 12, 12, 64, 64, [100, 0, 63, 64, 65]),
           (1, 1, 8, 1, 128, 16, [9001]), (2, 7, 8, 2, 128, 16, [333, 5]), (3, 13, 2, 2, 64, 48, [40, 0, 95]), (2, 48, 4, 4, 128, 32, [500, 31]),
-          (2, 27, 16, 4, 128, 16, [129, 1000]), (1, 64, 8, 1, 64, 128, [2000]), (2, 33, 3, 1, 64, 16, [16, 250]), (150, 1, 2, 1, 64, 16, [3, 200, 31, 0])]
+          (2, 27, 16, 4, 128, 16, [129, 1000]), (1, 64, 8, 1, 64, 128, [2000]), (2, 33, 3, 1, 64, 16, [16, 250]), (150, 1, 2, 1, 64, 16, [3, 200, 31, 0]),
+          # many tiles and units to a CTA, ends anywhere in them
+          (4, 8, 32, 8, 128, 64, [5000, 3001, 8064, 127]), (6, 40, 16, 16, 64, 16, [2900, 4096, 77, 5003, 640, 3333]), (1, 150, 4, 2, 128, 32, [3100])]
 
 
 @pytest.mark.parametrize("dtype", [BF16, torch.int8, E4M3])
@@ -300,11 +302,12 @@ def test_cache_attention_rows_that_see_nothing(dtype, G):
 
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
 @pytest.mark.parametrize("G", [1, 8, 32])
-def test_cache_attention_what_is_not_seen_does_not_reach_a_row(dtype, G):
+@pytest.mark.parametrize("contexts", [[37, 12], [30037, 20012]])
+def test_cache_attention_what_is_not_seen_does_not_reach_a_row(dtype, G, contexts):
     """NaN behind the end of a sequence, and infinities and NaN in new tokens that only some rows see."""
     from torsh_b200.ops.kv_cache import kv_cache_attention
     T, D = 6, 128
-    q, kp, vp, ks, vs, table, start = _case(2, T, G, 1, D, 16, [37, 12], dtype)
+    q, kp, vp, ks, vs, table, start = _case(2, T, G, 1, D, 16, contexts, dtype)
     clean = kp.clone(), vp.clone()
     for b in range(2):
         for pos in range(int(start[b]) + T, table.shape[1] * 16):           # never written

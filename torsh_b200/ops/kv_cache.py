@@ -25,7 +25,7 @@ from ._dispatch import F, I, L, P, call, fn, kernel_ok, on_device
 
 _WRITE = [P] * 8 + [L, P, P] + [I] * 9 + [P]
 _READ = [P] * 7 + [L, P, P] + [I] * 9 + [P]
-_ATTN = [P] * 7 + [L, P, P, P, L, L, P, P] + [I] * 10 + [F, P]
+_ATTN = [P] * 7 + [L, P, P, P, L, L, P, P] + [I] * 10 + [F, P, P]
 _KINDS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
 _TINY = 2.0 ** -100
 _CODES = (torch.int8, torch.float8_e4m3fn)
@@ -295,6 +295,8 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     if counts is not None:
         counts = _per_sequence("kv_cache_attention", "counts", counts, B, q.device)
     scale = 1.0 / math.sqrt(D) if scale is None else scale
+    if not 0 <= scale < math.inf:
+        raise ValueError(f"kv_cache_attention: scale is a number that is not negative, got {scale}")
     limit = 0x7FFF0000 if max_len is None else min(max_len, 0x7FFF0000)
     if q.dtype == torch.bfloat16 and _kernel_pages(k_pages) and _kernel_pages(v_pages) and page % 16 == 0 and page > 0:
         out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
@@ -313,7 +315,7 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
             ws = _workspace(B, T, Hq, H, D, q.device)
             call("tb_cache_attention", _ATTN, q.data_ptr(), strides, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
                  table.data_ptr(), table.stride(0), start.data_ptr(), _ptr(counts), _ptr(tree_mask), mb, mt, out.data_ptr(), ws.data_ptr(),
-                 B, T, Hq, H, D, page, table.shape[1], num_pages, limit, _KINDS[k_pages.dtype], scale, nv.stream_ptr())
+                 B, T, Hq, H, D, page, table.shape[1], num_pages, limit, _KINDS[k_pages.dtype], scale, nv.status_ptr(q.device), nv.stream_ptr())
         return out
     return _attention_plain(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, limit)
 
