@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
   const uint32_t ring_u = ca_smem(ring);
 
   const Deal deal = deal_tiles<CA_THREADS, CA_TILE, CA_WARPS>(a, scratch);
+  release_join();
   zero_empty<D, CA_THREADS>(a);
   if (deal.first >= deal.last) {
     if (threadIdx.x == 0) a.plan[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -521,6 +522,7 @@ __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const Ca
   constexpr int N = D / 32;                            // columns of a lane
   __shared__ float buf[CJ_WARPS][D];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 p = a.plan[blockIdx.x];
   if (p.w == 0 || p.z == 0 || p.z > p.w) return;       // nothing; a unit's beginning; not its first cut
   const int b = p.x, hr = p.y, per = p.w;
@@ -573,10 +575,16 @@ int cache_attn_join(const CacheAttnArgs& a, int D, int tile, cudaStream_t st) {
   // one sequence cuts few units into many parts, many sequences many units into few
   const long units = (long)a.B * a.Hkv * a.row_tiles;
   const int share = units * 8 >= a.grid ? 1 : CJ_WARPS;
-  const dim3 grid((unsigned)a.grid, (unsigned)((a.part_rows * share + CJ_WARPS - 1) / CJ_WARPS));
-  if (D == 64) cache_attn_join_kernel<64><<<grid, CJ_WARPS * 32, 0, st>>>(a, tile, share);
-  else cache_attn_join_kernel<128><<<grid, CJ_WARPS * 32, 0, st>>>(a, tile, share);
-  TB_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps the attention kernel: 2 us
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)a.grid, (unsigned)((a.part_rows * share + CJ_WARPS - 1) / CJ_WARPS));
+  cfg.blockDim = dim3(CJ_WARPS * 32);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  TB_CUDA_CHECK(D == 64 ? cudaLaunchKernelEx(&cfg, cache_attn_join_kernel<64>, a, tile, share) : cudaLaunchKernelEx(&cfg, cache_attn_join_kernel<128>, a, tile, share));
   return 0;
 }
 

@@ -158,6 +158,9 @@ __device__ __forceinline__ long rows_at(const CacheAttnArgs& a, int b, int h, in
   return ((long)p * a.Hkv + h) * a.page + (tile - slot * a.page_tiles) * 16;
 }
 
+// The kernel that joins the parts may be set up while this one runs; it waits for this one's end before it reads anything.
+__device__ __forceinline__ void release_join() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Sequences that see nothing: their rows are zeros.
 template <int D, int THREADS>
 __device__ __forceinline__ void zero_empty(const CacheAttnArgs& a) {

@@ -17,15 +17,20 @@
 //   warp 12    issues the products (warps 13-15: none; 512 threads take no more of the SM than 416, for 128 registers each)
 // TMEM: S and P of even and of odd tiles 128 columns each (P takes the first half of the S it came from), then O of either.
 //
-// 8-bit scales: scores are multiplied by the key's; P carries the value's, and the power of two that P is relative to (the largest
-// scale so far) is part of the running reference: R = max + log2(unit), so sums and O stay relative to one number.
+// 8-bit scales: scores are multiplied by the key's scale in fp32. The value's goes into the halves, relative to a power of two for each
+// 32 tokens (what a loading warp has of a tile): one rounding of 2^-12 for the scale and one for the product, as P has one, where
+// carrying it in P cost the softmax 32 more loads of broadcast scales a tile (3.5 us instead of 2). P of those tokens is shifted by the
+// quotient of their power of two and the largest so far (`unit`), which O is relative to.
 #include "cache_attention.cuh"
 #include "sm100.cuh"
+
+#include <type_traits>
 
 namespace tb {
 
 constexpr int CT_THREADS = 512;
 constexpr int CT_TILE = 128;
+constexpr int CT_UNIT = -80;   // log2 of the smallest power of two that values are relative to: sums times its inverse stay in range
 
 template <int D, int KIND> struct CtShape {
   static constexpr bool HALVES = KIND != CA_BF16;
@@ -36,9 +41,10 @@ template <int D, int KIND> struct CtShape {
   static constexpr int RAW = HALVES ? 2 * CT_TILE * D : 0;
   static constexpr int RAWS = HALVES ? 2 : 0;
   static constexpr int Q_OFF = 0, K_OFF = TILE, V_OFF = K_OFF + KST * TILE, RAW_OFF = V_OFF + VST * TILE;
-  // per value stage: scales of keys and of values, the four producer warps' largest value scale, and their tokens with odd values
-  static constexpr int SIDE_OFF = RAW_OFF + RAWS * RAW, SCALES = HALVES ? 2 * CT_TILE * 4 : 0, SIDE = SCALES + 32;
-  static constexpr int BAR_OFF = SIDE_OFF + VST * SIDE;
+  // per value stage: scales of keys, the four loading warps' powers of two, and their tokens with odd values
+  static constexpr int SIDE_OFF = RAW_OFF + RAWS * RAW, SCALES = HALVES ? CT_TILE * 4 : 0, SIDE = SCALES + 32;
+  static constexpr int TOP_OFF = SIDE_OFF + VST * SIDE;             // largest |q| of either half of a row
+  static constexpr int BAR_OFF = TOP_OFF + (HALVES ? 2 * CT_TILE * 4 : 0);
   // k_full[2], k_empty[2], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done[2], side_full[2], q_full
   static constexpr int NBARS = 21;
   static constexpr int ALLOC = BAR_OFF + NBARS * 8 + 8;
@@ -75,6 +81,7 @@ __device__ __forceinline__ void ct_odd_values(const CacheAttnArgs& a, uint32_t t
       const int pos = pos0 + w * 32 + __ffs(rest) - 1;
       const long row = rows_at(a, b, h, pos);
       const bool mine = live && row >= 0 && sees(a, b, t, pos, s);
+      const bool wild = KIND != CA_BF16 && row >= 0 && (__float_as_uint(__ldg(a.v_scales + row + (pos & 15))) & 0x7f800000u) == 0x7f800000u;
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
@@ -86,7 +93,7 @@ __device__ __forceinline__ void ct_odd_values(const CacheAttnArgs& a, uint32_t t
           if (row >= 0) {
             const long at = (row + (pos & 15)) * D + c + i;
             if (KIND == CA_BF16) v = __bfloat162float(((const bf16*)a.v_pages)[at]);
-            else v = (((const uint8_t*)a.v_pages)[at] & 0x7f) == 0x7f ? __int_as_float(0x7fffffff) : 0.f;
+            else if (wild || (KIND == CA_E4M3 && (((const uint8_t*)a.v_pages)[at] & 0x7f) == 0x7f)) v = __int_as_float(0x7fffffff);
           }
           const bool odd = (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
           if (mine && odd) o[i] = __float_as_uint(__uint_as_float(o[i]) + v);
@@ -152,6 +159,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
 
   // the deal uses the (not yet used) place of Q
   const Deal deal = deal_tiles<CT_THREADS, CT_TILE, 1>(a, (int*)smem);
+  release_join();
   zero_empty<D, CT_THREADS>(a);
   if (deal.first >= deal.last) {
     if (threadIdx.x == 0) a.plan[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -282,24 +290,23 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       if (++w.tile >= w.end) walk_next<CT_TILE>(a, w, 0);
       if (n + 1 < total) seek();
     };
-    // halves of the warp's codes of a tile
-    auto convert = [&](const uint8_t* raw, uint8_t* dst, bool odd_too, int first_new, uint32_t& odd) {
+    // halves of the warp's codes of a tile, keys as they are, values times their token's `scale` (lane: token 32 pw + lane)
+    auto convert = [&](auto is_value, const uint8_t* raw, uint8_t* dst, float scale, int first_new, uint32_t& odd) {
+      constexpr bool VALUE = decltype(is_value)::value;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const int ch = j * 32 + lane, tok = (pw * 2 + i) * 16 + ch / (D / 16), q = ch % (D / 16);
           uint4 v = *(const uint4*)(raw + (pw * 2 + i) * 16 * D + ch * 16);
-          if (KIND == CA_E4M3 && odd_too && tok >= first_new) {
+          if (VALUE && KIND == CA_E4M3 && tok >= first_new) {
             uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int z = 0; z < 32; z += 8)
-                if (((x[k] >> z) & 0x7fu) == 0x7fu) {
-                  x[k] &= ~(0xffu << z);
-                  odd |= 1u << (tok & 31);
-                }
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t nan = __vcmpeq4(x[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              x[k] &= ~nan;
+              if (nan) odd |= 1u << (tok & 31);
+            }
             v = make_uint4(x[0], x[1], x[2], x[3]);
           }
           uint4 lo, hi;
@@ -307,6 +314,14 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
           halves_of<KIND>(v.y, lo.z, lo.w);
           halves_of<KIND>(v.z, hi.x, hi.y);
           halves_of<KIND>(v.w, hi.z, hi.w);
+          if (VALUE) {
+            const __half2 sc = __float2half2_rn(__shfl_sync(0xffffffffu, scale, tok & 31));
+            auto times = [&](uint32_t& h) {
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h), sc);
+              h = *reinterpret_cast<const uint32_t*>(&y);
+            };
+            times(lo.x), times(lo.y), times(lo.z), times(lo.w), times(hi.x), times(hi.y), times(hi.z), times(hi.w);
+          }
           *(uint4*)(dst + ct_at(tok, 2 * q)) = lo;
           *(uint4*)(dst + ct_at(tok, 2 * q + 1)) = hi;
         }
@@ -321,19 +336,23 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       if (HALVES) {
         const uint8_t* raw = smem + L::RAW_OFF + (n & 1) * L::RAW;
         mbar_wait(&k_empty[kst], ((n / KST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
-        convert(raw, smem + L::K_OFF + kst * L::TILE, false, 0, odd);
+        convert(std::false_type{}, raw, smem + L::K_OFF + kst * L::TILE, 0.f, 0, odd);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[kst]);
+        // a scale that is no number, of a new token, is for the rows that see it (ct_odd_values)
+        const bool wild = (__float_as_uint(vs) & 0x7f800000u) == 0x7f800000u && pw * 32 + lane >= first_new;
+        if (wild) odd = 1u << lane;
+        const float big = warp_max(wild ? 0.f : vs);
+        const int unit = min(max((int)((__float_as_uint(big) + 0x7fffffu) >> 23) - 127, CT_UNIT), 127);
+        const int ex = (int)(__float_as_uint(vs) >> 23) - unit;       // of the scale relative to the unit, at most 127; a context's NaN stays one
+        const float rel = wild || ex < 127 - 25 ? 0.f : ex > 127 ? vs : __uint_as_float((__float_as_uint(vs) & 0x7fffffu) | ((uint32_t)ex << 23));
         mbar_wait(&v_empty[vst], ((n / VST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
         ((float*)side)[pw * 32 + lane] = ks;
-        ((float*)side)[CT_TILE + pw * 32 + lane] = vs;
-        const float top = warp_max(vs);
-        if (lane == 0) ((float*)(side + L::SCALES))[pw] = top;
+        if (lane == 0) ((int*)(side + L::SCALES))[pw] = unit;
         __syncwarp();
         if (lane == 0) mbar_arrive(&side_full[vst]);                  // the softmax does not wait for the values
-        if (edge) convert(raw + CT_TILE * D, vt, true, first_new, odd);
-        else convert(raw + CT_TILE * D, vt, false, 0, odd);
+        convert(std::true_type{}, raw + CT_TILE * D, vt, rel, first_new, odd);
       } else {
         if (edge) {
 #pragma unroll 1
@@ -355,10 +374,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
             }
         }
       }
-      if (KIND != CA_INT8) {
-        if (edge) odd = __reduce_or_sync(0xffffffffu, odd);
-        if (lane == 0) ((uint32_t*)(side + L::SCALES + 16))[pw] = odd;
-      }
+      if (edge) odd = __reduce_or_sync(0xffffffffu, odd);
+      if (lane == 0) ((uint32_t*)(side + L::SCALES + 16))[pw] = odd;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -392,52 +409,47 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
     int n = 0;                                       // the tile of the run that comes next
     while (true) {
       const int r = (w.hr - w.h * a.row_tiles) * CT_TILE + row, t = r / a.G;
-      const bool inside = t < a.T, live = t < w.s.count;
+      const bool live = t < w.s.count;
       const bool busy = __any_sync(0xffffffffu, live);   // a warp whose rows are all spare only keeps the others' pace
       float f = a.scale_log2;
       {
         // each group brings half of a row's columns; 8-bit caches need the whole row's largest value first
         const bf16* qp = a.q + w.b * a.qb + (long)t * a.qt + (long)(w.h * a.G + r - t * a.G) * a.qh;
-        float down = 1.f;
-        if (HALVES) {
-          float big = 0.f;
-          if (live) {
-#pragma unroll 1
-            for (int i0 = 0; i0 < D / 8; i0 += 8) {
-              uint4 v[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = __ldg((const uint4*)qp + i0 + i);
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(bf16_lo(v[i].x)), fabsf(bf16_hi(v[i].x))), fmaxf(fabsf(bf16_lo(v[i].y)), fabsf(bf16_hi(v[i].y)))),
-                                       fmaxf(fmaxf(fabsf(bf16_lo(v[i].z)), fabsf(bf16_hi(v[i].z))), fmaxf(fabsf(bf16_lo(v[i].w)), fabsf(bf16_hi(v[i].w))))));
-            }
-          }
-          const uint32_t ex = __float_as_uint(big) >> 23;
-          const bool plain = ex == 0 || ex > 253;
-          down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
-          if (!plain) f *= __uint_as_float(ex << 23);
-        }
-        f = fmaxf(f, 1e-30f);   // -inf (not seen) times a factor of zero would be no number
         uint4 v[D / 16];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) v[i] = live ? __ldg((const uint4*)qp + group * (D / 16) + i) : make_uint4(0u, 0u, 0u, 0u);
+        if (HALVES) {
+          float big = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          if (HALVES) {
+          for (int i = 0; i < D / 16; ++i)
+            big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(bf16_lo(v[i].x)), fabsf(bf16_hi(v[i].x))), fmaxf(fabsf(bf16_lo(v[i].y)), fabsf(bf16_hi(v[i].y)))),
+                                   fmaxf(fmaxf(fabsf(bf16_lo(v[i].z)), fabsf(bf16_hi(v[i].z))), fmaxf(fabsf(bf16_lo(v[i].w)), fabsf(bf16_hi(v[i].w))))));
+          float* tops = (float*)(smem + L::TOP_OFF);
+          tops[group * 128 + row] = big;
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          big = fmaxf(big, tops[(group ^ 1) * 128 + row]);
+          const uint32_t ex = __float_as_uint(big) >> 23;
+          const bool plain = ex == 0 || ex > 253;
+          const float down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
+          if (!plain) f *= __uint_as_float(ex << 23);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
             v[i].x = ct_pack<true>(bf16_lo(v[i].x) * down, bf16_hi(v[i].x) * down);
             v[i].y = ct_pack<true>(bf16_lo(v[i].y) * down, bf16_hi(v[i].y) * down);
             v[i].z = ct_pack<true>(bf16_lo(v[i].z) * down, bf16_hi(v[i].z) * down);
             v[i].w = ct_pack<true>(bf16_lo(v[i].w) * down, bf16_hi(v[i].w) * down);
           }
-          *(uint4*)(smem + L::Q_OFF + ct_at(row, group * (D / 16) + i)) = v[i];
         }
+        f = fmaxf(f, 1e-30f);   // -inf (not seen) times a factor of zero would be no number
+        if (!HALVES) asm volatile("bar.sync 1, 256;" ::: "memory");   // the last unit's output has left Q's place (8 bits: the barrier above)
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) *(uint4*)(smem + L::Q_OFF + ct_at(row, group * (D / 16) + i)) = v[i];
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // P = 2^(x f - ref), x the score (times the key's scale): ref = max f + log2(unit) - OFFSET
+      // P = 2^(x f - m f + OFFSET + shift), x the score (times the key's scale), shift that of the value's 32 tokens; l sums it unshifted
       float m = -INFINITY, l = 0.f;
-      int unit = HALVES ? -60 : 0;
+      int unit = HALVES ? CT_UNIT : 0;
       uint32_t odd[4] = {0u, 0u, 0u, 0u};
       int odd_pos = 0;
       bool any_tile = false;
@@ -457,7 +469,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         // Two passes over S, 64 columns at a time: the maximum, then P over the columns that have been read
         if (busy) {
           uint32_t v[2][32];
-          auto fetch = [&](int half) {
+          float now = m, also = -INFINITY;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
             tmem_ld32(ts + half * 64, v[0]);
             tmem_ld32(ts + half * 64 + 32, v[1]);
             tmem_wait_ld();
@@ -480,11 +494,13 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
                 for (int i = 0; i < 32; ++i)
                   if (!(((uint32_t)(c ? seen >> 32 : seen) >> i) & 1u)) v[c][i] = 0xff800000u;
             }
-          };
-          float now = m, also = -INFINITY;
-#pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            fetch(half);
+            if (HALVES || edge) {   // the second pass takes them as they are now
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                tmem_st16(ts + half * 64 + c * 32, reinterpret_cast<const uint32_t(&)[16]>(v[c][0]));
+                tmem_st16(ts + half * 64 + c * 32 + 16, reinterpret_cast<const uint32_t(&)[16]>(v[c][16]));
+              }
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -494,50 +510,54 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
               }
           }
           now = fmaxf(now, also);
-          int now_unit = unit;
+          int now_unit = unit, units[4];
           if (HALVES) {
-            const float* tops = (const float*)(side + L::SCALES);
-            const float big = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            now_unit = max(unit, (int)((__float_as_uint(big) + 0x7fffffu) >> 23) - 127);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              units[c] = ((const int*)(side + L::SCALES))[c];
+              now_unit = max(now_unit, units[c]);
+            }
+            tmem_wait_st();
+          } else if (edge) {
+            tmem_wait_st();
           }
           grow = now > m || now_unit > unit;
           // O of no tile yet, or of tiles that the row saw nothing of, is zero (or not there): any finite factor does
-          if (grow) alpha = m == -INFINITY ? 1.f : exp2f((m - now) * f + (float)(unit - now_unit));
+          if (grow) {
+            const float less = m == -INFINITY ? 1.f : exp2f((m - now) * f);
+            alpha = HALVES ? less * exp2f((float)(unit - now_unit)) : less;
+            l *= less;
+          }
           m = now;
           unit = now_unit;
-          const float ref = (m == -INFINITY ? 0.f : m * f) + (float)unit - OFFSET;
-          float2 l2 = make_float2(0.f, 0.f), l3 = l2;
-          const float2 f2 = make_float2(f, f), r2 = make_float2(-ref, -ref);
+          const float ref = (m == -INFINITY ? 0.f : m * f) - OFFSET;
+          const float2 f2 = make_float2(f, f);
 #pragma unroll 1
           for (int half = 0; half < 2; ++half) {
-            fetch(half);
+            tmem_ld32(ts + half * 64, v[0]);
+            tmem_ld32(ts + half * 64 + 32, v[1]);
+            tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+              const float shift = HALVES ? (float)max((half ? units[2 + c] : units[c]) - unit, -100) : 0.f;
+              const float2 r2 = make_float2(shift - ref, shift - ref);
+              float2 l2 = make_float2(0.f, 0.f), l3 = l2;
               uint32_t pk[16];
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), f2, r2);
                 const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), f2, r2);
-                float2 e = make_float2(exp2f(x.x), exp2f(x.y)), g = make_float2(exp2f(y.x), exp2f(y.y));
+                const float2 e = make_float2(exp2f(x.x), exp2f(x.y)), g = make_float2(exp2f(y.x), exp2f(y.y));
                 l2 = __fadd2_rn(l2, e);
                 l3 = __fadd2_rn(l3, g);
-                if (HALVES) {
-                  const float4 v4 = *(const float4*)(side + (CT_TILE + (half * 2 + c) * 32 + i) * 4);
-                  e = __fmul2_rn(e, make_float2(v4.x, v4.y));
-                  g = __fmul2_rn(g, make_float2(v4.z, v4.w));
-                }
                 pk[i / 2] = ct_pack<HALVES>(e.x, e.y);
                 pk[i / 2 + 1] = ct_pack<HALVES>(g.x, g.y);
               }
-              if (HALVES && edge) {   // a value's scale that is no number stays with the rows that see it
-                const uint32_t seen = (uint32_t)((half ? vis_hi : vis_lo) >> (32 * c));
-#pragma unroll
-                for (int i = 0; i < 16; ++i) pk[i] &= ((seen >> (2 * i)) & 1u ? 0xffffu : 0u) | ((seen >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
-              }
               tmem_st16(tp + (half * 2 + c) * 16, pk);
+              const float sum = (l2.x + l2.y) + (l3.x + l3.y);
+              l += HALVES ? sum * exp2f(-shift) : sum;
             }
           }
-          l = l * alpha + ((l2.x + l2.y) + (l3.x + l3.y));
           if (odd[0] | odd[1] | odd[2] | odd[3]) ct_odd_values<D, KIND>(a, to, odd, w.b, w.h, min(t, a.T - 1), live, odd_pos, w.s);
           if (any_tile && __any_sync(0xffffffffu, grow)) {
 #pragma unroll 1
@@ -555,12 +575,10 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
             }
           }
         }
-        if (KIND != CA_INT8) {
-          if (edge) mbar_wait(&v_full[st], (n / VST) & 1, abort_flag, status, TB_ERR_WAIT_FULL);
+        if (edge) mbar_wait(&v_full[st], (n / VST) & 1, abort_flag, status, TB_ERR_WAIT_FULL);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) odd[i] = edge ? ((const uint32_t*)(side + L::SCALES + 16))[i] : 0u;
-          odd_pos = pos0;
-        }
+        for (int i = 0; i < 4; ++i) odd[i] = edge ? ((const uint32_t*)(side + L::SCALES + 16))[i] : 0u;
+        odd_pos = pos0;
         any_tile = true;
         tmem_wait_st();
         tc_fence_before();
@@ -576,6 +594,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
       }
       const float mine_r = m == -INFINITY ? m : m * f + (float)unit;
+      if (HALVES) l *= exp2f(-(float)unit);             // relative to the same power of two as O
       // all products of the unit have read Q when both groups are here
       tc_fence_before();
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -594,35 +613,44 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       const int slot = slot_of(blockIdx.x, w.head > 0);
       const float inv = all > 0.f || all != all ? 1.f / all : 0.f;   // a row that sees nothing: zeros
       const long at = (long)slot * a.part_rows + row;
-      const bool part = !whole && row < a.part_rows;
-      if (part && group == 0) *(float2*)(a.part_ml + at * 2) = make_float2(top, all);
-      bf16* orow = a.out + (((long)w.b * a.T + (inside ? t : 0)) * a.Hq + w.h * a.G + (inside ? r - t * a.G : 0)) * D;
+      if (!whole && row < a.part_rows && group == 0) *(float2*)(a.part_ml + at * 2) = make_float2(top, all);
+      // this group's half of the columns, 16 at a time: through shared memory (Q's place), so that four lanes store 64 bytes of a row
       const uint32_t to0 = tmem_base + TM_O + lane_off;
+      float4* turn = (float4*)(smem + L::Q_OFF) + warp * 128;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D / 2; c0 += 32) {           // this group's half of the columns
-        const int c = group * (D / 2) + c0;
-        float y[32];
+      for (int c = group * (D / 2); c < (group + 1) * (D / 2); c += 16) {
         if (busy) {
-          uint32_t o0[32], o1[32];
-          tmem_ld32(to0 + c, o0);
-          tmem_ld32(to0 + 128 + c, o1);
+          uint32_t o0[16], o1[16];
+          tmem_ld16(to0 + c, o0);
+          tmem_ld16(to0 + 128 + c, o1);
           tmem_wait_ld();
+          float y[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = (has0 ? __uint_as_float(o0[i]) * f0 : 0.f) + (has1 ? __uint_as_float(o1[i]) * f1 : 0.f);
+          for (int i = 0; i < 16; ++i) {
+            y[i] = (has0 ? __uint_as_float(o0[i]) * f0 : 0.f) + (has1 ? __uint_as_float(o1[i]) * f1 : 0.f);
+            y[i] = live ? (whole ? y[i] * inv : y[i]) : 0.f;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) turn[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          __syncwarp();
         }
-        if (part) {
 #pragma unroll
-          for (int g = 0; g < 8; ++g) ((float4*)(a.part_o + at * D + c))[g] = live ? make_float4(y[g * 4], y[g * 4 + 1], y[g * 4 + 2], y[g * 4 + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-        } else if (whole && inside) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float* u = y + g * 8;
-            ((uint4*)(orow + c))[g] = live ? make_uint4(pack_bf16x2(u[0] * inv, u[1] * inv), pack_bf16x2(u[2] * inv, u[3] * inv),
-                                                        pack_bf16x2(u[4] * inv, u[5] * inv), pack_bf16x2(u[6] * inv, u[7] * inv))
-                                           : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 4; ++i) {
+          const int rl = i * 8 + (lane >> 2), rr = (warp & 3) * 32 + rl, piece = lane & 3;
+          const float4 z = busy ? turn[rl * 4 + (piece ^ ((rl >> 1) & 3))] : make_float4(0.f, 0.f, 0.f, 0.f);
+          if (!whole) {
+            if (rr < a.part_rows) *(float4*)(a.part_o + ((long)slot * a.part_rows + rr) * D + c + piece * 4) = z;
+          } else {
+            const int r2 = (w.hr - w.h * a.row_tiles) * CT_TILE + rr, t2 = r2 / a.G;
+            if (t2 < a.T) {
+              bf16* op = a.out + (((long)w.b * a.T + t2) * a.Hq + w.h * a.G + r2 - t2 * a.G) * D + c + piece * 4;
+              *(uint2*)op = make_uint2(pack_bf16x2(z.x, z.y), pack_bf16x2(z.z, z.w));
+            }
           }
         }
       }
+      __syncwarp();
       tc_fence_before();
       if (!walk_next<CT_TILE>(a, w, 0)) break;
     }
