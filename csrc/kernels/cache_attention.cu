@@ -130,13 +130,14 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
   Walk ld;
   walk_begin<CA_TILE>(a, ld, deal, warp);
   bool more = true;
-  long next_row = -1;
+  PageRef next{-1, 0};
   auto seek = [&]() {
     while (more && ld.tile >= ld.end) more = walk_next<CA_TILE>(a, ld, warp);
-    if (more) next_row = rows_at(a, ld.b, ld.h, ld.tile * CA_TILE);
+    if (more) next = page_ref(a, ld.b, ld.tile * CA_TILE);
   };
   auto load = [&](int stage) {
     if (more) {
+      const long next_row = row_of(a, next, ld.h);
       const int live = next_row < 0 ? 0 : min(ld.s.len - ld.tile * CA_TILE, CA_TILE);
       if (next_row < 0 && lane == 0) report_bad_index();
       const long row = max(next_row, 0l);

@@ -149,13 +149,18 @@ __device__ __forceinline__ bool walk_next(const CacheAttnArgs& a, Walk& w, int o
   return true;
 }
 
-// Rows of 16 tokens of a page, tokens `pos` .. of sequence b: the row of the first in the pool, -1 where the table names no page of it.
-__device__ __forceinline__ long rows_at(const CacheAttnArgs& a, int b, int h, int pos) {
+// Where 16 tokens lie, tokens `pos` .. of a sequence. In two steps, so that the table's answer is not waited for where it is asked:
+// the page that the table names and the place in it, later the row of the first token in the pool (-1: no page of the pool).
+struct PageRef {
+  int page, place;
+};
+__device__ __forceinline__ PageRef page_ref(const CacheAttnArgs& a, int b, int pos) {
   const int tile = pos >> 4;
   const int slot = a.page_shift >= 0 ? tile >> a.page_shift : tile / a.page_tiles;
-  const int p = __ldg(a.table + (long)b * a.table_ld + slot);
-  if ((unsigned)p >= (unsigned)a.num_pages) return -1;
-  return ((long)p * a.Hkv + h) * a.page + (tile - slot * a.page_tiles) * 16;
+  return {__ldg(a.table + (long)b * a.table_ld + slot), (tile - slot * a.page_tiles) * 16};
+}
+__device__ __forceinline__ long row_of(const CacheAttnArgs& a, const PageRef& r, int h) {
+  return (unsigned)r.page < (unsigned)a.num_pages ? ((long)r.page * a.Hkv + h) * a.page + r.place : -1;
 }
 
 // The kernel that joins the parts may be set up while this one runs; it waits for this one's end before it reads anything.

@@ -79,7 +79,7 @@ __device__ __forceinline__ void ct_odd_values(const CacheAttnArgs& a, uint32_t t
 #pragma unroll 1
     for (uint32_t rest = w == 0 ? words[0] : w == 1 ? words[1] : w == 2 ? words[2] : words[3]; rest; rest &= rest - 1) {
       const int pos = pos0 + w * 32 + __ffs(rest) - 1;
-      const long row = rows_at(a, b, h, pos);
+      const long row = row_of(a, page_ref(a, b, pos), h);
       const bool mine = live && row >= 0 && sees(a, b, t, pos, s);
       const bool wild = KIND != CA_BF16 && row >= 0 && (__float_as_uint(__ldg(a.v_scales + row + (pos & 15))) & 0x7f800000u) == 0x7f800000u;
 #pragma unroll 1
@@ -247,24 +247,38 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
     // of the tile last asked for: the scales of token 32 pw + lane, and the first token that is a new one (CT_TILE: none)
     float ks = 0.f, vs = 0.f;
     int first_new = CT_TILE;
-    long next[2];
+    PageRef next[2];
     auto seek = [&]() {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int pos = w.tile * CT_TILE + (pw * 2 + i) * 16;
-        next[i] = pos < w.s.len ? rows_at(a, w.b, w.h, pos) : -2;
+        if (pos < w.s.len) next[i] = page_ref(a, w.b, pos);
       }
     };
+    // The 16-byte piece of 32 j + lane: token of 16, and piece of it. Of 128-byte rows (8 bits, D = 128) eight neighbouring lanes have four
+    // pieces of two tokens, whose halves then go to all eight 16-byte places of the 128-byte swizzle; in order they met two by two.
+    auto piece_of = [&](int j, int& tok, int& q) {
+      if (HALVES && D == 128) {
+        tok = j * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 2) & 1);
+        q = (lane & 3) | ((lane >> 3) & 1) << 2;
+      } else {
+        const int ch = j * 32 + lane;
+        tok = ch / (D * L::ES / 16);
+        q = ch % (D * L::ES / 16);
+      }
+    };
+    auto raw_at = [](int tok, int q) { return tok * D + ((D == 128 ? q ^ ((tok & 1) << 2) : q) << 4); };
     auto copy = [&](const void* pages, uint32_t dst, const long (&rows)[2], int pos0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int tok0 = (pw * 2 + i) * 16;
         const int live = rows[i] < 0 ? 0 : min(w.s.len - pos0 - tok0, 16);
-        const uint8_t* src = (const uint8_t*)pages + max(rows[i], 0l) * (D * L::ES) + lane * 16;
+        const uint8_t* src = (const uint8_t*)pages + max(rows[i], 0l) * (D * L::ES);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const int ch = j * 32 + lane, tok = ch / (D * L::ES / 16);
-          ct_copy16(dst + (HALVES ? tok0 * D + ch * 16 : ct_at(tok0 + tok, ch % (D / 8))), src + j * 512, tok < live);
+          int tok, q;
+          piece_of(j, tok, q);
+          ct_copy16(dst + (HALVES ? raw_at(tok0 + tok, q) : ct_at(tok0 + tok, q)), src + tok * (D * L::ES) + q * 16, tok < live);
         }
       }
       ct_commit();
@@ -272,20 +286,26 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
     auto ask = [&](int n) {
       const int pos0 = w.tile * CT_TILE;
       first_new = pos0 + CT_TILE > min(w.s.start, w.s.len) ? max(w.s.start - pos0, 0) : CT_TILE;
-      if ((next[0] == -1 || next[1] == -1) && lane == 0) report_bad_index();
+      long rows[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool there = pos0 + (pw * 2 + i) * 16 < w.s.len;
+        rows[i] = there ? row_of(a, next[i], w.h) : -1;
+        if (there && rows[i] < 0 && lane == 0) report_bad_index();
+      }
       if (HALVES) {
         const int pos = pos0 + pw * 32 + lane;
-        const long row = lane >= 16 ? next[1] : next[0];
+        const long row = lane >= 16 ? rows[1] : rows[0];
         const bool live = row >= 0 && pos < w.s.len;
         ks = live ? __ldg(a.k_scales + row + (lane & 15)) : 0.f;
         vs = live ? __ldg(a.v_scales + row + (lane & 15)) : 0.f;
-        copy(a.k_pages, smem_base + L::RAW_OFF + (n & 1) * L::RAW, next, pos0);
-        copy(a.v_pages, smem_base + L::RAW_OFF + (n & 1) * L::RAW + CT_TILE * D, next, pos0);
+        copy(a.k_pages, smem_base + L::RAW_OFF + (n & 1) * L::RAW, rows, pos0);
+        copy(a.v_pages, smem_base + L::RAW_OFF + (n & 1) * L::RAW + CT_TILE * D, rows, pos0);
       } else {
         mbar_wait(&k_empty[n % KST], ((n / KST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
-        copy(a.k_pages, smem_base + L::K_OFF + (n % KST) * L::TILE, next, pos0);
+        copy(a.k_pages, smem_base + L::K_OFF + (n % KST) * L::TILE, rows, pos0);
         mbar_wait(&v_empty[n % VST], ((n / VST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
-        copy(a.v_pages, smem_base + L::V_OFF + (n % VST) * L::TILE, next, pos0);
+        copy(a.v_pages, smem_base + L::V_OFF + (n % VST) * L::TILE, rows, pos0);
       }
       if (++w.tile >= w.end) walk_next<CT_TILE>(a, w, 0);
       if (n + 1 < total) seek();
@@ -297,8 +317,10 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const int ch = j * 32 + lane, tok = (pw * 2 + i) * 16 + ch / (D / 16), q = ch % (D / 16);
-          uint4 v = *(const uint4*)(raw + (pw * 2 + i) * 16 * D + ch * 16);
+          int tok, q;
+          piece_of(j, tok, q);
+          tok += (pw * 2 + i) * 16;
+          uint4 v = *(const uint4*)(raw + raw_at(tok, q));
           if (VALUE && KIND == CA_E4M3 && tok >= first_new) {
             uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
