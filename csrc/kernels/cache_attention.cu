@@ -515,8 +515,9 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
   ca_wait<0>();
 }
 
-// Joins the parts of the units that the deal has cut. Blocks x look at the unit that CTA x began with: if that is its first cut, they
-// join it. `share` warps have a row between them, and its parts.
+// Joins the parts of the units that the deal has cut. Blocks x are either units, or CTAs of the attention kernel and look at the unit that
+// the CTA began with: if that is its first cut, they join it (whichever is fewer: a block that finds nothing to do still costs a launch
+// of its own, and 4736 of them took 5 us). `share` warps have a row between them, and its parts.
 constexpr int CJ_WARPS = 8;
 template <int D>
 __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const CacheAttnArgs a, int tile, int share) {
@@ -524,16 +525,27 @@ __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const Ca
   __shared__ float buf[CJ_WARPS][D];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 p = a.plan[blockIdx.x];
-  if (p.w == 0 || p.z == 0 || p.z > p.w) return;       // nothing; a unit's beginning; not its first cut
-  const int b = p.x, hr = p.y, per = p.w;
+  int b, hr, per, first;
+  if (a.before) {
+    const int units = a.Hkv * a.row_tiles;
+    b = blockIdx.x / units, hr = blockIdx.x - b * units;
+    per = a.plan[0].w;
+  } else {
+    const int4 p = a.plan[blockIdx.x];
+    if (p.w == 0 || p.z == 0 || p.z > p.w) return;     // nothing; a unit's beginning; not its first cut
+    b = p.x, hr = p.y, per = p.w;
+    first = blockIdx.x * per - p.z;
+  }
+  const SeqLen s = seq_len(a, b);
+  const int nt = (s.len + tile - 1) / tile;
+  if (a.before) first = a.before[b] + hr * nt;
+  if (nt == 0) return;                                 // zeros already
+  const int c0 = first / per, c1 = (first + nt - 1) / per;
+  if (c0 == c1) return;                                // whole: written already
   const int h = a.row_tiles == 1 ? hr : hr / a.row_tiles;
   const int r = blockIdx.y * (CJ_WARPS / share) + warp / share, sub = warp % share;
   const int row = (hr - h * a.row_tiles) * a.part_rows + r, t = row / a.G;
   const bool mine = r < a.part_rows && t < a.T;
-  const SeqLen s = seq_len(a, b);
-  const int nt = (s.len + tile - 1) / tile;
-  const int c0 = blockIdx.x - 1, c1 = (blockIdx.x * per - p.z + nt - 1) / per;
   float top = -INFINITY, all = 0.f, y[N] = {};
   if (mine) {
     for (int k = c0 + lane; k <= c1; k += 32) {
@@ -572,15 +584,17 @@ __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const Ca
   for (int i = 0; i < N; i += 2) *(uint32_t*)(op + i) = t < s.count ? pack2<false>(y[i] * norm, y[i + 1] * norm) : 0u;
 }
 
+static long ca_units(const CacheAttnArgs& a) { return (long)a.B * a.Hkv * a.row_tiles; }
+
 int cache_attn_join(const CacheAttnArgs& a, int D, int tile, cudaStream_t st) {
   // one sequence cuts few units into many parts, many sequences many units into few
-  const long units = (long)a.B * a.Hkv * a.row_tiles;
+  const long units = ca_units(a);
   const int share = units * 8 >= a.grid ? 1 : CJ_WARPS;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps the attention kernel: 2 us
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a.grid, (unsigned)((a.part_rows * share + CJ_WARPS - 1) / CJ_WARPS));
+  cfg.gridDim = dim3((unsigned)(a.before ? units : a.grid), (unsigned)((a.part_rows * share + CJ_WARPS - 1) / CJ_WARPS));
   cfg.blockDim = dim3(CJ_WARPS * 32);
   cfg.stream = st;
   cfg.attrs = &early;
@@ -595,6 +609,7 @@ static int cache_attn_launch(CacheAttnArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   if (int r = smem_opt_in(done, cache_attn_kernel<D, KIND, NT>, S::SMEM)) return r;
   a.grid = S::OCC * sm_count();
+  if (ca_units(a) > a.grid) a.before = nullptr;
   cache_attn_kernel<D, KIND, NT><<<a.grid, CA_THREADS, S::SMEM, st>>>(a);
   TB_CUDA_CHECK(cudaGetLastError());
   return cache_attn_join(a, D, CA_TILE, st);
@@ -635,49 +650,63 @@ int tb_set_check_word_cache_attention(int* word) {
 TB_EXPORT long tb_cache_attention_workspace(int B, int T, int Hq, int Hkv, int D) {
   if (ensure_device() || Hkv <= 0) return -1;
   const long rows = (long)T * (Hq / Hkv), slots = ca_slots(rows > CA_MAX_ROWS);
-  return slots * ca_part_rows(rows) * (D * 4 + 8) + slots / 2 * 16;
+  return slots * ca_part_rows(rows) * (D * 4 + 8) + slots / 2 * (16 + 4);
 }
 
 // q [B, T, Hq, D] bf16 (strides in elements, multiples of 8; 16-byte aligned), out contiguous. ws: tb_cache_attention_workspace() bytes,
 // 16-byte aligned, used by this call alone.
-TB_EXPORT int tb_cache_attention(const void* q, const long* q_strides, const void* k_pages, const void* v_pages, const float* k_scales,
-                                 const float* v_scales, const int* table, long table_ld, const int* start, const int* counts,
-                                 const uint8_t* mask, long mask_b, long mask_t, void* out, void* ws, int B, int T, int Hq, int Hkv,
-                                 int D, int page, int pages_per_seq, int num_pages, int max_len, int kind, float scale, int* status, cudaStream_t st) {
+struct CacheAttnCall {
+  const void* q;
+  long qb, qt, qh;
+  const void *k_pages, *v_pages;
+  const float *k_scales, *v_scales;
+  const int* table;
+  long table_ld;
+  const int *start, *counts;
+  const uint8_t* mask;
+  long mask_b, mask_t;
+  void *out, *ws;
+  long B, T, Hq, Hkv, D, page, pages_per_seq, num_pages, max_len, kind;
+  int* status;
+  double scale;
+};
+TB_EXPORT int tb_cache_attention(const CacheAttnCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();
-  if (B <= 0 || T <= 0 || Hq <= 0) return 0;
-  if (!q || !out || !ws || !k_pages || !v_pages || !table || !start || (kind != CA_BF16 && (!k_scales || !v_scales)))
+  const long D = c->D, page = c->page, rows = c->Hkv > 0 ? c->T * (c->Hq / c->Hkv) : 0;
+  const int kind = (int)c->kind;
+  if (c->B <= 0 || c->T <= 0 || c->Hq <= 0) return 0;
+  if (!c->q || !c->out || !c->ws || !c->k_pages || !c->v_pages || !c->table || !c->start || (kind != CA_BF16 && (!c->k_scales || !c->v_scales)))
     TB_FAIL(TB_E_ARG, "cache attention: null pointer");
   if (D != 64 && D != 128) TB_FAIL(TB_E_ARG, "cache attention: head dim 64 or 128");
-  if (Hkv <= 0 || Hq % Hkv || kind < 0 || kind > 2) TB_FAIL(TB_E_ARG, "cache attention: query heads must be a multiple of the cache's");
-  if (page <= 0 || page % CA_TILE || num_pages < 0 || pages_per_seq < 0 || max_len < 0) TB_FAIL(TB_E_ARG, "cache attention: pages of a multiple of %d tokens", CA_TILE);
-  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)ws | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15 || q_strides[0] % 8 || q_strides[1] % 8 || q_strides[2] % 8)
+  if (c->Hkv <= 0 || c->Hq % c->Hkv || c->kind < 0 || c->kind > 2) TB_FAIL(TB_E_ARG, "cache attention: query heads must be a multiple of the cache's");
+  if (page <= 0 || page % CA_TILE || c->num_pages < 0 || c->pages_per_seq < 0 || c->max_len < 0) TB_FAIL(TB_E_ARG, "cache attention: pages of a multiple of %d tokens", CA_TILE);
+  if (((uintptr_t)c->q | (uintptr_t)c->out | (uintptr_t)c->ws | (uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15 || c->qb % 8 || c->qt % 8 || c->qh % 8)
     TB_FAIL(TB_E_ARG, "cache attention: 16-byte aligned rows");
-  if (kind != CA_BF16 && (((uintptr_t)k_scales | (uintptr_t)v_scales) & 15)) TB_FAIL(TB_E_ARG, "cache attention: 16-byte aligned scales");
+  if (kind != CA_BF16 && (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 15)) TB_FAIL(TB_E_ARG, "cache attention: 16-byte aligned scales");
+  if (c->B > 0x7fffffff || c->Hq > 0x7fffffff || rows > 0x7fffff00l || page > 0x7fff0000l || c->num_pages > 0x7fffffff || c->pages_per_seq > 0x7fff0000l)
+    TB_FAIL(TB_E_TOO_LARGE, "cache attention: too much for one call");
   CacheAttnArgs a{};
-  a.q = (const bf16*)q, a.qb = q_strides[0], a.qt = q_strides[1], a.qh = q_strides[2];
-  a.k_pages = k_pages, a.v_pages = v_pages, a.k_scales = k_scales, a.v_scales = v_scales;
-  a.table = table, a.table_ld = table_ld, a.start = start, a.counts = counts;
-  a.mask = mask, a.mask_b = mask_b, a.mask_t = mask_t, a.out = (bf16*)out;
-  a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.page = page, a.num_pages = num_pages;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  const long rows = (long)T * a.G;
+  a.q = (const bf16*)c->q, a.qb = c->qb, a.qt = c->qt, a.qh = c->qh;
+  a.k_pages = c->k_pages, a.v_pages = c->v_pages, a.k_scales = c->k_scales, a.v_scales = c->v_scales;
+  a.table = c->table, a.table_ld = c->table_ld, a.start = c->start, a.counts = c->counts;
+  a.mask = c->mask, a.mask_b = c->mask_b, a.mask_t = c->mask_t, a.out = (bf16*)c->out;
+  a.B = (int)c->B, a.T = (int)c->T, a.Hq = (int)c->Hq, a.Hkv = (int)c->Hkv, a.G = a.Hq / a.Hkv, a.page = (int)page, a.num_pages = (int)c->num_pages;
+  a.scale_log2 = (float)(c->scale * 1.4426950408889634);
   const bool tc = rows > CA_MAX_ROWS;
   const int nt = ca_row_blocks(rows);
   const int per_tile = tc ? 128 : 8 * nt;
   a.row_tiles = (int)((rows + per_tile - 1) / per_tile);
-  a.page_tiles = page / CA_TILE;
+  a.page_tiles = (int)(page / CA_TILE);
   a.page_shift = (a.page_tiles & (a.page_tiles - 1)) ? -1 : __builtin_ctz((unsigned)a.page_tiles);
-  const long held = (long)pages_per_seq * page;
-  a.limit = (int)(held < max_len ? held : max_len);
-  const long tiles = ((long)a.limit + CA_TILE - 1) / CA_TILE * B * Hkv * a.row_tiles;
-  if (rows > 0x7fffff00l || tiles > 0x7fff0000l || a.limit > 0x7fff0000l || (long)B * Hkv * a.row_tiles > 0x7fff0000l)
-    TB_FAIL(TB_E_TOO_LARGE, "cache attention: too much for one call");
+  const long held = c->pages_per_seq * page, limit = held < c->max_len ? held : c->max_len;
+  a.limit = (int)limit;
+  if (limit > 0x7fff0000l || (double)(limit + CA_TILE) / CA_TILE * (double)ca_units(a) > 2e9) TB_FAIL(TB_E_TOO_LARGE, "cache attention: too much for one call");
   const long slots = ca_slots(tc);
   a.part_rows = ca_part_rows(rows);
-  a.part_o = (float*)ws;
+  a.part_o = (float*)c->ws;
   a.part_ml = a.part_o + slots * a.part_rows * D;
   a.plan = (int4*)(a.part_ml + slots * a.part_rows * 2);
-  if (tc) return cache_attn_tc(a, D, kind, status, st);
+  a.before = (int*)(a.plan + slots / 2);               // there are at most as many sequences as units, and units as CTAs, where it is used
+  if (tc) return cache_attn_tc(a, (int)D, kind, c->status, st);
   return D == 64 ? cache_attn_kind<64>(a, kind, nt, st) : cache_attn_kind<128>(a, kind, nt, st);
 }

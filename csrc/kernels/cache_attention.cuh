@@ -22,6 +22,7 @@ struct CacheAttnArgs {
   bf16* out;                   // [B, T, Hq, D] contiguous
   float *part_o, *part_ml;     // partial results, [slot][row][D] and [slot][row] of (maximum, sum): see slot_of()
   int4* plan;                  // of each CTA: the sequence, head and row tile, and tile that it begins with, and the tiles of a CTA (0: it has none)
+  int* before;                 // the tiles in front of each sequence; null: the parts are looked for CTA by CTA
   int B, T, Hq, Hkv, G, page, page_tiles, page_shift, num_pages, row_tiles, grid;   // page_shift: log2 of a page's tiles, or -1
   int part_rows;               // rows of a slot of partial results
   int limit;                   // tokens of a sequence that the table can name, or fewer
@@ -85,6 +86,7 @@ __device__ __forceinline__ Deal deal_tiles(const CacheAttnArgs& a, int* scratch)
     int total;
     const int before = all + block_prefix<THREADS>(n, scratch, total);
     if (b0 == 0) keep_n = n, keep_before = before;
+    if (a.before && blockIdx.x == 0 && b < a.B) a.before[b] = before;
     all += total;
   }
   d.per = max((all + a.grid - 1) / a.grid, 1);

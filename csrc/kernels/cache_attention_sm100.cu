@@ -697,6 +697,7 @@ static int cache_attn_tc_launch(const CacheAttnArgs& a, int* status, cudaStream_
 
 int cache_attn_tc(CacheAttnArgs& a, int D, int kind, int* status, cudaStream_t st) {
   a.grid = sm_count();
+  if ((long)a.B * a.Hkv * a.row_tiles > a.grid) a.before = nullptr;
   if (D == 64) {
     if (kind == CA_BF16) return cache_attn_tc_launch<64, CA_BF16>(a, status, st);
     return kind == CA_INT8 ? cache_attn_tc_launch<64, CA_INT8>(a, status, st) : cache_attn_tc_launch<64, CA_E4M3>(a, status, st);

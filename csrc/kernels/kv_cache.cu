@@ -237,8 +237,6 @@ static int kv_launch(const KvArgs& a, int D, bool write, cudaStream_t st) {
 static int kv_check(const KvArgs& a, int D, int kind, int dtype) {
   if (D != 64 && D != 128) TB_FAIL(TB_E_ARG, "kv cache: head dim 64 or 128");
   if (kind < 0 || kind > 2 || (dtype != 0 && dtype != 1)) TB_FAIL(TB_E_ARG, "kv cache: pages in bf16, int8 or e4m3, rows in bf16 or fp32");
-  if (a.page <= 0 || a.num_pages < 0 || a.pages_per_seq < 0 || a.H <= 0) TB_FAIL(TB_E_ARG, "kv cache: bad sizes");
-  if (a.B > 65535 || (long)a.T * a.H > 0x7fffff00l) TB_FAIL(TB_E_TOO_LARGE, "kv cache: at most 65535 sequences and 2^31 rows a sequence in one call");
   for (int z = 0; z < 2; ++z)
     if (!a.pages[z] || ((uintptr_t)a.pages[z] & 15) || (kind != KV_BF16 && !a.scales[z])) TB_FAIL(TB_E_ARG, "kv cache: pages must be 16-byte aligned and 8-bit pages have scales");
   if (!a.table) TB_FAIL(TB_E_ARG, "kv cache: no page table");
@@ -260,31 +258,46 @@ int tb_set_check_word_kv_cache(int* word) {
   return 0;
 }
 
-// k, v [B, T, H, D]: strides (batch, token, head) in elements, multiples of 16 bytes; rows t >= counts[b] are left out.
-TB_EXPORT int tb_kv_write(const void* k, const void* v, const long* strides, void* k_pages, void* v_pages, float* k_scales,
-                          float* v_scales, const int* table, long table_ld, const int* start, const int* counts, int B, int T,
-                          int H, int D, int page, int pages_per_seq, int num_pages, int kind, int dtype, cudaStream_t st) {
-  TB_ENSURE_DEVICE();
-  if (B <= 0 || T <= 0) return 0;
-  KvArgs a{{k, v}, {strides[0], strides[3]}, {strides[1], strides[4]}, {strides[2], strides[5]}, {nullptr, nullptr}, {k_pages, v_pages},
-           {k_scales, v_scales}, table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages, FastDiv::of(H > 0 ? H : 1), FastDiv::of(page > 0 ? page : 1)};
+// write: x[0], x[1] = k, v [B, T, H, D] with strides (batch, token, head) in elements, multiples of 16 bytes; rows t >= counts[b] are left out.
+// read: x[0], x[1] [B, T, H, D] contiguous, written; rows t >= counts[b], and rows that no page holds, are zeros.
+struct KvCall {
+  void* x[2];
+  long strides[6];
+  void* pages[2];
+  float* scales[2];
+  const int* table;
+  long table_ld;
+  const int *start, *counts;
+  long B, T, H, D, page, pages_per_seq, num_pages, kind, dtype;
+};
+static int kv_call(const KvCall* c, bool write, cudaStream_t st) {
+  if (c->B <= 0 || c->T <= 0) return 0;
+  if (c->B > 65535 || c->H <= 0 || c->T > 0x7fffff00l || c->H > 0x7fffff00l || c->T * c->H > 0x7fffff00l)
+    TB_FAIL(TB_E_TOO_LARGE, "kv cache: at most 65535 sequences and 2^31 rows a sequence in one call");
+  if (c->page <= 0 || c->page > 0x7fffff00l || c->num_pages < 0 || c->num_pages > 0x7fffffff || c->pages_per_seq < 0 || c->pages_per_seq > 0x7fffffff)
+    TB_FAIL(TB_E_ARG, "kv cache: bad sizes");
+  KvArgs a{};
+  for (int z = 0; z < 2; ++z) {
+    if (write) a.x[z] = c->x[z], a.sb[z] = c->strides[3 * z], a.st[z] = c->strides[3 * z + 1], a.sh[z] = c->strides[3 * z + 2];
+    else a.y[z] = c->x[z];
+    a.pages[z] = c->pages[z], a.scales[z] = c->scales[z];
+  }
+  a.table = c->table, a.start = c->start, a.counts = c->counts, a.table_ld = c->table_ld;
+  a.B = (int)c->B, a.T = (int)c->T, a.H = (int)c->H, a.page = (int)c->page, a.pages_per_seq = (int)c->pages_per_seq, a.num_pages = (int)c->num_pages;
+  a.by_h = FastDiv::of((unsigned)a.H), a.by_page = FastDiv::of((unsigned)a.page);
+  const int D = (int)c->D, kind = (int)c->kind, dtype = (int)c->dtype;
   if (int r = kv_check(a, D, kind, dtype)) return r;
+  if (!c->x[0] || !c->x[1] || (((uintptr_t)c->x[0] | (uintptr_t)c->x[1]) & 15)) TB_FAIL(TB_E_ARG, "kv cache: rows must be 16-byte aligned");
   const int N = dtype == 0 ? 8 : 4;
-  for (int i = 0; i < 6; ++i)
-    if (strides[i] % N) TB_FAIL(TB_E_ARG, "kv cache: strides must be multiples of 16 bytes");
-  if (!k || !v || (((uintptr_t)k | (uintptr_t)v) & 15)) TB_FAIL(TB_E_ARG, "kv cache: k and v must be 16-byte aligned");
-  return dtype == 0 ? kv_dispatch<bf16>(a, D, kind, true, st) : kv_dispatch<float>(a, D, kind, true, st);
+  for (int i = 0; write && i < 6; ++i)
+    if (c->strides[i] % N) TB_FAIL(TB_E_ARG, "kv cache: strides must be multiples of 16 bytes");
+  return dtype == 0 ? kv_dispatch<bf16>(a, D, kind, write, st) : kv_dispatch<float>(a, D, kind, write, st);
 }
-
-// yk, yv [B, T, H, D] contiguous: rows t >= counts[b] and rows that no page holds are zeros.
-TB_EXPORT int tb_kv_read(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales, void* yk, void* yv,
-                         const int* table, long table_ld, const int* start, const int* counts, int B, int T, int H, int D,
-                         int page, int pages_per_seq, int num_pages, int kind, int dtype, cudaStream_t st) {
+TB_EXPORT int tb_kv_write(const KvCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();
-  if (B <= 0 || T <= 0) return 0;
-  KvArgs a{{nullptr, nullptr}, {0, 0}, {0, 0}, {0, 0}, {yk, yv}, {(void*)k_pages, (void*)v_pages}, {(float*)k_scales, (float*)v_scales},
-           table, start, counts, table_ld, B, T, H, page, pages_per_seq, num_pages, FastDiv::of(H > 0 ? H : 1), FastDiv::of(page > 0 ? page : 1)};
-  if (int r = kv_check(a, D, kind, dtype)) return r;
-  if (!yk || !yv || (((uintptr_t)yk | (uintptr_t)yv) & 15)) TB_FAIL(TB_E_ARG, "kv cache: outputs must be 16-byte aligned");
-  return dtype == 0 ? kv_dispatch<bf16>(a, D, kind, false, st) : kv_dispatch<float>(a, D, kind, false, st);
+  return kv_call(c, true, st);
+}
+TB_EXPORT int tb_kv_read(const KvCall* c, cudaStream_t st) {
+  TB_ENSURE_DEVICE();
+  return kv_call(c, false, st);
 }

@@ -163,25 +163,36 @@ static int rotary_launch(const RotaryArgs& a, bool half, bool vec, cudaStream_t 
 }  // namespace tb
 using namespace tb;
 
-// q [tokens, hq, D], k [tokens, hk, D] (k null: hk = 0) with strides in elements, columns contiguous; yq, yk contiguous.
-TB_EXPORT int tb_rotary(const void* q, const void* k, void* yq, void* yk, const long* pos, const double* freqs, long tokens, int hq,
-                        int hk, int D, int R, long ldq, long lhq, long ldk, long lhk, int half, float magnitude, int inverse,
-                        int dtype, cudaStream_t st) {
+// q [tokens, hq, D], k [tokens, hk, D] (hk = 0: none) with strides in elements, columns contiguous; yq, yk contiguous.
+struct RotaryCall {
+  const void *q, *k;
+  void *yq, *yk;
+  const long* pos;
+  const double* freqs;
+  long tokens, hq, hk, D, R, ldq, lhq, ldk, lhk, half, inverse, dtype;
+  double magnitude;
+};
+TB_EXPORT int tb_rotary(const RotaryCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();
-  if (tokens <= 0 || hq + hk <= 0 || D == 0) return 0;
-  if (!q || !yq || (hk > 0 && (!k || !yk)) || !pos || (R > 0 && !freqs)) TB_FAIL(TB_E_ARG, "rotary: null pointer");
-  if (R < 0 || R % 2 || R > D || R > 2 * ROT_MAX_PAIRS) TB_FAIL(TB_E_ARG, "rotary: %d turned columns of %d (even, at most %d)", R, D, 2 * ROT_MAX_PAIRS);
-  if (hq < 0 || hk < 0 || ceil_div(tokens, ROT_TOKENS) <= 0) TB_FAIL(TB_E_TOO_LARGE, "rotary: too many tokens or heads");
-  if (dtype != 0 && dtype != 1) TB_FAIL(TB_E_ARG, "rotary: bf16 or fp32");
+  const void *q = c->q, *k = c->k;
+  void *yq = c->yq, *yk = c->yk;
+  const long tokens = c->tokens, ldq = c->ldq, lhq = c->lhq, ldk = c->ldk, lhk = c->lhk;
+  if (tokens <= 0 || c->hq + c->hk <= 0 || c->D == 0) return 0;
+  if (c->R < 0 || c->R % 2 || c->R > c->D || c->R > 2 * ROT_MAX_PAIRS) TB_FAIL(TB_E_ARG, "rotary: %ld turned columns of %ld (even, at most %d)", c->R, c->D, 2 * ROT_MAX_PAIRS);
+  if (!q || !yq || (c->hk > 0 && (!k || !yk)) || !c->pos || (c->R > 0 && !c->freqs)) TB_FAIL(TB_E_ARG, "rotary: null pointer");
+  if (c->hq < 0 || c->hk < 0 || c->hq + c->hk > 0x7fffffff / 2 || c->D > 0x7fffffff / 2 || tokens > 0xfffffff0l) TB_FAIL(TB_E_TOO_LARGE, "rotary: too many tokens or heads");
+  if (c->dtype != 0 && c->dtype != 1) TB_FAIL(TB_E_ARG, "rotary: bf16 or fp32");
+  const int hq = (int)c->hq, hk = (int)c->hk, D = (int)c->D, R = (int)c->R, dtype = (int)c->dtype;
+  const bool half = c->half != 0;
   const int N = dtype == 0 ? 8 : 4;
   bool vec = D % N == 0 && D / N <= ROT_THREADS && (!half || (R / 2) % N == 0);
   const uintptr_t at = (uintptr_t)q | (uintptr_t)yq | (hk ? (uintptr_t)k | (uintptr_t)yk : 0);
   vec = vec && at % 16 == 0 && ldq % N == 0 && lhq % N == 0 && (!hk || (ldk % N == 0 && lhk % N == 0));
-  RotaryArgs a{{q, k}, {yq, yk}, {ldq, ldk}, {lhq, lhk}, {hq, hk}, pos, freqs, tokens, D, R, 1, magnitude, inverse ? -1.f : 1.f};
+  RotaryArgs a{{q, k}, {yq, yk}, {ldq, ldk}, {lhq, lhk}, {hq, hk}, c->pos, c->freqs, tokens, D, R, 1, (float)c->magnitude, c->inverse ? -1.f : 1.f};
   // few tokens: several blocks share a token's heads, until each SM has two blocks or a block has one pass of its threads
   const long blocks = ceil_div(tokens, ROT_TOKENS);
   const int passes = ceil_div((long)(hq + hk) * D / (vec ? N : 2), ROT_THREADS);
   long s = 2l * sm_count() / blocks;
   a.splits = (int)(s < 1 ? 1 : s > passes ? passes : s);
-  return dtype == 0 ? rotary_launch<bf16>(a, half != 0, vec, st) : rotary_launch<float>(a, half != 0, vec, st);
+  return dtype == 0 ? rotary_launch<bf16>(a, half, vec, st) : rotary_launch<float>(a, half, vec, st);
 }

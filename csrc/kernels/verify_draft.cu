@@ -311,15 +311,25 @@ int tb_set_check_word_verify(int* word) {
   return 0;
 }
 
-TB_EXPORT int tb_verify_draft(const void* probs, const void* draft, const long* tokens, const long* parents, const float* uniforms,
-                              const int* counts, long* accepted, long* path, long* next, long pb, long pt, long db, long dt,
-                              long parents_ld, int B, int T, int V, int dtype, cudaStream_t st) {
+struct VerifyCall {
+  const void *probs, *draft;
+  long pb, pt, db, dt;
+  const long *tokens, *parents;
+  long parents_ld;
+  const float* uniforms;
+  const int* counts;
+  long* out;                    // accepted [B], next token [B], path [B, T]
+  long B, T, V, dtype;
+};
+TB_EXPORT int tb_verify_draft(const VerifyCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();
-  if (B <= 0) return 0;
-  if (T < 1 || T > VD_MAX_NODES || V < 1) TB_FAIL(TB_E_ARG, "verify: 1 to %d nodes and at least one token in the vocabulary", VD_MAX_NODES);
-  if (!probs || !tokens || !uniforms || !accepted || !path || !next) TB_FAIL(TB_E_ARG, "verify: null pointer");
-  if (dtype != 0 && dtype != 1) TB_FAIL(TB_E_ARG, "verify: bf16 or fp32");
-  if (B > 0x7fffffff / VD_CLUSTER || V > (1 << 22)) TB_FAIL(TB_E_TOO_LARGE, "verify: at most 2^22 tokens in the vocabulary");
-  VerifyArgs a{probs, draft, pb, pt, db, dt, tokens, parents, parents_ld, uniforms, counts, accepted, path, next, B, T, V};
+  if (c->B <= 0) return 0;
+  if (c->T < 1 || c->T > VD_MAX_NODES || c->V < 1) TB_FAIL(TB_E_ARG, "verify: 1 to %d nodes and at least one token in the vocabulary", VD_MAX_NODES);
+  if (!c->probs || !c->tokens || !c->uniforms || !c->out) TB_FAIL(TB_E_ARG, "verify: null pointer");
+  if (c->dtype != 0 && c->dtype != 1) TB_FAIL(TB_E_ARG, "verify: bf16 or fp32");
+  if (c->B > 0x7fffffff / VD_CLUSTER || c->V > (1 << 22)) TB_FAIL(TB_E_TOO_LARGE, "verify: at most 2^22 tokens in the vocabulary");
+  const VerifyArgs a{c->probs, c->draft, c->pb, c->pt, c->db, c->dt, c->tokens, c->parents, c->parents_ld, c->uniforms, c->counts,
+                     c->out, c->out + 2 * c->B, c->out + c->B, (int)c->B, (int)c->T, (int)c->V};
+  const int dtype = (int)c->dtype;
   return dtype == 0 ? verify_launch<bf16>(a, st) : verify_launch<float>(a, st);
 }

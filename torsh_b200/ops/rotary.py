@@ -12,10 +12,9 @@ import math
 
 import torch
 
-from .. import _native as nv
-from ._dispatch import F, I, L, P, call, dtype_code, kernel_ok, on_device
+from ._dispatch import Record, kernel_ok
 
-_ROTARY = [P, P, P, P, P, P, L, I, I, I, I, L, L, L, L, I, F, I, I, P]
+_ROTARY = Record("tb_rotary", "18qd")
 SCALINGS = ("none", "linear", "ntk", "yarn", "wavelength")
 _MAX_DIM = 512   # turned columns whose angles the kernel keeps
 
@@ -78,26 +77,28 @@ def _rotary_plain(x, positions, freqs, interleaved, magnitude, inverse):
 
 def _flat(x):
     """``(x, token stride, head stride)`` of ``[..., H, D]`` with contiguous columns and one stride over all leading dimensions."""
-    if x.dim() == 4 and x.stride(3) == 1 and (x.shape[0] == 1 or x.stride(0) == x.shape[1] * x.stride(1)):
-        return x, x.stride(1), x.stride(2)
-    if x.dim() == 3 and x.stride(2) == 1:
-        return x, x.stride(0), x.stride(1)
+    st = x.stride()
+    if len(st) == 4:
+        if st[3] == 1 and (x.shape[0] == 1 or st[0] == x.shape[1] * st[1]):
+            return x, st[1], st[2]
+    elif len(st) == 3 and st[2] == 1:
+        return x, st[0], st[1]
     x = x.contiguous()
     return x, x.shape[-2] * x.shape[-1], x.shape[-1]
 
 
 def _launch(q, k, positions, freqs, interleaved, magnitude, inverse):
     qc, ldq, lhq = _flat(q)
-    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    kc, yk, ldk, lhk, hk = None, None, 0, 0, 0
-    if k is not None:
+    yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    D = q.shape[-1]
+    if k is None:
+        yk, kp, ykp, hk, ldk, lhk = None, 0, 0, 0, 0, 0
+    else:
         kc, ldk, lhk = _flat(k)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        hk = k.shape[-2]
-    with on_device(q):
-        call("tb_rotary", _ROTARY, qc.data_ptr(), kc.data_ptr() if hk else None, yq.data_ptr(), yk.data_ptr() if hk else None,
-             positions.data_ptr(), freqs.data_ptr(), positions.numel(), q.shape[-2], hk, q.shape[-1], 2 * freqs.numel(), ldq, lhq, ldk,
-             lhk, 0 if interleaved else 1, magnitude, int(inverse), dtype_code(q), nv.stream_ptr())
+        yk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        kp, ykp, hk = kc.data_ptr(), yk.data_ptr(), k.shape[-2]
+    _ROTARY(q.get_device(), qc.data_ptr(), kp, yq.data_ptr(), ykp, positions.data_ptr(), freqs.data_ptr(), positions.numel(), q.shape[-2],
+            hk, D, 2 * freqs.numel(), ldq, lhq, ldk, lhk, not interleaved, inverse, q.dtype is torch.float32, magnitude)
     return yq, yk
 
 
@@ -129,27 +130,28 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     pair: ``2 * len(freqs)`` columns of ``D`` turn, the rest pass through. ``interleaved`` pairs columns ``(2i, 2i + 1)``, as
     :func:`~torsh_b200.ops.elementwise.rope` does; otherwise ``(i, i + len(freqs))``. Differentiable in ``q`` and ``k``.
     """
-    if q.dim() < 2 or (k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype)):
+    shape = q.shape
+    if len(shape) < 2 or (k is not None and (k.shape[:-2] != shape[:-2] or k.shape[-1] != shape[-1] or k.dtype != q.dtype)):
         raise ValueError("rotary: q and k are [..., heads, D] of one type with the same leading dimensions and D")
-    if freqs.dim() != 1 or 2 * freqs.numel() > q.shape[-1]:
-        raise ValueError(f"rotary: freqs has one entry for each pair of at most {q.shape[-1]} columns")
-    if positions.is_floating_point() or positions.dtype == torch.bool:
+    if freqs.dim() != 1 or 2 * freqs.numel() > shape[-1]:
+        raise ValueError(f"rotary: freqs has one entry for each pair of at most {shape[-1]} columns")
+    if positions.dtype is not torch.int64 and (positions.is_floating_point() or positions.dtype == torch.bool):
         raise TypeError("rotary: positions are integers")
-    lead = q.shape[:-2]
+    lead = shape[:-2]
     if positions.shape != lead:
         try:
             positions = positions.expand(lead)
         except RuntimeError:
             raise ValueError(f"rotary: positions {tuple(positions.shape)} do not fit {tuple(lead)}") from None
-    for t in (k, positions, freqs):
-        if t is not None and t.device != q.device:
-            raise ValueError("rotary: all tensors are on one device")
+    at = q.get_device()
+    if positions.get_device() != at or freqs.get_device() != at or (k is not None and k.get_device() != at):
+        raise ValueError("rotary: all tensors are on one device")
     if kernel_ok(q, k) and 2 * freqs.numel() <= _MAX_DIM:
-        if positions.dtype != torch.int64 or not positions.is_contiguous():
+        if positions.dtype is not torch.int64 or not positions.is_contiguous():
             positions = positions.to(torch.int64).contiguous()
-        if freqs.dtype != torch.float64 or not freqs.is_contiguous():
+        if freqs.dtype is not torch.float64 or not freqs.is_contiguous():
             freqs = freqs.to(torch.float64).contiguous()
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
             return _Rotary.apply(q, k, positions, freqs, interleaved, float(magnitude))
         return _launch(q, k, positions, freqs, interleaved, magnitude, False)
     f = freqs.to(torch.float64)

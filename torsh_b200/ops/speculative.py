@@ -8,10 +8,9 @@ from __future__ import annotations
 
 import torch
 
-from .. import _native as nv
-from ._dispatch import I, L, P, call, dtype_code, on_device
+from ._dispatch import Record
 
-_VERIFY = [P] * 9 + [L] * 5 + [I] * 4 + [P]
+_VERIFY = Record("tb_verify_draft", "16q")
 _MAX_NODES = 1024
 
 
@@ -36,8 +35,9 @@ def _check(probs, tokens, uniforms, draft_probs, parents, counts):
         raise ValueError(f"verify_draft: parents are integers, [{T}] or [{B}, {T}]")
     if counts is not None and (counts.shape != (B,) or counts.is_floating_point()):
         raise ValueError(f"verify_draft: counts are integers, [{B}]")
+    at = probs.get_device()
     for t in (tokens, uniforms, draft_probs, parents, counts):
-        if t is not None and t.device != probs.device:
+        if t is not None and t.get_device() != at:
             raise ValueError("verify_draft: all tensors are on one device")
 
 
@@ -63,26 +63,30 @@ def verify_draft(probs: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tens
     if not probs.is_cuda:
         return _verify_plain(probs, tokens, uniforms, draft_probs, parents, counts)
     B, T, V = probs.shape
-    if probs.stride(2) != 1:
+    pb, pt, step = probs.stride()
+    if step != 1:
         probs = probs.contiguous()
-    if draft_probs is not None and draft_probs.stride(2) != 1:
-        draft_probs = draft_probs.contiguous()
-    tokens = tokens.to(torch.int64).contiguous()
-    uniforms = uniforms.to(torch.float32).contiguous()
-    if parents is not None:
+        pb, pt, _ = probs.stride()
+    dp = db = dt = 0
+    if draft_probs is not None and T > 1:
+        if draft_probs.stride(2) != 1:
+            draft_probs = draft_probs.contiguous()
+        dp = draft_probs.data_ptr()
+        db, dt, _ = draft_probs.stride()
+    if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    if uniforms.dtype is not torch.float32 or not uniforms.is_contiguous():
+        uniforms = uniforms.to(torch.float32).contiguous()
+    if parents is not None and (parents.dtype is not torch.int64 or not parents.is_contiguous()):
         parents = parents.to(torch.int64).contiguous()
-    if counts is not None:
+    if counts is not None and (counts.dtype is not torch.int32 or not counts.is_contiguous()):
         counts = counts.to(torch.int32).contiguous()
     out = torch.empty(B * (T + 2), dtype=torch.int64, device=probs.device)
-    accepted, nxt, path = out[:B], out[B:2 * B], out[2 * B:].view(B, T)
-    d = draft_probs if T > 1 else None
-    with on_device(probs):
-        call("tb_verify_draft", _VERIFY, probs.data_ptr(), None if d is None else d.data_ptr(), tokens.data_ptr(),
-             None if parents is None else parents.data_ptr(), uniforms.data_ptr(), None if counts is None else counts.data_ptr(),
-             accepted.data_ptr(), path.data_ptr(), nxt.data_ptr(), probs.stride(0), probs.stride(1), 0 if d is None else d.stride(0),
-             0 if d is None else d.stride(1), T if parents is not None and parents.dim() == 2 else 0, B, T, V, dtype_code(probs),
-             nv.stream_ptr())
-    return accepted, path, nxt
+    _VERIFY(probs.get_device(), probs.data_ptr(), dp, pb, pt, db, dt, tokens.data_ptr(), 0 if parents is None else parents.data_ptr(),
+            T if parents is not None and parents.dim() == 2 else 0, uniforms.data_ptr(), 0 if counts is None else counts.data_ptr(), out.data_ptr(),
+            B, T, V, probs.dtype is torch.float32)
+    accepted, nxt, path = out.split([B, B, B * T])
+    return accepted, path.view(B, T), nxt
 
 
 def _verify_plain(probs, tokens, uniforms, draft_probs=None, parents=None, counts=None):
