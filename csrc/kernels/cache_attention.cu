@@ -3,7 +3,7 @@
 //   O[t] = sum_n P[t, n] V[n],  P = softmax(scale q_t . K[n]) over the context [0, start) and the new tokens that t's mask names
 //
 // The rows of one key/value head (the T tokens of its G query heads, row t G + g) share its keys. A warp takes 16 tokens at a time
-// for 8, 16 or 32 rows, the other way round: S^T = K Q^T and O^T += V^T P^T are mma.sync m16n8k16 products in which the tokens (then
+// for 8 or 16 rows, the other way round: S^T = K Q^T and O^T += V^T P^T are mma.sync m16n8k16 products in which the tokens (then
 // the columns of V) are the 16 and the rows the 8, so that one row costs 8 and not 16. Keys and values come out of a ring of the
 // warp's own, filled by 16-byte cp.async: a page is a multiple of 16 tokens, so a tile is one contiguous piece of one page. Nothing
 // but the end of a unit waits for another warp. These products are memory-bound (16 tokens of 256 bytes are 8 KB, which take 180
@@ -17,6 +17,7 @@
 // The work of all sequences is dealt to the CTAs in equal runs of tiles (deal_tiles), so ragged batches and single long sequences
 // fill the GPU alike; a unit cut by the deal is joined by cache_attn_join_kernel.
 #include "cache_attention.cuh"
+#include "decode_calls.h"
 
 namespace tb {
 
@@ -27,6 +28,9 @@ constexpr int CA_TILE = 16;   // tokens of a warp's tile
 __device__ __forceinline__ uint32_t ca_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ca_copy16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ca_copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void ca_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void ca_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -74,7 +78,7 @@ template <int D, int KIND, int NT> struct CaShape {
   static constexpr int TILE_BYTES = CA_TILE * ROW;
   static constexpr int STAGE = 2 * TILE_BYTES + (HALVES ? 2 * CA_TILE * 4 : 0);
   static constexpr int STAGES = 3;
-  static constexpr int OCC = NT == 4 || TILE_BYTES == 4096 ? 2 : NT == 2 ? 3 : 4;   // CTAs of an SM
+  static constexpr int OCC = TILE_BYTES == 4096 ? 2 : NT == 2 ? 3 : 4;   // CTAs of an SM
   static constexpr int MB = D / 16;                        // 16-column blocks of O
   static constexpr int BLOCKS = MB * NT;                   // of 16 columns and 8 rows: 512 bytes of floats
   static constexpr int PASS = 2 * TILE_BYTES / 512 < BLOCKS ? 2 * TILE_BYTES / 512 : BLOCKS;   // of which a stage takes so many
@@ -144,12 +148,22 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
       const uint8_t* kp = (const uint8_t*)a.k_pages + row * S::ROW + lane * 16;
       const uint8_t* vp = (const uint8_t*)a.v_pages + row * S::ROW + lane * 16;
       const uint32_t dst = ring_u + stage * S::STAGE;
+      if (live == CA_TILE) {
 #pragma unroll
-      for (int i = 0; i < S::TILE_BYTES / 512; ++i) {
-        const int ch = i * 32 + lane, tok = ch / S::CPR;
-        const uint32_t at = dst + chunk_at<S::CPR>(tok, ch % S::CPR);
-        ca_copy16(at, kp + i * 512, tok < live);
-        ca_copy16(at + S::TILE_BYTES, vp + i * 512, tok < live);
+        for (int i = 0; i < S::TILE_BYTES / 512; ++i) {
+          const int ch = i * 32 + lane;
+          const uint32_t at = dst + chunk_at<S::CPR>(ch / S::CPR, ch % S::CPR);
+          ca_copy16(at, kp + i * 512);
+          ca_copy16(at + S::TILE_BYTES, vp + i * 512);
+        }
+      } else {   // zeros behind the end: what lies there may be anything
+#pragma unroll 1
+        for (int i = 0; i < S::TILE_BYTES / 512; ++i) {
+          const int ch = i * 32 + lane, tok = ch / S::CPR;
+          const uint32_t at = dst + chunk_at<S::CPR>(tok, ch % S::CPR);
+          ca_copy16(at, kp + i * 512, tok < live);
+          ca_copy16(at + S::TILE_BYTES, vp + i * 512, tok < live);
+        }
       }
       if (HALVES && lane < 8) {
         const float* sc = (lane < 4 ? a.k_scales : a.v_scales) + row + (lane & 3) * 4;
@@ -174,6 +188,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
     // Q as the second operand: lane (g, c) holds row g; 8-bit keys give lane c the D / 4 neighbouring columns from c D / 4 on
     uint32_t qf[NT][D / 16][2];
     float qs[NT][2];     // of rows 2c, 2c + 1, as the scores have them
+    float s0[NT][2];     // what their scores begin with: int8 keys go in as 1152 + code (one instruction less per two), which is taken off here
     int tt[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -181,7 +196,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
       const int t = r / a.G;
       const bool live = t < w.s.count;
       const bf16* qp = a.q + w.b * a.qb + (long)t * a.qt + (long)(h * a.G + r - t * a.G) * a.qh;
-      float mine = a.scale_log2;
+      float mine = a.scale_log2, all = 0.f;
       if (!HALVES) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -209,11 +224,20 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
           for (int z = 0; z < 2; ++z) {
             const uint32_t v = qf[n][kk][z];
             qf[n][kk][z] = pack2<true>(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down);
+            if (KIND == CA_INT8) {
+              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][kk][z]));
+              all += y.x + y.y;
+            }
           }
+        if (KIND == CA_INT8) {
+          all += __shfl_xor_sync(0xffffffffu, all, 1);
+          all += __shfl_xor_sync(0xffffffffu, all, 2);
+        }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         qs[n][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
+        s0[n][e] = KIND == CA_INT8 ? -1152.f * __shfl_sync(0xffffffffu, all, (2 * c + e) * 4) : 0.f;
         tt[n][e] = min(__shfl_sync(0xffffffffu, t, (2 * c + e) * 4), a.T);
       }
     }
@@ -242,7 +266,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+        for (int e = 0; e < 4; ++e) sc[n][e] = s0[n][e & 1];
       if (!HALVES) {
         const int tok = lane & 15;
         const uint32_t ka = ca_smem(kt) + tok * S::ROW;
@@ -263,8 +287,8 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4) {
             uint32_t kf[4];
-            halves_of<KIND>(w0[k4], kf[0], kf[2]);
-            halves_of<KIND>(w1[k4], kf[1], kf[3]);
+            halves_of<KIND, false>(w0[k4], kf[0], kf[2]);
+            halves_of<KIND, false>(w1[k4], kf[1], kf[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma16816<HALVES>(sc[n], kf, qf[n][q * 4 + k4][0], qf[n][q * 4 + k4][1]);
           }
@@ -548,6 +572,7 @@ __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const Ca
   const bool mine = r < a.part_rows && t < a.T;
   float top = -INFINITY, all = 0.f, y[N] = {};
   if (mine) {
+#pragma unroll 4
     for (int k = c0 + lane; k <= c1; k += 32) {
       const float2 z = *(const float2*)(a.part_ml + ((long)slot_of(k, k > c0) * a.part_rows + r) * 2);
       const float now = fmaxf(top, z.x), ref = now == -INFINITY ? 0.f : now;
@@ -556,7 +581,7 @@ __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const Ca
     }
     const float now = warp_max(top), ref = now == -INFINITY ? 0.f : now;
     all = warp_sum(all * exp2f(top - ref));
-#pragma unroll 4
+#pragma unroll 8
     for (int k = c0 + sub; k <= c1; k += share) {
       const long at = (long)slot_of(k, k > c0) * a.part_rows + r;
       const float f = exp2f(a.part_ml[at * 2] - ref);
@@ -617,8 +642,7 @@ static int cache_attn_launch(CacheAttnArgs& a, cudaStream_t st) {
 
 template <int D, int KIND>
 static int cache_attn_rows(CacheAttnArgs& a, int nt, cudaStream_t st) {
-  if (nt == 1) return cache_attn_launch<D, KIND, 1>(a, st);
-  return nt == 2 ? cache_attn_launch<D, KIND, 2>(a, st) : cache_attn_launch<D, KIND, 4>(a, st);
+  return nt == 1 ? cache_attn_launch<D, KIND, 1>(a, st) : cache_attn_launch<D, KIND, 2>(a, st);
 }
 
 template <int D>
@@ -628,10 +652,12 @@ static int cache_attn_kind(CacheAttnArgs& a, int kind, int nt, cudaStream_t st) 
   return cache_attn_rows<D, CA_E4M3>(a, nt, st);
 }
 
-// Blocks of 8 rows that a CTA takes: 1, 2 or 4.
-static int ca_row_blocks(long rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+// Blocks of 8 rows that a CTA takes.
+static int ca_row_blocks(long rows) { return rows <= 8 ? 1 : 2; }
 constexpr int CA_MAX_OCC = 4;
-// Up to here the rows go to this file's kernel, beyond to the one on tcgen05.
+// Up to here the rows go to this file's kernel, beyond to the one on tcgen05. Both measured (us, this one / that one; B x context, eight
+// heads of D = 128): 16 rows bf16 8 x 2000 22 / 34, 8 x 16000 72 / 106, int8 28 / 37 and 80 / 145; 24 rows (32 of this one's) bf16 40 / 34
+// and 218 / 106, int8 42 / 37 and 212 / 145. With D = 64 and 24 rows it is 26 / 28 and 84 / 86, int8 28 / 31 and 95 / 112.
 constexpr long CA_MAX_ROWS = 16;
 static long ca_slots(bool tc) { return 2l * (tc ? 1 : CA_MAX_OCC) * sm_count(); }
 // Rows of a slot of partial results: a multiple of 4, so that what follows stays aligned.
@@ -655,21 +681,6 @@ TB_EXPORT long tb_cache_attention_workspace(int B, int T, int Hq, int Hkv, int D
 
 // q [B, T, Hq, D] bf16 (strides in elements, multiples of 8; 16-byte aligned), out contiguous. ws: tb_cache_attention_workspace() bytes,
 // 16-byte aligned, used by this call alone.
-struct CacheAttnCall {
-  const void* q;
-  long qb, qt, qh;
-  const void *k_pages, *v_pages;
-  const float *k_scales, *v_scales;
-  const int* table;
-  long table_ld;
-  const int *start, *counts;
-  const uint8_t* mask;
-  long mask_b, mask_t;
-  void *out, *ws;
-  long B, T, Hq, Hkv, D, page, pages_per_seq, num_pages, max_len, kind;
-  int* status;
-  double scale;
-};
 TB_EXPORT int tb_cache_attention(const CacheAttnCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();
   const long D = c->D, page = c->page, rows = c->Hkv > 0 ? c->T * (c->Hq / c->Hkv) : 0;

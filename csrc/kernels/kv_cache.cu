@@ -13,6 +13,7 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "decode_calls.h"
 #include "host_util.h"
 
 namespace tb {
@@ -47,24 +48,47 @@ __device__ __forceinline__ long kv_row(const KvArgs& a, int b, int t, int h) {
   return ((long)p * a.H + h) * a.page + (pos - slot * (unsigned)a.page);
 }
 
+// Largest |x| of 8 elements, as the bits of a float without its sign: a NaN counts for more than an infinity, that for more than any
+// number. Of bf16 two at a time.
+__device__ __forceinline__ uint32_t big8(const uint4& v) {
+  auto m = [](uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); };
+  const uint32_t x = m(m(v.x, v.y), m(v.z, v.w));
+  return max(x << 16, x & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t big8(const uint4& v, const uint4& w) {
+  const uint32_t k = 0x7fffffffu;
+  return max(max(max(v.x & k, v.y & k), max(v.z & k, v.w & k)), max(max(w.x & k, w.y & k), max(w.z & k, w.w & k)));
+}
 template <int G>
-__device__ __forceinline__ float group_max(float v) {
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = G / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    Vec16<T> v;
-    v.load_nc(p);
-    v.get(f);
-  } else {
-    const float4 u = __ldg((const float4*)p), w = __ldg((const float4*)p + 1);
-    f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = w.x, f[5] = w.y, f[6] = w.z, f[7] = w.w;
+// 8 elements as they lie in memory, and as floats.
+template <typename T> struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg((const uint4*)p + i);
   }
-}
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ uint32_t big() const {
+    if constexpr (sizeof(T) == 2) return big8(v[0]);
+    else return big8(v[0], v[1]);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t* w = &v[0].x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (sizeof(T) == 2) f[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+      else f[j] = __uint_as_float(w[j]);
+    }
+  }
+};
 
 // x / s to the nearest integer, halves to even, decided exactly: n is next to the quotient, x - n s is exact in one fma (s has
 // 24 bits, n 7, and the rest is smaller than s), and s / 2 is exact. A quotient in fp32 can round onto a half that x / s is not.
@@ -88,7 +112,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvArgs a) {
   const int b = blockIdx.y;
   const int n = a.counts ? min(a.counts[b], a.T) : a.T;
   if ((int)(blockIdx.x * (PER * R) / (unsigned)a.H) >= n) return;
-  float f[R][2][8];
+  Raw8<T> x[R][2];
   long row[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -97,56 +121,60 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvArgs a) {
     row[i] = -1;
     if (t < n) {
 #pragma unroll
-      for (int z = 0; z < 2; ++z) load8<T>((const T*)a.x[z] + b * a.sb[z] + t * a.st[z] + h * a.sh[z] + lane * 8, f[i][z]);
+      for (int z = 0; z < 2; ++z) x[i][z].load((const T*)a.x[z] + b * a.sb[z] + t * a.st[z] + h * a.sh[z] + lane * 8);
       row[i] = kv_row(a, b, t, h);
       if (row[i] < 0 && lane == 0) report_bad_index();
     } else {
 #pragma unroll
-      for (int z = 0; z < 2; ++z)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[i][z][j] = 0.f;
+      for (int z = 0; z < 2; ++z) x[i][z].clear();
     }
   }
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-      float (&x)[8] = f[i][z];
+      float f[8];
+      x[i][z].get(f);
       if constexpr (KIND == KV_BF16) {
         Vec16<bf16> v;
-        v.set(x);
+        if constexpr (sizeof(T) == 2) v.raw = x[i][z].v[0];
+        else v.set(f);
         if (row[i] >= 0) v.store((bf16*)a.pages[z] + row[i] * D + lane * 8);
       } else {
-        float big = 0.f;
-        bool wild = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          big = fmaxf(big, fabsf(x[j]));
-          wild |= (__float_as_uint(x[j]) & 0x7f800000u) == 0x7f800000u;
-        }
-        big = group_max<G>(wild ? __int_as_float(0x7f800000) : big);
-        wild = big > FLT_MAX;
-        const bool none = big < 7.888609052210118e-31f;   // 2^-100
+        const uint32_t bits = group_max<G>(x[i][z].big());
+        const float big = __uint_as_float(bits);
+        const bool wild = bits >= 0x7f800000u, none = bits < 0x0d800000u;   // 2^-100
         float s, inv;
         if (KIND == KV_INT8) {
           s = __fdiv_rn(big, 127.f);
           inv = __fdiv_rn(1.f, none ? 1.f : s);
         } else {
           // big = m 2^e with m in [1, 2); 448 = 1.75 x 2^8
-          const uint32_t u = __float_as_uint(big);
-          const int k = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u);
+          const int k = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u);
           s = __int_as_float((k + 127) << 23);
           inv = __int_as_float((127 - k) << 23);
         }
         uint32_t w[2] = {0u, 0u};
         if (!none && !wild) {
           if (KIND == KV_INT8) {
+            // x / s to the nearest by a sum with 1.5 x 2^23. Where the rest x - n s (exact) is a half of s, or more for the error of
+            // inv, the element is decided again by kv_round
+            float most = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv_round(x[j], s, inv) & 0xffu) << (8 * (j & 3));
+            for (int j = 0; j < 8; ++j) {
+              const float t = fmaf(f[j], inv, 12582912.f);
+              most = fmaxf(most, fabsf(fmaf(12582912.f - t, s, f[j])));
+              w[j >> 2] |= (__float_as_uint(t) & 0xffu) << (8 * (j & 3));
+            }
+            if (most >= 0.4999f * s) {
+              w[0] = w[1] = 0u;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv_round(f[j], s, inv) & 0xffu) << (8 * (j & 3));
+            }
           } else {
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
-              w[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[j] * inv, x[j + 1] * inv), __NV_SATFINITE, __NV_E4M3)
+              w[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[j] * inv, f[j + 1] * inv), __NV_SATFINITE, __NV_E4M3)
                            << (8 * (j & 3));
           }
         }
@@ -260,16 +288,6 @@ int tb_set_check_word_kv_cache(int* word) {
 
 // write: x[0], x[1] = k, v [B, T, H, D] with strides (batch, token, head) in elements, multiples of 16 bytes; rows t >= counts[b] are left out.
 // read: x[0], x[1] [B, T, H, D] contiguous, written; rows t >= counts[b], and rows that no page holds, are zeros.
-struct KvCall {
-  void* x[2];
-  long strides[6];
-  void* pages[2];
-  float* scales[2];
-  const int* table;
-  long table_ld;
-  const int *start, *counts;
-  long B, T, H, D, page, pages_per_seq, num_pages, kind, dtype;
-};
 static int kv_call(const KvCall* c, bool write, cudaStream_t st) {
   if (c->B <= 0 || c->T <= 0) return 0;
   if (c->B > 65535 || c->H <= 0 || c->T > 0x7fffff00l || c->H > 0x7fffff00l || c->T * c->H > 0x7fffff00l)

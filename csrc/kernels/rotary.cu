@@ -6,16 +6,19 @@
 // the same map with sin negated. Position and frequency meet in 64 bits: p * f / 2pi is reduced to a fraction of a turn
 // before it is rounded to fp32 (p * f rounded to fp32 first is off by 0.06 rad at p = 10^6), then sincospif.
 //
-// Bound by memory: x is read and y written once. The angles of a token are worked out once per block into shared memory and
-// stay in a thread's registers while it walks down the heads: R/2 sine/cosine pairs for every (Hq + Hk) D elements.
+// Bound by memory: x is read and y written once. The angles of a token are worked out once per block into shared memory:
+// R/2 sine/cosine pairs for every (Hq + Hk) D elements, while the block's loads are on their way.
 #include "common.cuh"
+#include "decode_calls.h"
 #include "host_util.h"
 
 namespace tb {
 
 constexpr int ROT_THREADS = 256;
 constexpr int ROT_MAX_PAIRS = 256;   // R <= 512
-constexpr int ROT_TOKENS = 2;        // tokens of a block
+constexpr int ROT_MAX_TOKENS = 8;    // tokens of a block
+constexpr int ROT_ANGLES = 1024;     // pairs of a block, over its tokens
+constexpr int ROT_TABLE = ROT_ANGLES + 8 * ROT_MAX_TOKENS;
 
 struct RotaryArgs {
   const void* x[2];      // q, k: [tokens, heads, D] with strides
@@ -25,11 +28,19 @@ struct RotaryArgs {
   const long* pos;
   const double* freqs;
   long tokens;
-  int D, R, splits;      // splits: blocks that share a token's heads
+  int D, R, per_block;   // per_block: tokens of a block
+  FastDiv by_heads;
   float magnitude, sign;
 };
 
-__device__ __forceinline__ void rot_angles(const RotaryArgs& a, long t0, int n, float2* tab) {
+// Cosines and sines of the block's tokens. A thread of the vector kernel needs K neighbouring pairs: pair K i + j lies at place j G + i of
+// its token, so that neighbouring threads read neighbouring words (in order they met four by four in a bank).
+struct RotTable {
+  int K, G;
+  __device__ __forceinline__ int stride() const { return K * G; }
+  __device__ __forceinline__ int at(int i, int j) const { return j * G + i; }
+};
+__device__ __forceinline__ void rot_angles(const RotaryArgs& a, long t0, int n, const RotTable& k, float2* tab) {
   const int half = a.R >> 1;
   for (int i = threadIdx.x; i < n * half; i += ROT_THREADS) {
     const int t = i / half, p = i - t * half;
@@ -37,83 +48,84 @@ __device__ __forceinline__ void rot_angles(const RotaryArgs& a, long t0, int n, 
     const float frac = (float)(turns - rint(turns));
     float s, c;
     sincospif(2.f * frac, &s, &c);
-    tab[t * half + p] = make_float2(c * a.magnitude, s * a.magnitude * a.sign);
+    tab[t * k.stride() + k.at(p / k.K, p % k.K)] = make_float2(c * a.magnitude, s * a.magnitude * a.sign);
   }
 }
 
-// VEC: 16-byte vectors. A thread owns one column position of a row (item) and walks down the heads.
+// A thread owns one 16-byte column position (item) of U rows (a head of a token). Its loads are on their way while the block works the
+// angles of its tokens out.
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_vec_kernel(const RotaryArgs a) {
   constexpr int N = Vec16<T>::N;
-  constexpr int U = HALF ? 2 : 4;      // heads in flight
-  __shared__ float2 tab[ROT_TOKENS * ROT_MAX_PAIRS];
+  constexpr int U = HALF ? 2 : 4;      // rows in flight
+  __shared__ float2 tab[ROT_TABLE];
+  constexpr int K = HALF ? N : N / 2;
   const int half = a.R >> 1, D = a.D;
-  const long t0 = (long)blockIdx.x * ROT_TOKENS;
-  const int nt = (int)min((long)ROT_TOKENS, a.tokens - t0);
+  const RotTable place{K, (half + K - 1) / K};
+  const long t0 = (long)blockIdx.x * a.per_block;
+  const int nt = (int)min((long)a.per_block, a.tokens - t0);
   // items of a head row. HALF: vectors of the first halves (with their partners), then the vectors that pass through
   const int turned = HALF ? half / N : (a.R + N - 1) / N;
   const int items = HALF ? turned + (D - a.R) / N : D / N;
   const int rows = ROT_THREADS / items;
   const int it = threadIdx.x % items, row = threadIdx.x / items;
-  rot_angles(a, t0, nt, tab);
-  __syncthreads();
-  if (row >= rows) return;
-  const int total = a.heads[0] + a.heads[1];
   const bool turn = it < turned;
   const int c0 = HALF ? (turn ? it * N : a.R + (it - turned) * N) : it * N;
-  for (int t = 0; t < nt; ++t) {
-    float2 cs[HALF ? N : N / 2];
-    if (turn) {
+  const int heads = a.heads[0] + a.heads[1], total = row < rows ? nt * heads : 0;
+  bool ready = false;
+  for (int first = blockIdx.y * U * rows + row; first - row < nt * heads || !ready; first += gridDim.y * U * rows) {
+    Vec16<T> u[U], w[U];
+    T* dst[U];
+    int tok[U];
 #pragma unroll
-      for (int j = 0; j < (HALF ? N : N / 2); ++j) {
-        const int p = HALF ? c0 + j : (c0 >> 1) + j;
-        cs[j] = p < half ? tab[t * half + p] : make_float2(1.f, 0.f);
+    for (int i = 0; i < U; ++i) {
+      const int r = first + i * rows;
+      if (r < total) {
+        const int t = (int)a.by_heads.div((unsigned)r), h = r - t * heads;
+        const int z = h >= a.heads[0];
+        const int hh = h - (z ? a.heads[0] : 0);
+        const T* src = (const T*)(z ? a.x[1] : a.x[0]) + (t0 + t) * (z ? a.ld[1] : a.ld[0]) + hh * (z ? a.lh[1] : a.lh[0]) + c0;
+        dst[i] = (T*)(z ? a.y[1] : a.y[0]) + ((t0 + t) * (z ? a.heads[1] : a.heads[0]) + hh) * D + c0;
+        tok[i] = t * place.stride() + it;
+        u[i].load_nc(src);
+        if (HALF && turn) w[i].load_nc(src + half);
       }
     }
-    for (int h0 = blockIdx.y * rows + row; h0 < total; h0 += U * rows * a.splits) {
-      Vec16<T> u[U], w[U];
-      T* dst[U];
+    if (!ready) {
+      rot_angles(a, t0, nt, place, tab);
+      __syncthreads();
+      ready = true;
+    }
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int h = h0 + i * rows * a.splits;
-        if (h < total) {
-          const int z = h >= a.heads[0];
-          const int hh = h - (z ? a.heads[0] : 0);
-          const T* src = (const T*)(z ? a.x[1] : a.x[0]) + (t0 + t) * (z ? a.ld[1] : a.ld[0]) + hh * (z ? a.lh[1] : a.lh[0]) + c0;
-          dst[i] = (T*)(z ? a.y[1] : a.y[0]) + ((t0 + t) * (z ? a.heads[1] : a.heads[0]) + hh) * D + c0;
-          u[i].load_nc(src);
-          if (HALF && turn) w[i].load_nc(src + half);
-        }
-      }
+    for (int i = 0; i < U; ++i) {
+      if (first + i * rows < total) {
+        if (turn) {
+          float f[N];
+          u[i].get(f);
+          if (HALF) {
+            float g[N];
+            w[i].get(g);
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (h0 + i * rows * a.splits < total) {
-          if (turn) {
-            float f[N];
-            u[i].get(f);
-            if (HALF) {
-              float g[N];
-              w[i].get(g);
-#pragma unroll
-              for (int j = 0; j < N; ++j) {
-                const float x = f[j], y = g[j];
-                f[j] = x * cs[j].x - y * cs[j].y;
-                g[j] = x * cs[j].y + y * cs[j].x;
-              }
-              w[i].set(g);
-              w[i].store(dst[i] + half);
-            } else {
-#pragma unroll
-              for (int j = 0; j < N / 2; ++j) {
-                const float x = f[2 * j], y = f[2 * j + 1];
-                f[2 * j] = x * cs[j].x - y * cs[j].y;
-                f[2 * j + 1] = x * cs[j].y + y * cs[j].x;
-              }
+            for (int j = 0; j < N; ++j) {
+              const float2 cs = tab[tok[i] + j * place.G];
+              const float x = f[j], y = g[j];
+              f[j] = x * cs.x - y * cs.y;
+              g[j] = x * cs.y + y * cs.x;
             }
-            u[i].set(f);
+            w[i].set(g);
+            w[i].store(dst[i] + half);
+          } else {
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) {
+              const float2 cs = (c0 >> 1) + j < half ? tab[tok[i] + j * place.G] : make_float2(1.f, 0.f);
+              const float x = f[2 * j], y = f[2 * j + 1];
+              f[2 * j] = x * cs.x - y * cs.y;
+              f[2 * j + 1] = x * cs.y + y * cs.x;
+            }
           }
-          u[i].store(dst[i]);
+          u[i].set(f);
         }
+        u[i].store(dst[i]);
       }
     }
   }
@@ -122,15 +134,15 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_vec_kernel(const RotaryArg
 // Head sizes, pairings and addresses that 16-byte vectors do not fit: one pair (or one column that passes through) at a time.
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_scalar_kernel(const RotaryArgs a) {
-  __shared__ float2 tab[ROT_TOKENS * ROT_MAX_PAIRS];
+  __shared__ float2 tab[ROT_TABLE];
   const int half = a.R >> 1, D = a.D;
-  const long t0 = (long)blockIdx.x * ROT_TOKENS;
-  const int nt = (int)min((long)ROT_TOKENS, a.tokens - t0);
-  rot_angles(a, t0, nt, tab);
+  const long t0 = (long)blockIdx.x * a.per_block;
+  const int nt = (int)min((long)a.per_block, a.tokens - t0);
+  rot_angles(a, t0, nt, RotTable{1, half}, tab);
   __syncthreads();
   const int items = half + D - a.R, total = a.heads[0] + a.heads[1];
   for (int t = 0; t < nt; ++t)
-    for (long i = (long)blockIdx.y * ROT_THREADS + threadIdx.x; i < (long)total * items; i += (long)a.splits * ROT_THREADS) {
+    for (long i = (long)blockIdx.y * ROT_THREADS + threadIdx.x; i < (long)total * items; i += (long)gridDim.y * ROT_THREADS) {
       const int h = (int)(i / items), it = (int)(i - (long)h * items);
       const int z = h >= a.heads[0];
       const int hh = h - (z ? a.heads[0] : 0);
@@ -150,8 +162,33 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_scalar_kernel(const Rotary
 }
 
 template <typename T>
-static int rotary_launch(const RotaryArgs& a, bool half, bool vec, cudaStream_t st) {
-  const dim3 grid((unsigned)ceil_div(a.tokens, ROT_TOKENS), (unsigned)a.splits);
+static int rotary_launch(RotaryArgs& a, bool half, bool vec, cudaStream_t st) {
+  // A block's tokens: as many as its threads have rows in flight for, and as many more as give each thread an angle while there are 24
+  // blocks for each SM, of which it holds 4 at a time. (8192 tokens of 64 heads of 128: 2 tokens 46 us; 1, whose 64 angles leave six
+  // warps of eight idle, 55; 4, whose last round of blocks is half empty, 52.)
+  constexpr int N = Vec16<T>::N;
+  const int heads = a.heads[0] + a.heads[1];
+  const int items = half ? a.R / 2 / N + (a.D - a.R) / N : a.D / N;
+  const long rows = vec ? (long)(ROT_THREADS / items) * (half ? 2 : 4) : 1;
+  long per = vec ? rows / heads : 1;
+  if (a.R) {
+    long full = ROT_THREADS / (a.R / 2);
+    const long room = a.tokens / (24l * sm_count());
+    full = full < room ? full : room;
+    per = per > full ? per : full;
+  }
+  const long most = a.R ? ROT_ANGLES / (a.R / 2) : ROT_MAX_TOKENS;
+  per = per < 1 ? 1 : per > ROT_MAX_TOKENS ? ROT_MAX_TOKENS : per;
+  per = per > most ? most : per;
+  a.per_block = (int)per;
+  a.by_heads = FastDiv::of((unsigned)heads);
+  // few tokens with many heads: several blocks to a token
+  const long all = vec ? (per * heads + rows - 1) / rows : ceil_div((long)heads * (a.R / 2 + a.D - a.R), 8 * ROT_THREADS);
+  const long want = a.tokens / per < sm_count() ? all : 1;
+  const long chunks = want < 65535 ? want : 65535;
+  const long blocks = (a.tokens + per - 1) / per;
+  if (blocks > 0x7fffffffl) TB_FAIL(TB_E_TOO_LARGE, "rotary: too many tokens or heads");
+  const dim3 grid((unsigned)blocks, (unsigned)chunks);
   if (vec && half) rotary_vec_kernel<T, true><<<grid, ROT_THREADS, 0, st>>>(a);
   else if (vec) rotary_vec_kernel<T, false><<<grid, ROT_THREADS, 0, st>>>(a);
   else if (half) rotary_scalar_kernel<T, true><<<grid, ROT_THREADS, 0, st>>>(a);
@@ -164,14 +201,6 @@ static int rotary_launch(const RotaryArgs& a, bool half, bool vec, cudaStream_t 
 using namespace tb;
 
 // q [tokens, hq, D], k [tokens, hk, D] (hk = 0: none) with strides in elements, columns contiguous; yq, yk contiguous.
-struct RotaryCall {
-  const void *q, *k;
-  void *yq, *yk;
-  const long* pos;
-  const double* freqs;
-  long tokens, hq, hk, D, R, ldq, lhq, ldk, lhk, half, inverse, dtype;
-  double magnitude;
-};
 TB_EXPORT int tb_rotary(const RotaryCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();
   const void *q = c->q, *k = c->k;
@@ -188,11 +217,6 @@ TB_EXPORT int tb_rotary(const RotaryCall* c, cudaStream_t st) {
   bool vec = D % N == 0 && D / N <= ROT_THREADS && (!half || (R / 2) % N == 0);
   const uintptr_t at = (uintptr_t)q | (uintptr_t)yq | (hk ? (uintptr_t)k | (uintptr_t)yk : 0);
   vec = vec && at % 16 == 0 && ldq % N == 0 && lhq % N == 0 && (!hk || (ldk % N == 0 && lhk % N == 0));
-  RotaryArgs a{{q, k}, {yq, yk}, {ldq, ldk}, {lhq, lhk}, {hq, hk}, c->pos, c->freqs, tokens, D, R, 1, (float)c->magnitude, c->inverse ? -1.f : 1.f};
-  // few tokens: several blocks share a token's heads, until each SM has two blocks or a block has one pass of its threads
-  const long blocks = ceil_div(tokens, ROT_TOKENS);
-  const int passes = ceil_div((long)(hq + hk) * D / (vec ? N : 2), ROT_THREADS);
-  long s = 2l * sm_count() / blocks;
-  a.splits = (int)(s < 1 ? 1 : s > passes ? passes : s);
+  RotaryArgs a{{q, k}, {yq, yk}, {ldq, ldk}, {lhq, lhk}, {hq, hk}, c->pos, c->freqs, tokens, D, R, 1, {}, (float)c->magnitude, c->inverse ? -1.f : 1.f};
   return dtype == 0 ? rotary_launch<bf16>(a, half, vec, st) : rotary_launch<float>(a, half, vec, st);
 }

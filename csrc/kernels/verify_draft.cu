@@ -17,6 +17,7 @@
 #include <utility>
 
 #include "common.cuh"
+#include "decode_calls.h"
 #include "host_util.h"
 
 namespace tb {
@@ -311,16 +312,6 @@ int tb_set_check_word_verify(int* word) {
   return 0;
 }
 
-struct VerifyCall {
-  const void *probs, *draft;
-  long pb, pt, db, dt;
-  const long *tokens, *parents;
-  long parents_ld;
-  const float* uniforms;
-  const int* counts;
-  long* out;                    // accepted [B], next token [B], path [B, T]
-  long B, T, V, dtype;
-};
 TB_EXPORT int tb_verify_draft(const VerifyCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();
   if (c->B <= 0) return 0;

@@ -61,6 +61,24 @@ def test_rotary(dtype, interleaved, B, T, Hq, Hk, D, R):
     assert none is None and torch.equal(only, yq.detach())
 
 
+def test_rotary_gradient_of_a_gradient_and_of_one_output():
+    from torsh_b200.ops.rotary import rotary, rotary_frequencies
+    g = _gen(3)
+    q, k = (torch.randn(2, 3, 2, 64, device=DEV, generator=g).requires_grad_() for _ in range(2))
+    pos = torch.arange(3, device=DEV).expand(2, 3).contiguous()
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    yq, yk = rotary(q, k, pos, freqs)
+    gq, gk = torch.autograd.grad(yq.sum(), (q, k), allow_unused=True)      # nothing comes back through k but zeros
+    _rotary_close(gq, torch.ones_like(yq), _turn64(torch.ones_like(yq), pos, freqs, True, 1.0, True), 1.0)
+    assert gk is None or not gk.any()
+    dy = torch.randn_like(q).requires_grad_()
+    yq, _ = rotary(q, None, pos, freqs)
+    (gq,) = torch.autograd.grad(yq, q, dy, create_graph=True)
+    w = torch.randn_like(q)
+    (gd,) = torch.autograd.grad((gq * w).sum(), dy)                        # the rotation of w
+    _rotary_close(gd, w, _turn64(w, pos, freqs, True, 1.0), 1.0)
+
+
 def test_rotary_strides_and_shared_positions():
     from torsh_b200.ops.rotary import rotary, rotary_frequencies
     B, T, H, D = 3, 11, 4, 64

@@ -1,12 +1,14 @@
 """In-tree native build: nvcc for the sm_100a kernels, g++ for the host runtime.
 
-Two shared libraries are produced under ``torsh_b200/lib``:
+Two shared libraries and an extension module are produced under ``torsh_b200/lib``:
 
 * ``libtorsh_b200_cuda.so``  - every ``csrc/kernels/*.cu`` (kernels + ``extern "C"`` launchers)
 * ``libtorsh_b200_host.so``  - every ``csrc/host/*.cpp`` (TCP store, TRSH codec, bucket planner,
   pipeline scheduler, caching-allocator model, C ABI, ...)
+* ``_decode_calls.so``       - ``csrc/torch/decode_calls.cpp``: the decoding operators' checks, allocations and autograd node on the
+  tensors themselves, for calls whose GPU time is shorter than their Python
 
-Both are loaded with ``ctypes`` by :mod:`torsh_b200._native`. Objects are rebuilt only when a
+The libraries are loaded with ``ctypes`` by :mod:`torsh_b200._native`. Objects are rebuilt only when a
 source or header is newer. The reference detects CUDA in ``crates/torsh-backend/build.rs:21-101``
 and lists ``sm_70..sm_89`` arch flags in ``crates/torsh-utils/src/cpp_extension.rs``; here there is
 exactly one target, ``sm_100a``.
@@ -104,12 +106,31 @@ def build_host(verbose: bool = False) -> Path:
     return out
 
 
+def build_torch(verbose: bool = False) -> Path:
+    import sysconfig
+
+    import torch
+    src, out = CSRC / "torch" / "decode_calls.cpp", LIBDIR / "_decode_calls.so"
+    LIBDIR.mkdir(parents=True, exist_ok=True)
+    if _newer(src, out, [CSRC / "include" / "decode_calls.h"]):
+        base = Path(torch.__file__).resolve().parent
+        cuda = Path(_nvcc()).resolve().parent.parent / "include"
+        inc = [CSRC / "include", base / "include", base / "include" / "torch" / "csrc" / "api" / "include", cuda, sysconfig.get_paths()["include"]]
+        cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+        _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+              *(f"-isystem{p}" if i else f"-I{p}" for i, p in enumerate(inc)), str(src), "-o", str(out), f"-L{base / 'lib'}", "-lc10", "-lc10_cuda",
+              "-ltorch_cpu", "-ltorch", "-ltorch_python"], verbose)
+    return out
+
+
 def build_all(verbose: bool = False) -> None:
     build_cuda(verbose)
     build_host(verbose)
+    build_torch(verbose)
 
 
 if __name__ == "__main__":
     build_cuda(verbose="-v" in sys.argv, ptxas_info="--ptxas" in sys.argv)
     build_host(verbose="-v" in sys.argv)
+    build_torch(verbose="-v" in sys.argv)
     print("built:", *[p.name for p in LIBDIR.glob("*.so")])

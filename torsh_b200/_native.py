@@ -69,6 +69,34 @@ def host():
     return _host_lib
 
 
+_decode = None
+
+
+def decode_calls():
+    """The extension module of the decoding operators (``csrc/torch/decode_calls.cpp``), bound to the kernel library on first use."""
+    global _decode
+    if _decode is None:
+        lib = require_cuda()
+        with _lock:
+            if _decode is None:
+                import importlib.util
+                import sys
+                path = _LIBDIR / "_decode_calls.so"
+                if not path.exists() and os.environ.get("TORSH_B200_NO_AUTOBUILD") != "1":
+                    from . import _build
+                    _build.build_torch()
+                if not path.exists():
+                    raise NativeError(f"{path} is missing: run `python -m torsh_b200._build`")
+                spec = importlib.util.spec_from_file_location("torsh_b200._decode_calls", path)
+                mod = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(mod)
+                mod.bind(sys.modules[__name__], *(c_void_p.from_address(ctypes.addressof(getattr(lib, f))).value for f in (
+                    "tb_set_device", "tb_last_error", "tb_rotary", "tb_kv_write", "tb_kv_read", "tb_cache_attention",
+                    "tb_cache_attention_workspace", "tb_verify_draft")))
+                _decode = mod
+    return _decode
+
+
 def cuda_available() -> bool:
     return torch.cuda.is_available()
 

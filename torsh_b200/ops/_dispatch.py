@@ -2,7 +2,6 @@
 from __future__ import annotations
 
 import ctypes
-import struct
 
 import torch
 
@@ -49,7 +48,7 @@ def fn(name: str, argtypes):
     return f
 
 
-_KERNELS_PER_CALL = {"tb_flash_attn_bwd": 3, "tb_lamb_multi": 2, "tb_bn_fwd": 3, "tb_bn_bwd": 2, "tb_cache_attention": 2}
+_KERNELS_PER_CALL = {"tb_flash_attn_bwd": 3, "tb_lamb_multi": 2, "tb_bn_fwd": 3, "tb_bn_bwd": 2}
 
 
 def call(name: str, argtypes, *args):
@@ -57,27 +56,3 @@ def call(name: str, argtypes, *args):
     if rc != 0:
         nv.check(rc, name)
     nv.launch_count += _KERNELS_PER_CALL.get(name, 1)
-
-
-class Record:
-    """A launcher of the CUDA library that takes its arguments as one record of 8-byte fields (``q`` an integer or an address, ``d`` a
-    double), packed in one call: 25 arguments through ``call`` cost 4 us of Python, the record 1. The launch goes to the device of
-    ``index``, on that device's current stream, whichever device the caller is on."""
-
-    def __init__(self, name: str, fields: str):
-        self.name, self.pack, self.f, self.kernels = name, struct.Struct("=" + fields).pack, None, _KERNELS_PER_CALL.get(name, 1)
-
-    def __call__(self, index: int, *fields) -> None:
-        f = self.f
-        if f is None:
-            f = self.f = fn(self.name, [ctypes.c_char_p, P])
-        d = torch._C._cuda_getDevice()
-        if d != index:
-            with torch.cuda.device(index):
-                return self(index, *fields)
-        if d != nv._bound_device:
-            nv.stream_ptr()   # tells the library which device is current
-        rc = f(self.pack(*fields), torch._C._cuda_getCurrentRawStream(d))
-        if rc != 0:
-            nv.check(rc, self.name)
-        nv.launch_count += self.kernels

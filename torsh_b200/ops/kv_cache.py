@@ -15,81 +15,58 @@ Rows whose largest magnitude is below 2^-100 are held as zeros; a row that has a
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
 from .. import _native as nv
-from ._dispatch import I, Record, fn
 
-_WRITE, _READ = Record("tb_kv_write", "25q"), Record("tb_kv_read", "25q")
-_ATTN = Record("tb_cache_attention", "28qd")
-_KINDS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
-_ROWS = {torch.bfloat16: 0, torch.float32: 1}
 _TINY = 2.0 ** -100
 _CODES = (torch.int8, torch.float8_e4m3fn)
-_INTS = (torch.int32, torch.int64)
 
 
 # ------------------------------------------------------------------------------------------------ checks
-def _check_pages(what, k_pages, v_pages, k_scales, v_scales, page_table, B, at):
-    """Refuses pages, scales and tables that do not belong together; returns whether the kernels take the pages."""
-    shape, dt = k_pages.shape, k_pages.dtype
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not dt:
+def _check_pages(what, k_pages, v_pages, k_scales, v_scales, page_table, B, device):
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
         raise ValueError(f"{what}: k_pages and v_pages are [num_pages, H, page, D] of one shape and type")
+    dt = k_pages.dtype
     if dt in _CODES:
-        rows = shape[:3]
         for s in (k_scales, v_scales):
-            if s is None or s.shape != rows or s.dtype is not torch.float32 or not s.is_contiguous():
-                raise ValueError(f"{what}: pages of {dt} need contiguous fp32 scales {tuple(rows)}")
-            if s.get_device() != at:
-                raise ValueError(f"{what}: all tensors are on one device")
+            if s is None or s.shape != k_pages.shape[:3] or s.dtype != torch.float32 or not s.is_contiguous():
+                raise ValueError(f"{what}: pages of {dt} need contiguous fp32 scales {tuple(k_pages.shape[:3])}")
     elif not dt.is_floating_point or dt.itemsize == 1:
         raise TypeError(f"{what}: pages of bf16, int8 or float8_e4m3fn (or another 16- to 64-bit floating type on the plain path), got {dt}")
     elif k_scales is not None or v_scales is not None:
         raise ValueError(f"{what}: pages of {dt} have no scales")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError(f"{what}: pages have to be contiguous")
-    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.dtype not in _INTS:
+    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: page_table is [{B}, pages], int32")
-    if k_pages.get_device() != at or v_pages.get_device() != at or page_table.get_device() != at:
-        raise ValueError(f"{what}: all tensors are on one device")
-    return at >= 0 and dt in _KINDS and shape[3] in (64, 128) and not (k_pages.data_ptr() | v_pages.data_ptr()) % 16
+    for t in (k_pages, v_pages, k_scales, v_scales, page_table):
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: all tensors are on one device")
 
 
-def _per_sequence(what, name, t, B, at):
+def _per_sequence(what, name, t, B, device):
     """A vector of B integers as the kernels read it."""
-    if t.dtype is torch.int32 and t.shape == (B,) and t.get_device() == at and t.is_contiguous():
-        return t
-    if t.shape != (B,) or t.is_floating_point() or t.get_device() != at:
-        raise ValueError(f"{what}: {name} is a vector of {B} integers on the device of the others")
+    if t.shape != (B,) or t.is_floating_point() or t.device != device:
+        raise ValueError(f"{what}: {name} is a vector of {B} integers on {device}")
     return t.to(torch.int32).contiguous()
+
+
+def _no_grad(what, *tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under no_grad()")
 
 
 def _table(page_table):
     return page_table if page_table.dtype is torch.int32 and page_table.stride(1) == 1 else page_table.to(torch.int32).contiguous()
 
 
-def _no_grad(what, t):
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{what} has no backward pass: call it under no_grad()")
-
-
-def _aligned_rows(x):
-    """``(x, address, strides)`` with 16-byte rows at any stride that keeps them aligned; copied where they are not."""
+def _rows(x):
+    """Rows that start on 16 bytes; copied where they do not."""
     n = 16 // x.element_size()
-    a, b, c, d = x.stride()
-    p = x.data_ptr()
-    if d != 1 or p % 16 or a % n or b % n or c % n:
-        x = x.clone(memory_format=torch.contiguous_format)
-        a, b, c, d = x.stride()
-        p = x.data_ptr()
-    return x, p, a, b, c
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+    return x if x.stride(3) == 1 and not x.data_ptr() % 16 and not any(s % n for s in x.stride()[:3]) else x.clone(memory_format=torch.contiguous_format)
 
 
 # ------------------------------------------------------------------------------------------------ the formulas in PyTorch
@@ -148,28 +125,26 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     left out. Positions that the table does not reach, or to which it gives a page outside the pool, are skipped (and reported where
     the device-side index checks are on). Two sequences may share pages, but not the positions that one call writes.
     """
-    if k.dim() != 4 or v.shape != k.shape or v.dtype is not k.dtype or not k.is_floating_point():
+    if k.is_cuda and (nv._decode or nv.decode_calls()).kv_write(k, v, k_pages, v_pages, page_table, start, counts, k_scales, v_scales):
+        return
+    # not as the kernel takes it: refused, converted, or computed here
+    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or not k.is_floating_point():
         raise ValueError("kv_cache_write: k and v are [B, T, H, D] of one floating type")
     B, T, H, D = k.shape
-    dev = k.get_device()
-    kernel = _check_pages("kv_cache_write", k_pages, v_pages, k_scales, v_scales, page_table, B, dev)
-    num_pages, Hp, page, Dp = k_pages.shape
-    if Hp != H or Dp != D or v.get_device() != dev:
-        raise ValueError(f"kv_cache_write: pages of {Hp} heads of {Dp}, rows of {H} of {D}")
-    _no_grad("kv_cache_write", k)
-    _no_grad("kv_cache_write", v)
-    start = _per_sequence("kv_cache_write", "start", start, B, dev)
+    _check_pages("kv_cache_write", k_pages, v_pages, k_scales, v_scales, page_table, B, k.device)
+    if k_pages.shape[1] != H or k_pages.shape[3] != D or v.device != k.device:
+        raise ValueError(f"kv_cache_write: pages of {k_pages.shape[1]} heads of {k_pages.shape[3]}, rows of {H} of {D}")
+    _no_grad("kv_cache_write", k, v)
+    start = _per_sequence("kv_cache_write", "start", start, B, k.device)
     if counts is not None:
-        counts = _per_sequence("kv_cache_write", "counts", counts, B, dev)
+        counts = _per_sequence("kv_cache_write", "counts", counts, B, k.device)
     if k.numel() == 0:
         return
-    if kernel and k.dtype in _ROWS:
-        k, kp, *ks = _aligned_rows(k)
-        v, vp, *vs = _aligned_rows(v)
-        table = _table(page_table)
-        _WRITE(dev, kp, vp, *ks, *vs, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), table.data_ptr(), table.stride(0),
-               start.data_ptr(), _ptr(counts), B, T, H, D, page, table.shape[1], num_pages, _KINDS[k_pages.dtype], _ROWS[k.dtype])
-        return
+    num_pages, _, page, _ = k_pages.shape
+    if k.is_cuda:
+        with torch.cuda.device(k.device):
+            if nv.decode_calls().kv_write(_rows(k), _rows(v), k_pages, v_pages, _table(page_table), start, counts, k_scales, v_scales):
+                return
     at = torch.arange(T, device=k.device)
     slot, row, there = _slots(page_table, num_pages, page, start.long()[:, None] + at)
     if counts is not None:
@@ -188,27 +163,28 @@ def kv_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
                   dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """Reads ``lengths[b]`` tokens of each sequence back, from position ``begin[b]`` (0) on: keys and values ``[B, max_len, H, D]`` in
     ``dtype``. Rows from ``lengths[b]`` on, and rows that no page of the pool holds, are zeros."""
+    fast = k_pages.is_cuda and dtype in (torch.bfloat16, torch.float32)
+    if fast:
+        out = (nv._decode or nv.decode_calls()).kv_read(k_pages, v_pages, page_table, lengths, max_len, begin, k_scales, v_scales, dtype is torch.float32)
+        if out is not None:
+            return out
+    # not as the kernel takes it: refused, converted, or computed here
     B = page_table.shape[0] if page_table.dim() == 2 else -1
-    at = k_pages.get_device()
-    kernel = _check_pages("kv_cache_read", k_pages, v_pages, k_scales, v_scales, page_table, B, at)
+    dev = k_pages.device
+    _check_pages("kv_cache_read", k_pages, v_pages, k_scales, v_scales, page_table, B, dev)
     if max_len < 0:
         raise ValueError("kv_cache_read: max_len is not negative")
     if not dtype.is_floating_point or dtype.itemsize < 2:
         raise TypeError(f"kv_cache_read: rows are read in a floating type of 16 bits or more, got {dtype}")
     num_pages, H, page, D = k_pages.shape
-    lengths = _per_sequence("kv_cache_read", "lengths", lengths, B, at)
+    lengths = _per_sequence("kv_cache_read", "lengths", lengths, B, dev)
     if begin is not None:
-        begin = _per_sequence("kv_cache_read", "begin", begin, B, at)
-    dev = k_pages.device
-    if kernel and dtype in _ROWS:
-        k = torch.empty((B, max_len, H, D), dtype=dtype, device=dev)
-        v = torch.empty_like(k)
-        if k.numel():
-            table = _table(page_table)
-            _READ(at, k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 0, 0, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
-                  table.data_ptr(), table.stride(0), _ptr(begin), lengths.data_ptr(), B, max_len, H, D, page, table.shape[1], num_pages,
-                  _KINDS[k_pages.dtype], _ROWS[dtype])
-        return k, v
+        begin = _per_sequence("kv_cache_read", "begin", begin, B, dev)
+    if fast:
+        with torch.cuda.device(dev):
+            out = nv.decode_calls().kv_read(k_pages, v_pages, _table(page_table), lengths, int(max_len), begin, k_scales, v_scales, dtype is torch.float32)
+        if out is not None:
+            return out
     at = torch.arange(max_len, device=dev)[None].expand(B, -1)
     slot, row, there = _slots(page_table, num_pages, page, at if begin is None else at + begin.long()[:, None])
     there = there & (at < lengths[:, None])
@@ -219,25 +195,6 @@ def kv_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
 
 
 # ------------------------------------------------------------------------------------------------ attention
-_ws_bytes: dict = {}
-
-
-def _workspace(q, B, T, Hq, Hkv, D, at):
-    """Workspace of one call: bytes from the allocator each time, so that calls on several streams, or in several captured graphs, never share them."""
-    key = (B, T, Hq, Hkv, D, at)
-    n = _ws_bytes.get(key)
-    if n is None:
-        f = fn("tb_cache_attention_workspace", [I] * 5)
-        f.restype = ctypes.c_long
-        with torch.cuda.device(at):
-            nv.stream_ptr()   # makes the library's device current
-            n = int(f(B, T, Hq, Hkv, D))
-        if len(_ws_bytes) > 4096:
-            _ws_bytes.clear()
-        _ws_bytes[key] = n
-    return torch.empty(n, dtype=torch.uint8, device=q.device)
-
-
 def _attention_plain(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, limit):
     """fp32 (fp64 for fp64) maths; the CPU path and the test oracle. What a row does not see is never multiplied: an infinity there stays there."""
     B, T, Hq, D = q.shape
@@ -291,44 +248,38 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     places that a row does not see do not reach it. ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
     not read. Pages outside the pool read as zeros. No backward pass.
     """
+    if q.is_cuda:
+        out = (nv._decode or nv.decode_calls()).kv_attention(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, max_len,
+                                                             nv.status_ptr(q.device))
+        if out is not None:
+            return out
+    # not as the kernels take it: refused, converted, or computed here
     if q.dim() != 4 or not q.is_floating_point():
         raise ValueError("kv_cache_attention: q is [B, T, Hq, D]")
     B, T, Hq, D = q.shape
-    at = q.get_device()
-    kernel = _check_pages("kv_cache_attention", k_pages, v_pages, k_scales, v_scales, page_table, B, at)
+    _check_pages("kv_cache_attention", k_pages, v_pages, k_scales, v_scales, page_table, B, q.device)
     num_pages, H, page, Dk = k_pages.shape
     if Dk != D or H == 0 or Hq % H:
         raise ValueError(f"kv_cache_attention: {Hq} query heads of {D} over {H} heads of {Dk}")
-    mask = mb = mt = 0
-    if tree_mask is not None:
-        if tree_mask.dtype is not torch.bool or tree_mask.get_device() != at or tree_mask.shape not in ((T, T), (B, T, T)):
-            raise ValueError(f"kv_cache_attention: tree_mask is bool [{T}, {T}] or [{B}, {T}, {T}] on the device of q")
-        st = tree_mask.stride()
-        if st[-1] != 1:
-            tree_mask = tree_mask.contiguous()
-            st = tree_mask.stride()
-        mask, mt, mb = tree_mask.data_ptr(), st[-2], st[0] if len(st) == 3 else 0
+    if tree_mask is not None and (tree_mask.shape not in ((T, T), (B, T, T)) or tree_mask.dtype != torch.bool or tree_mask.device != q.device):
+        raise ValueError(f"kv_cache_attention: tree_mask is bool [{T}, {T}] or [{B}, {T}, {T}] on {q.device}")
     if max_len is not None and max_len < 0:
         raise ValueError("kv_cache_attention: max_len is not negative")
     _no_grad("kv_cache_attention", q)
-    start = _per_sequence("kv_cache_attention", "start", start, B, at)
+    start = _per_sequence("kv_cache_attention", "start", start, B, q.device)
     if counts is not None:
-        counts = _per_sequence("kv_cache_attention", "counts", counts, B, at)
-    scale = 1.0 / math.sqrt(D) if scale is None else scale
+        counts = _per_sequence("kv_cache_attention", "counts", counts, B, q.device)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0 <= scale < math.inf:
         raise ValueError(f"kv_cache_attention: scale is a number that is not negative, got {scale}")
-    limit = 0x7FFF0000 if max_len is None else min(max_len, 0x7FFF0000)
-    if kernel and q.dtype is torch.bfloat16 and page % 16 == 0 and page > 0:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        if out.numel() == 0:
+    limit = 0x7FFF0000 if max_len is None else min(int(max_len), 0x7FFF0000)
+    if q.is_cuda:
+        mask = tree_mask if tree_mask is None or tree_mask.stride(-1) == 1 else tree_mask.contiguous()
+        with torch.cuda.device(q.device):
+            out = nv.decode_calls().kv_attention(_rows(q), k_pages, v_pages, _table(page_table), start, mask, counts, k_scales, v_scales, scale, limit,
+                                                 nv.status_ptr(q.device))
+        if out is not None:
             return out
-        q, qp, qb, qt, qh = _aligned_rows(q)
-        table = _table(page_table)
-        ws = _workspace(q, B, T, Hq, H, D, at)
-        _ATTN(at, qp, qb, qt, qh, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), table.data_ptr(), table.stride(0),
-              start.data_ptr(), _ptr(counts), mask, mb, mt, out.data_ptr(), ws.data_ptr(), B, T, Hq, H, D, page, table.shape[1], num_pages,
-              limit, _KINDS[k_pages.dtype], nv.status_ptr(q.device), scale)
-        return out
     return _attention_plain(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, limit)
 
 
@@ -360,7 +311,7 @@ class PagedKVCache:
                  page: int = 64, num_pages: int | None = None, device="cuda"):
         if page <= 0 or page % 16:
             raise ValueError("PagedKVCache: pages hold a multiple of 16 tokens")
-        if dtype not in _KINDS and not (dtype.is_floating_point and dtype.itemsize > 1):
+        if dtype not in _CODES and not (dtype.is_floating_point and dtype.itemsize > 1):
             raise TypeError(f"PagedKVCache: bfloat16, int8 or float8_e4m3fn, got {dtype}")
         self.page, self.batch, self.dtype = page, batch, dtype
         per = -(-max_len // page)

@@ -12,11 +12,9 @@ import math
 
 import torch
 
-from ._dispatch import Record, kernel_ok
+from .. import _native as nv
 
-_ROTARY = Record("tb_rotary", "18qd")
 SCALINGS = ("none", "linear", "ntk", "yarn", "wavelength")
-_MAX_DIM = 512   # turned columns whose angles the kernel keeps
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, trained_len: int = 4096,
@@ -75,52 +73,6 @@ def _rotary_plain(x, positions, freqs, interleaved, magnitude, inverse):
     return torch.cat([turned, rest], -1).to(x.dtype)
 
 
-def _flat(x):
-    """``(x, token stride, head stride)`` of ``[..., H, D]`` with contiguous columns and one stride over all leading dimensions."""
-    st = x.stride()
-    if len(st) == 4:
-        if st[3] == 1 and (x.shape[0] == 1 or st[0] == x.shape[1] * st[1]):
-            return x, st[1], st[2]
-    elif len(st) == 3 and st[2] == 1:
-        return x, st[0], st[1]
-    x = x.contiguous()
-    return x, x.shape[-2] * x.shape[-1], x.shape[-1]
-
-
-def _launch(q, k, positions, freqs, interleaved, magnitude, inverse):
-    qc, ldq, lhq = _flat(q)
-    yq = torch.empty_like(q, memory_format=torch.contiguous_format)
-    D = q.shape[-1]
-    if k is None:
-        yk, kp, ykp, hk, ldk, lhk = None, 0, 0, 0, 0, 0
-    else:
-        kc, ldk, lhk = _flat(k)
-        yk = torch.empty_like(k, memory_format=torch.contiguous_format)
-        kp, ykp, hk = kc.data_ptr(), yk.data_ptr(), k.shape[-2]
-    _ROTARY(q.get_device(), qc.data_ptr(), kp, yq.data_ptr(), ykp, positions.data_ptr(), freqs.data_ptr(), positions.numel(), q.shape[-2],
-            hk, D, 2 * freqs.numel(), ldq, lhq, ldk, lhk, not interleaved, inverse, q.dtype is torch.float32, magnitude)
-    return yq, yk
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, freqs, interleaved, magnitude):
-        ctx.save_for_backward(positions, freqs)
-        ctx.form = (interleaved, magnitude)
-        ctx.like = (q.shape, q.dtype, None if k is None else k.shape)
-        return _launch(q, k, positions, freqs, interleaved, magnitude, False)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        # a rotation's gradient is the rotation back, with the same factor
-        positions, freqs = ctx.saved_tensors
-        qs, dt, ks = ctx.like
-        if ks is None:
-            return _launch(dq, None, positions, freqs, *ctx.form, True)[0], None, None, None, None, None
-        gq, gk = _launch(dq, dk, positions, freqs, *ctx.form, True)
-        return gq, gk, None, None, None, None
-
-
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool = True,
            magnitude: float = 1.0):
     """Turns queries and keys by their positions; returns ``(q', k')`` (``k'`` is None where ``k`` is).
@@ -130,6 +82,11 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     pair: ``2 * len(freqs)`` columns of ``D`` turn, the rest pass through. ``interleaved`` pairs columns ``(2i, 2i + 1)``, as
     :func:`~torsh_b200.ops.elementwise.rope` does; otherwise ``(i, i + len(freqs))``. Differentiable in ``q`` and ``k``.
     """
+    if q.is_cuda:
+        out = (nv._decode or nv.decode_calls()).rotary(q, k, positions, freqs, interleaved, magnitude)
+        if out is not None:
+            return out
+    # not as the kernel takes it: refused, converted, or computed here
     shape = q.shape
     if len(shape) < 2 or (k is not None and (k.shape[:-2] != shape[:-2] or k.shape[-1] != shape[-1] or k.dtype != q.dtype)):
         raise ValueError("rotary: q and k are [..., heads, D] of one type with the same leading dimensions and D")
@@ -146,13 +103,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     at = q.get_device()
     if positions.get_device() != at or freqs.get_device() != at or (k is not None and k.get_device() != at):
         raise ValueError("rotary: all tensors are on one device")
-    if kernel_ok(q, k) and 2 * freqs.numel() <= _MAX_DIM:
-        if positions.dtype is not torch.int64 or not positions.is_contiguous():
-            positions = positions.to(torch.int64).contiguous()
-        if freqs.dtype is not torch.float64 or not freqs.is_contiguous():
-            freqs = freqs.to(torch.float64).contiguous()
-        if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
-            return _Rotary.apply(q, k, positions, freqs, interleaved, float(magnitude))
-        return _launch(q, k, positions, freqs, interleaved, magnitude, False)
+    if q.is_cuda:
+        with torch.cuda.device(q.device):
+            out = nv.decode_calls().rotary(q, k, positions.to(torch.int64).contiguous(), freqs.to(torch.float64).contiguous(), interleaved, magnitude)
+        if out is not None:
+            return out
     f = freqs.to(torch.float64)
     return tuple(None if x is None else _rotary_plain(x, positions, f, interleaved, magnitude, False) for x in (q, k))

@@ -8,9 +8,8 @@ from __future__ import annotations
 
 import torch
 
-from ._dispatch import Record
+from .. import _native as nv
 
-_VERIFY = Record("tb_verify_draft", "16q")
 _MAX_NODES = 1024
 
 
@@ -59,34 +58,21 @@ def verify_draft(probs: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tens
     a sequence there are. Tokens outside the vocabulary and parents that do not come before their node are never accepted;
     a NaN or a negative number counts as no probability; where nothing has any, ``next_token`` is -1.
     """
+    if probs.is_cuda:
+        out = (nv._decode or nv.decode_calls()).verify(probs, tokens, uniforms, draft_probs, parents, counts)
+        if out is not None:
+            return out
+    # not as the kernel takes it: refused, converted, or computed here
     _check(probs, tokens, uniforms, draft_probs, parents, counts)
-    if not probs.is_cuda:
-        return _verify_plain(probs, tokens, uniforms, draft_probs, parents, counts)
-    B, T, V = probs.shape
-    pb, pt, step = probs.stride()
-    if step != 1:
-        probs = probs.contiguous()
-        pb, pt, _ = probs.stride()
-    dp = db = dt = 0
-    if draft_probs is not None and T > 1:
-        if draft_probs.stride(2) != 1:
-            draft_probs = draft_probs.contiguous()
-        dp = draft_probs.data_ptr()
-        db, dt, _ = draft_probs.stride()
-    if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
-        tokens = tokens.to(torch.int64).contiguous()
-    if uniforms.dtype is not torch.float32 or not uniforms.is_contiguous():
-        uniforms = uniforms.to(torch.float32).contiguous()
-    if parents is not None and (parents.dtype is not torch.int64 or not parents.is_contiguous()):
-        parents = parents.to(torch.int64).contiguous()
-    if counts is not None and (counts.dtype is not torch.int32 or not counts.is_contiguous()):
-        counts = counts.to(torch.int32).contiguous()
-    out = torch.empty(B * (T + 2), dtype=torch.int64, device=probs.device)
-    _VERIFY(probs.get_device(), probs.data_ptr(), dp, pb, pt, db, dt, tokens.data_ptr(), 0 if parents is None else parents.data_ptr(),
-            T if parents is not None and parents.dim() == 2 else 0, uniforms.data_ptr(), 0 if counts is None else counts.data_ptr(), out.data_ptr(),
-            B, T, V, probs.dtype is torch.float32)
-    accepted, nxt, path = out.split([B, B, B * T])
-    return accepted, path.view(B, T), nxt
+    if probs.is_cuda:
+        rows = lambda x: x if x is None or x.stride(2) == 1 else x.contiguous()   # noqa: E731
+        as_ = lambda x, t: x if x is None else x.to(t).contiguous()   # noqa: E731
+        with torch.cuda.device(probs.device):
+            out = nv.decode_calls().verify(rows(probs), as_(tokens, torch.int64), as_(uniforms, torch.float32), rows(draft_probs), as_(parents, torch.int64),
+                                           as_(counts, torch.int32))
+        if out is not None:
+            return out
+    return _verify_plain(probs, tokens, uniforms, draft_probs, parents, counts)
 
 
 def _verify_plain(probs, tokens, uniforms, draft_probs=None, parents=None, counts=None):
