@@ -243,3 +243,61 @@ def test_verify_refusals(bad, exc):
     verify_draft(**kw)
     with pytest.raises(exc):
         verify_draft(**{**kw, **bad})
+
+
+# ------------------------------------------------------------------------------------------------ together
+def _llama(layers=2, seed=0, hidden=32, heads=2):
+    from torsh_b200.models.llama import LlamaConfig, LlamaModel
+    torch.manual_seed(seed)
+    m = LlamaModel(LlamaConfig(vocab_size=50, hidden_size=hidden, intermediate_size=64, num_layers=layers, num_heads=heads, max_seq_len=256, initializer_range=0.3))
+    return m.eval()
+
+
+def _greedy(m, ids, n):
+    with torch.no_grad():
+        for _ in range(n):
+            ids = torch.cat([ids, m(ids)[:, -1].argmax(-1, keepdim=True)], 1)
+    return ids
+
+
+@pytest.mark.parametrize("S", [1, 5])
+def test_generate_from_a_cache_is_the_whole_context_run_again(S):
+    m, small = _llama(), _llama(1, 7)
+    ids = torch.randint(0, 50, (3, S))
+    want = _greedy(m, ids, 20)
+    assert torch.equal(m.generate(ids, 20), want)
+    for draft, k in ((small, 1), (small, 3), (m, 4)):      # the model itself as the draft: everything is accepted
+        assert torch.equal(m.generate(ids, 20, draft=draft, drafted=k), want)
+    assert m.generate(ids, 0) is ids
+    assert m.generate(ids, 7, cache_dtype=torch.int8).shape == (3, S + 7)
+
+
+def test_generate_samples_and_refuses():
+    m, small = _llama(), _llama(1, 7)
+    ids = torch.randint(0, 50, (2, 4))
+    g = lambda: torch.Generator().manual_seed(3)   # noqa: E731
+    assert torch.equal(m.generate(ids, 9, 1.0, generator=g()), m.generate(ids, 9, 1.0, generator=g()))
+    assert m.generate(ids, 9, 1.0, draft=small, generator=g()).shape == (2, 13)
+    for bad in (dict(temperature=-1.0), dict(draft=small, drafted=0)):
+        with pytest.raises(ValueError):
+            m.generate(ids, 2, **bad)
+
+
+def test_decode_of_a_tree_gives_each_path_its_own_states():
+    m = _llama()
+    ids = torch.randint(0, 50, (2, 6))
+    c = m.make_cache(2, 40, page=16)
+    c.reserve(6)
+    m.decode(ids, c)
+    c.advance(6)
+    parents = torch.tensor([-1, 0, 0, 1, 2])
+    tokens = torch.randint(0, 50, (2, 5))
+    mask = tree_mask_of(parents)
+    c.reserve(5)
+    h = m.decode(tokens, c, mask).view(2, 5, -1)
+    for i in range(5):
+        path = mask[i].nonzero().flatten()
+        flat = m.make_cache(2, 40, page=16)
+        flat.reserve(6 + len(path))
+        want = m.decode(torch.cat([ids, tokens[:, path]], 1), flat).view(2, 6 + len(path), -1)[:, -1]
+        torch.testing.assert_close(h[:, i], want, rtol=1e-4, atol=1e-4)

@@ -583,3 +583,37 @@ def test_a_tree_step_through_the_cache(dtype):
     assert cache.host_lengths == chain.host_lengths
     for x, y in zip(cache.read(0), chain.read(0)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("cache_dtype", [BF16, E4M3])
+def test_llama_decodes_from_the_cache(cache_dtype):
+    """Hidden states of the last tokens, prompt and steps through the cache, are as near to fp32 as those of the whole context run at once
+    (twice as far at most; an e4m3 cache rounds keys and values by 2^-4 where bf16 does by 2^-8: sixteen times)."""
+    from torsh_b200.models.llama import LlamaConfig, LlamaModel
+    torch.manual_seed(0)
+    cfg = LlamaConfig.tiny(num_layers=3, initializer_range=0.05)
+    m = LlamaModel(cfg).to(DEV, BF16).eval()
+    ref = LlamaModel(cfg).double().eval()
+    ref.load_state_dict({k: v.double().cpu() for k, v in m.state_dict().items()})
+    ids = torch.randint(0, cfg.vocab_size, (3, 70), device=DEV)
+    with torch.no_grad():
+        want = ref.decode(ids.cpu(), ref.make_cache(3, 80)).view(3, 70, -1)
+        whole = m.decode(ids, _primed(m, 3, 80, BF16, 70)).view(3, 70, -1)
+        c = _primed(m, 3, 80, cache_dtype, 60)
+        got = [m.decode(ids[:, :60], c).view(3, 60, -1)]
+        c.advance(60)
+        for i in range(60, 70):
+            c.reserve(1)
+            got.append(m.decode(ids[:, i:i + 1], c).view(3, 1, -1))
+            c.advance(1)
+    got = torch.cat(got, 1)
+    off = lambda x: (x.double().cpu() - want).norm()   # noqa: E731
+    assert off(got) <= (2 if cache_dtype == BF16 else 16) * off(whole)
+    out = m.generate(ids[:, :9], 12, draft=m, drafted=3, cache_dtype=cache_dtype)
+    assert out.shape == (3, 21) and torch.equal(out[:, :9], ids[:, :9])
+
+
+def _primed(m, batch, most, dtype, n):
+    c = m.make_cache(batch, most, dtype, page=16)
+    c.reserve(n)
+    return c

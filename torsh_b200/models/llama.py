@@ -18,9 +18,12 @@ import torch
 from .. import nn
 from ..ops import attention as attn_ops
 from ..ops import elementwise as ew
+from ..ops import kv_cache as kv_ops
 from ..ops import linear as lin_ops
 from ..ops import norm as norm_ops
+from ..ops import rotary as rot_ops
 from ..ops import softmax as sm_ops
+from ..ops import speculative as spec_ops
 
 
 @dataclass
@@ -92,6 +95,18 @@ class LlamaBlock(nn.Module):
         ctx = attn_ops.rope_flash_attention_qkvpacked(qkv, B, S, H, D, cfg.rope_theta)
         x = self.o(ctx, residual=x)
         h, x = norm_ops.rms_norm_fork(x, self.post_attn_norm.weight, cfg.rms_eps)
+        return self.down(ew.swiglu(self.gate_up(h)), residual=x)
+
+
+    def step(self, x, B: int, T: int, cache, layer: int, positions, freqs, tree_mask=None, counts=None):
+        """``T`` new tokens per sequence on top of ``cache`` (:class:`~torsh_b200.ops.kv_cache.PagedKVCache`), which gets their keys and values."""
+        cfg, H, D = self.cfg, self.local_heads, self.cfg.head_dim
+        h = norm_ops.rms_norm(x, self.input_norm.weight, cfg.rms_eps)
+        qkv = self.qkv(h).view(B, T, 3, H, D)
+        q, k = rot_ops.rotary(qkv[:, :, 0], qkv[:, :, 1], positions, freqs)
+        cache.write(layer, k, qkv[:, :, 2], counts)
+        x = self.o(cache.attend(layer, q, tree_mask, counts).reshape(B * T, H * D), residual=x)
+        h = norm_ops.rms_norm(x, self.post_attn_norm.weight, cfg.rms_eps)
         return self.down(ew.swiglu(self.gate_up(h)), residual=x)
 
 
@@ -168,6 +183,93 @@ class LlamaModel(nn.Module):
         if targets is None:
             return logits.view(B, S, -1)[..., : self.cfg.vocab_size]
         return sm_ops.cross_entropy(logits, targets.reshape(-1), num_classes=self.cfg.vocab_size)
+
+    # ------------------------------------------------------------------------------------------------ generation
+    def make_cache(self, batch: int, max_len: int, dtype: torch.dtype | None = None, page: int = 64):
+        """A cache for ``batch`` sequences of up to ``max_len`` tokens; ``dtype`` is the weights' unless given (int8 and float8_e4m3fn hold half)."""
+        cfg = self.cfg
+        return kv_ops.PagedKVCache(len(self.layers), cfg.num_heads, cfg.head_dim, batch, max_len, dtype or self.embed.dtype, page, device=self.embed.device)
+
+    @torch.no_grad()
+    def decode(self, tokens: torch.Tensor, cache, tree_mask: torch.Tensor | None = None, counts: torch.Tensor | None = None):
+        """Hidden states ``[B * T, E]`` (after the final norm) of ``T`` new tokens per sequence on top of the cache, which gets their keys
+        and values; its lengths stay (:meth:`~torsh_b200.ops.kv_cache.PagedKVCache.advance` keeps them). With ``tree_mask`` a token's
+        position is its depth in the tree."""
+        if not (self.first_stage and self.last_stage) or self.tp is not None:
+            raise NotImplementedError("LlamaModel.decode: the whole model on one device")
+        B, T = tokens.shape
+        if not hasattr(self, "_rotary_freqs") or self._rotary_freqs.device != tokens.device:
+            self._rotary_freqs = rot_ops.rotary_frequencies(self.cfg.head_dim, self.cfg.rope_theta, device=tokens.device)[0]
+        depth = torch.arange(T, device=tokens.device) if tree_mask is None else tree_mask.sum(-1) - 1
+        positions = cache.lengths.long()[:, None] + depth
+        x = ew.embedding(tokens, self.embed).reshape(B * T, -1)
+        for i, blk in enumerate(self.layers):
+            x = blk.step(x, B, T, cache, i, positions, self._rotary_freqs, tree_mask, counts)
+        return norm_ops.rms_norm(x, self.norm.weight, self.cfg.rms_eps)
+
+    def _probs(self, h, temperature: float):
+        """fp32 probabilities ``[rows, V]`` of the next token; all on the likeliest one at temperature 0."""
+        logits = lin_ops.linear(h, self.lm_head, None)[:, : self.cfg.vocab_size].float()
+        if temperature == 0:
+            return torch.zeros_like(logits).scatter_(1, logits.argmax(-1, keepdim=True), 1.0)
+        return torch.softmax(logits / temperature, -1)
+
+    @torch.no_grad()
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 0.0, draft: "LlamaModel | None" = None, drafted: int = 4,
+                 cache_dtype: torch.dtype | None = None, generator: torch.Generator | None = None) -> torch.Tensor:
+        """``input_ids [B, S]`` and ``max_new_tokens`` more tokens each, from a cache of keys and values instead of running the context again.
+
+        With ``draft`` (a smaller model over the same vocabulary) each round drafts ``drafted`` tokens and verifies them in one pass of this
+        model (:func:`~torsh_b200.ops.speculative.verify_draft`): the tokens are distributed as without it, and the same at temperature 0
+        up to the rounding of sums over different numbers of rows."""
+        if temperature < 0:
+            raise ValueError("generate: temperature is not negative")
+        if draft is not None and (draft.cfg.vocab_size != self.cfg.vocab_size or drafted < 1):
+            raise ValueError("generate: the draft model has the same vocabulary, and drafts at least one token")
+        B, S = input_ids.shape
+        if S == 0 or max_new_tokens <= 0:
+            return input_ids
+        dev = input_ids.device
+        room = S + max_new_tokens + (drafted if draft is not None else 0)
+        rand = lambda *s: torch.rand(*s, device=dev, generator=generator)   # noqa: E731
+        models = [self] if draft is None else [self, draft]
+        caches = [m.make_cache(B, room + 1, cache_dtype) for m in models]
+        for m, c in zip(models, caches):            # all of the prompt but its last token, which the first step feeds
+            if S > 1:
+                c.reserve(S - 1)
+                m.decode(input_ids[:, :-1], c)
+                c.advance(S - 1)
+        done = [input_ids[b].tolist() for b in range(B)]
+        last = input_ids[:, -1:]
+        while min(len(d) for d in done) < S + max_new_tokens:
+            T = 1 if draft is None else drafted + 1
+            tokens, q = last, []
+            if draft is not None:
+                c = caches[1]
+                c.reserve(T)
+                for _ in range(drafted):            # one token more than is drafted: its keys are needed where all are accepted
+                    p = draft._probs(draft.decode(tokens[:, -1:], c), temperature)
+                    c.advance(1)
+                    nxt = spec_ops.verify_draft(p[:, None], tokens[:, -1:], rand(B, 1))[2]
+                    tokens, q = torch.cat([tokens, nxt[:, None]], 1), q + [p]
+                draft.decode(tokens[:, -1:], c)
+                c.advance(1)
+            caches[0].reserve(T)
+            probs = self._probs(self.decode(tokens, caches[0]), temperature).view(B, T, -1)
+            taken, _, nxt = spec_ops.verify_draft(probs, tokens, rand(B, T), torch.stack(q, 1) if q else None)
+            took = taken.tolist()
+            caches[0].advance([n + 1 for n in took])
+            for b, (n, more) in enumerate(zip(took, torch.cat([tokens[:, 1:], nxt[:, None]], 1).tolist())):
+                done[b] += more[:n] + more[-1:]
+            if draft is not None:
+                caches[1].truncate(caches[0].host_lengths)
+            last = nxt[:, None]
+            full = [b for b in range(B) if len(done[b]) >= S + max_new_tokens]
+            for b in full:                          # sequences that are done stay where they are: no room beyond is asked for
+                keep = min(caches[0].host_lengths[b], S + max_new_tokens - 1)
+                for c in caches:
+                    c.truncate([keep if i == b else n for i, n in enumerate(c.host_lengths)])
+        return torch.tensor([d[: S + max_new_tokens] for d in done], dtype=input_ids.dtype, device=dev)
 
 
 LlamaForCausalLM = LlamaModel

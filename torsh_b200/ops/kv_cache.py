@@ -1,7 +1,8 @@
 """Paged cache of keys and values in 16 or 8 bits: writing, reading back, and attention of the newest tokens over it.
 
-Kernels: ``csrc/kernels/kv_cache.cu`` and ``csrc/kernels/cache_attention.cu``; CPU tensors, and types or head sizes that the kernels do
-not take, run the same formulas in PyTorch. The reference has no cache: its generation loop runs the whole context through the model
+Kernels: ``csrc/kernels/kv_cache.cu``, ``csrc/kernels/cache_attention.cu`` (up to 16 query rows to a head of the cache) and
+``csrc/kernels/cache_attention_sm100.cu`` (more); CPU tensors, and types or head sizes that the kernels do not take, run the same
+formulas in PyTorch. The reference has no cache: its generation loop runs the whole context through the model
 for every token (``crates/torsh-text/src/generation.rs``).
 
 Layout: ``k_pages`` and ``v_pages`` are ``[num_pages, H, page, D]`` (a page holds ``page`` consecutive tokens of one sequence, a
@@ -353,7 +354,8 @@ class PagedKVCache:
                scale: float | None = None) -> torch.Tensor:
         """:func:`kv_cache_attention` of tokens that :meth:`write` has just written."""
         (kp, vp), (ks, vs) = self.layers[layer], self.scales[layer]
-        return kv_cache_attention(q, kp, vp, self.page_table, self.lengths, tree_mask, counts, ks, vs, scale)
+        longest = max(self.host_lengths, default=0) + q.shape[1]
+        return kv_cache_attention(q, kp, vp, self.page_table, self.lengths, tree_mask, counts, ks, vs, scale, longest)
 
     def read(self, layer: int, dtype: torch.dtype = torch.bfloat16):
         """All keys and values of a layer, ``[B, longest, H, D]``."""
@@ -388,6 +390,14 @@ class PagedKVCache:
         tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
         self.lengths += torch.tensor(tokens, dtype=torch.int32, device=self.lengths.device)
         self.host_lengths = [n + t for n, t in zip(self.host_lengths, tokens)]
+
+    def truncate(self, lengths) -> None:
+        """Shortens the sequences to ``lengths`` (one per sequence): what lies behind is written over. Their pages stay theirs."""
+        lengths = [int(n) for n in lengths]
+        if len(lengths) != self.batch or any(not 0 <= n <= was for n, was in zip(lengths, self.host_lengths)):
+            raise ValueError(f"PagedKVCache: lengths {lengths} of sequences that have {self.host_lengths}")
+        self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        self.host_lengths = lengths
 
     def release(self, b: int) -> None:
         """Gives sequence ``b``'s pages back; its place takes a new sequence from position 0."""
