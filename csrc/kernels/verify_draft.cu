@@ -75,29 +75,29 @@ __device__ __forceinline__ double mass_at(const Row& r, int c, int end) {
 }
 template <typename T>
 __device__ __forceinline__ double sum_range(const Row& r, int c0, int end, int lane) {
-  double part[4] = {0.0, 0.0, 0.0, 0.0}, sum = 0.0;
-  int c = c0 + lane;
-  for (; c + 32 * (VD_UNROLL - 1) < end; c += 32 * VD_UNROLL) {
+  double part[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int c = c0 + lane; c < end; c += 32 * VD_UNROLL) {
     float p[VD_UNROLL], q[VD_UNROLL];
 #pragma unroll
-    for (int i = 0; i < VD_UNROLL; ++i) p[i] = to_f<T>(((const T*)r.p)[c + 32 * i]);
+    for (int i = 0; i < VD_UNROLL; ++i) p[i] = c + 32 * i < end ? to_f<T>(((const T*)r.p)[c + 32 * i]) : 0.f;
     if (r.q) {
 #pragma unroll
-      for (int i = 0; i < VD_UNROLL; ++i) q[i] = to_f<T>(((const T*)r.q)[c + 32 * i]);
+      for (int i = 0; i < VD_UNROLL; ++i) q[i] = c + 32 * i < end ? to_f<T>(((const T*)r.q)[c + 32 * i]) : 0.f;
     } else {
 #pragma unroll
       for (int i = 0; i < VD_UNROLL; ++i) q[i] = 0.f;
     }
+    if (r.out) {
 #pragma unroll
-    for (int i = 0; i < VD_UNROLL; ++i) {
-      const int at = c + 32 * i - r.base;
-      const bool gone = r.out && ((r.out[at >> 5] >> (at & 31)) & 1u);
-      part[i & 3] += gone ? 0.0 : mass_of(p[i], q[i]);
+      for (int i = 0; i < VD_UNROLL; ++i) {
+        const int at = c + 32 * i - r.base;
+        if (c + 32 * i < end && ((r.out[at >> 5] >> (at & 31)) & 1u)) p[i] = 0.f;
+      }
     }
+#pragma unroll
+    for (int i = 0; i < VD_UNROLL; ++i) part[i & 3] += mass_of(p[i], q[i]);
   }
-  sum = (part[0] + part[1]) + (part[2] + part[3]);
-  for (; c < end; c += 32) sum += mass_at<T>(r, c, end);
-  return warp_sum_d(sum);
+  return warp_sum_d((part[0] + part[1]) + (part[2] + part[3]));
 }
 
 // Of the masses of 32 N consecutive ranges (lane l of a warp holds m[0 .. N-1] of ranges N l ..): the range in which the running sum,
@@ -152,15 +152,16 @@ __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_WARPS * 
   const float* u = a.uniforms + (long)b * a.T;
   const float last_u = u[a.T - 1];
 
-  for (int i = tid; i < n; i += VD_THREADS) {
+  for (int i = tid; i < a.T; i += VD_THREADS) {          // not up to n: its load is under way, too
     const long tk = a.tokens[(long)b * a.T + i];
     const long pr = par ? par[i] : i - 1;
-    const bool ok = i > 0 && tk >= 0 && tk < a.V && pr >= 0 && pr < i;   // anything else is never accepted
-    if (i > 0 && !ok) report_bad_index();
+    const float un = u[i];
+    const bool ok = i > 0 && i < n && tk >= 0 && tk < a.V && pr >= 0 && pr < i;   // anything else is never accepted
+    if (i > 0 && i < n && !ok) report_bad_index();
     parent[i] = ok ? (int)pr : -1;
     token[i] = ok ? (int)tk : -1;
     mass[i] = ok ? to_f<T>(probs[pr * a.pt + tk]) : 0.f;
-    num[i] = u[i];
+    num[i] = un;
     dmass[i] = ok && draft ? to_f<T>(draft[pr * a.dt + tk]) : 0.f;
   }
   for (int i = tid; i < words; i += VD_THREADS) out_bits[i] = 0;
@@ -258,13 +259,16 @@ __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_WARPS * 
   __shared__ double chunk[VD_MAX_CHUNKS];
   const int c0 = hit * len, c1 = min(c0 + len, a.V), wide = max(256, ((len / 32 + VD_MAX_CHUNKS - 1) / VD_MAX_CHUNKS) * 32);
   const int chunks = (c1 - c0 + wide - 1) / wide;
-  for (int k = warp; k < VD_MAX_CHUNKS; k += VD_WARPS) {
-    const double s = k < chunks ? sum_range<T>(row, c0 + k * wide, min(c0 + (k + 1) * wide, c1), lane) : 0.0;
-    if (lane == 0) chunk[k] = s;
+  if (chunks > 1) {
+    for (int k = warp; k < VD_MAX_CHUNKS; k += VD_WARPS) {
+      const double s = k < chunks ? sum_range<T>(row, c0 + k * wide, min(c0 + (k + 1) * wide, c1), lane) : 0.0;
+      if (lane == 0) chunk[k] = s;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (warp) return;
-  {
+  hit = 0;
+  if (chunks > 1) {
     double m[VD_MAX_CHUNKS / 32];
 #pragma unroll
     for (int i = 0; i < VD_MAX_CHUNKS / 32; ++i) m[i] = chunk[VD_MAX_CHUNKS / 32 * lane + i];
