@@ -97,7 +97,8 @@ bool pages_ok(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor
     if (s->defined() && (!here(*s, device) || s->scalar_type() != at::kFloat || s->sizes() != kp.sizes().slice(0, 3) || !s->is_contiguous() || !aligned(s->const_data_ptr())))
       return false;
   }
-  return here(table, device) && table.dim() == 2 && table.size(0) == B && table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1);
+  // an empty pool or table holds nothing: the formulas in PyTorch say so
+  return here(table, device) && kp.numel() > 0 && table.numel() > 0 && table.dim() == 2 && table.size(0) == B && table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1);
 }
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? (T*)t.const_data_ptr() : nullptr; }

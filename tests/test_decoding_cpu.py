@@ -130,6 +130,39 @@ def test_cpu_attention_keeps_what_is_not_seen_apart():
     assert not none.any()
 
 
+@pytest.mark.parametrize("B,T", [(0, 3), (2, 0)])
+def test_attention_over_nothing(B, T):
+    kp, vp = torch.randn(2, 1, 16, 8), torch.randn(2, 1, 16, 8)
+    table, start = torch.zeros(B, 1, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
+    assert kv_cache_attention(torch.randn(B, T, 2, 8), kp, vp, table, start).shape == (B, T, 2, 8)
+    kv_cache_write(torch.randn(B, T, 1, 8), torch.randn(B, T, 1, 8), kp, vp, table, start)
+    assert kv_cache_read(kp, vp, table, start, 4)[0].shape == (B, 4, 1, 8)
+
+
+def test_an_empty_pool_or_table_holds_nothing():
+    k = torch.randn(2, 3, 1, 8)
+    for pages, width in ((0, 2), (2, 0)):
+        kp, vp = torch.zeros(pages, 1, 16, 8), torch.zeros(pages, 1, 16, 8)
+        table, start = torch.zeros(2, width, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+        kv_cache_write(k, k, kp, vp, table, start)
+        assert not kp.any() and not kv_cache_read(kp, vp, table, start + 3, 3)[0].any()
+        assert not kv_cache_attention(k, kp, vp, table, start).any()
+
+
+def test_negative_starts_and_integers_beyond_32_bits():
+    kp, vp = torch.zeros(2, 1, 16, 8), torch.zeros(2, 1, 16, 8)
+    table = torch.tensor([[0], [1]])
+    k = torch.ones(2, 4, 1, 8)
+    kv_cache_write(k, k, kp, vp, table, torch.tensor([-2, -1]))             # these sequences are left out
+    kv_cache_write(k, k, kp, vp, table, torch.tensor([1 << 32, -(1 << 32)]))
+    kv_cache_write(k, k, kp, vp, table + (1 << 32), torch.tensor([0, 0]))   # no pages of the pool
+    assert not kp.any()
+    kv_cache_write(k, k, kp, vp, table, torch.tensor([0, 2]), torch.tensor([1 << 32, 1]))
+    assert kp[0, 0, :4].eq(1).all() and kp[1, 0, 2].eq(1).all() and kp.sum() == 5 * 8
+    rk, _ = kv_cache_read(kp, vp, table, torch.tensor([1 << 33, 3]), 4)
+    assert rk[0].eq(1).all() and rk[1, 2].eq(1).all() and rk.float().sum() == 5 * 8
+
+
 def test_tree_masks():
     parents = torch.tensor([-1, 0, 1, 1, 0, 4, -1])
     m = tree_mask_of(parents)

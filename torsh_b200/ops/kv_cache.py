@@ -52,7 +52,12 @@ def _per_sequence(what, name, t, B, device):
     """A vector of B integers as the kernels read it."""
     if t.shape != (B,) or t.is_floating_point() or t.device != device:
         raise ValueError(f"{what}: {name} is a vector of {B} integers on {device}")
-    return t.to(torch.int32).contiguous()
+    return _int32(t).contiguous()
+
+
+def _int32(t):
+    """As 32-bit integers; what does not fit becomes the next that does, which no table reaches and no pool has."""
+    return t.clamp(-0x80000000, 0x7FFFFFFF).to(torch.int32) if t.dtype == torch.int64 else t.to(torch.int32)
 
 
 def _no_grad(what, *tensors):
@@ -61,7 +66,7 @@ def _no_grad(what, *tensors):
 
 
 def _table(page_table):
-    return page_table if page_table.dtype is torch.int32 and page_table.stride(1) == 1 else page_table.to(torch.int32).contiguous()
+    return page_table if page_table.dtype is torch.int32 and page_table.stride(1) == 1 else _int32(page_table).contiguous()
 
 
 def _rows(x):
@@ -123,8 +128,8 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     """Writes the keys and values of ``T`` new tokens per sequence into their pages, quantised to the pages' type.
 
     ``k`` and ``v`` are ``[B, T, H, D]``; token ``t`` of sequence ``b`` goes to position ``start[b] + t``, tokens from ``counts[b]`` on are
-    left out. Positions that the table does not reach, or to which it gives a page outside the pool, are skipped (and reported where
-    the device-side index checks are on). Two sequences may share pages, but not the positions that one call writes.
+    left out, and so are sequences whose ``start`` is negative. Positions that the table does not reach, or to which it gives a page
+    outside the pool, are skipped (and reported where the device-side index checks are on). Two sequences may share pages, but not the positions that one call writes.
     """
     if k.is_cuda and (nv._decode or nv.decode_calls()).kv_write(k, v, k_pages, v_pages, page_table, start, counts, k_scales, v_scales):
         return
@@ -148,6 +153,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
                 return
     at = torch.arange(T, device=k.device)
     slot, row, there = _slots(page_table, num_pages, page, start.long()[:, None] + at)
+    there = there & (start >= 0)[:, None]
     if counts is not None:
         there = there & (at < counts[:, None])
     slot, row = slot[there], row[there]
@@ -205,7 +211,7 @@ def _attention_plain(q, k_pages, v_pages, page_table, start, tree_mask, counts, 
     start = start.long().clamp(min=0)
     live = torch.full((B,), T, device=dev) if counts is None else counts.long().clamp(0, T)
     n = min(limit, page_table.shape[1] * page)
-    if n:
+    if n and B:
         n = min(n, int((start + live).max()))
     at = torch.arange(n, device=dev)
     slot, row, there = _slots(page_table, num_pages, page, at[None].expand(B, -1))
@@ -248,6 +254,9 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     ordinary decoding step. Rows from ``counts[b]`` on, and rows that see nothing, come out as zeros; infinities and NaN in
     places that a row does not see do not reach it. ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
     not read. Pages outside the pool read as zeros. No backward pass.
+
+    For more than 16 query rows to a head of the cache the kernel turns 8-bit values into halves relative to the largest scale of their 32
+    positions: a value whose scale is less than 2^-25 of a neighbour's counts as zero, whether or not the row sees that neighbour.
     """
     if q.is_cuda:
         out = (nv._decode or nv.decode_calls()).kv_attention(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, max_len,

@@ -69,7 +69,7 @@ def verify_draft(probs: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tens
         as_ = lambda x, t: x if x is None else x.to(t).contiguous()   # noqa: E731
         with torch.cuda.device(probs.device):
             out = nv.decode_calls().verify(rows(probs), as_(tokens, torch.int64), as_(uniforms, torch.float32), rows(draft_probs), as_(parents, torch.int64),
-                                           as_(counts, torch.int32))
+                                           None if counts is None else counts.clamp(1, probs.shape[1]).to(torch.int32).contiguous())
         if out is not None:
             return out
     return _verify_plain(probs, tokens, uniforms, draft_probs, parents, counts)
