@@ -617,3 +617,220 @@ def _primed(m, batch, most, dtype, n):
     c = m.make_cache(batch, most, dtype, page=16)
     c.reserve(n)
     return c
+
+
+# ------------------------------------------------------------------------------------------------ at the edges of the documentation
+@pytest.mark.parametrize("G", [2, 24])
+@pytest.mark.parametrize("dtype", [torch.int8, E4M3])
+def test_cache_attention_scales_below_zero(dtype, G):
+    """Scales of a caller's own may have any sign."""
+    from torsh_b200.ops.kv_cache import kv_cache_attention
+    q, kp, vp, ks, vs, table, start = _case(2, 3, 2 * G, 2, 128, 16, [300, 41], dtype)
+    ks, vs = (x * torch.where(torch.rand(x.shape, device=DEV, generator=_gen(i)) < 0.5, -1, 1) for i, x in enumerate((ks, vs)))
+    got = kv_cache_attention(q, kp, vp, table, start, None, None, ks, vs)
+    _attention_close(got, *_attend64(q, kp, vp, ks, vs, table, start, None, None, 128 ** -0.5), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.int8])
+@pytest.mark.parametrize("shape", [(2, 1500, 4, 2, 64, 48, [0, 70]), (1, 700, 2, 1, 128, 80, [0]), (4, 20, 3, 3, 64, 16, [5, 0, 33, 1])])
+def test_cache_attention_of_a_prompt(dtype, shape):
+    """Prompts: many row tiles that begin in the middle of a key tile, most of them without a context, with pages of no power of two."""
+    from torsh_b200.ops.kv_cache import kv_cache_attention
+    q, kp, vp, ks, vs, table, start = _case(*shape, dtype)
+    B, T, _, _, D = shape[:5]
+    got = kv_cache_attention(q, kp, vp, table, start, None, None, ks, vs)
+    _attention_close(got, *_attend64(q, kp, vp, ks, vs, table, start, None, None, D ** -0.5), dtype)
+    # a mask that is a view of a larger one, off any boundary and with rows of odd length
+    big = torch.rand(T + 3, T + 5, device=DEV, generator=_gen(T)) < 0.3
+    mask = big[1:T + 1, 3:T + 3]
+    got = kv_cache_attention(q, kp, vp, table, start, mask, None, ks, vs)
+    _attention_close(got, *_attend64(q, kp, vp, ks, vs, table, start, mask, None, D ** -0.5), dtype)
+    assert torch.equal(got, kv_cache_attention(q, kp, vp, table, start, mask.contiguous(), None, ks, vs))
+
+
+def test_cache_calls_on_many_sequences_and_on_none():
+    from torsh_b200.ops.kv_cache import kv_cache_attention, kv_cache_read, kv_cache_write
+    B = 70000
+    kp, vp, ks, vs = _cache(300, 1, 16, 64, torch.int8, 1)
+    table = (torch.arange(B, device=DEV) % 300).int()[:, None]
+    start = (torch.arange(B, device=DEV) % 17 - 1).int()                    # a negative start is no context
+    q = torch.randn(B, 1, 2, 64, device=DEV, generator=_gen(0)).to(BF16)
+    got = kv_cache_attention(q, kp, vp, table, start, None, None, ks, vs)
+    want = torch.where((start >= 16)[:, None, None, None], 7.0, 7.0)        # every value is code 1 times scale 7
+    assert ((got.float() - want).abs() <= 7 * 2.0 ** -8).all()
+    for n in (0, 1):
+        e, t = q[:n], table[:n]
+        assert kv_cache_attention(e, kp, vp, t, start[:n], None, None, ks, vs).shape == e.shape
+        assert kv_cache_attention(e[:, :0], kp, vp, t, start[:n], None, None, ks, vs).shape == (n, 0, 2, 64)
+        assert kv_cache_read(kp, vp, t, start[:n], 0, None, ks, vs)[0].shape == (n, 0, 1, 64)
+    kv_cache_write(q[:0, :, :1], q[:0, :, :1], kp, vp, table[:0], start[:0], None, ks, vs)
+    for pool, wide in ((0, 1), (300, 0)):                                   # an empty pool, a table without columns
+        args = kp[:pool], vp[:pool], table[:3, :wide]
+        kv_cache_write(q[:3, :, :1], q[:3, :, :1], *args, start[:3], None, ks[:pool], vs[:pool])
+        assert not kv_cache_read(*args, start[3:6], 4, None, ks[:pool], vs[:pool])[0].any()
+        assert not kv_cache_attention(q[:3], *args, start[3:6], None, None, ks[:pool], vs[:pool]).any()
+
+
+def test_cache_integers_beyond_32_bits_are_not_wrapped():
+    from torsh_b200.ops.kv_cache import kv_cache_attention, kv_cache_read, kv_cache_write
+    kp, vp, _, _ = _cache(2, 1, 16, 64, BF16, 0)
+    table = torch.tensor([[0], [1]], device=DEV)
+    k = torch.ones(2, 4, 1, 64, device=DEV, dtype=BF16)
+    for tab, start in ((table, [1 << 32, -(1 << 32)]), (table, [-1, 1 << 31]), (table + (1 << 32), [0, 0])):
+        kv_cache_write(k, k, kp, vp, tab, torch.tensor(start, device=DEV))
+        kv_cache_write(k, k, kp, vp, tab.clamp(max=2 ** 31 - 1).int(), torch.tensor(start, device=DEV).clamp(-2 ** 31, 2 ** 31 - 1).int())
+    assert not kp.any()
+    kv_cache_write(k, k, kp, vp, table, torch.tensor([0, 12], device=DEV))
+    big = torch.tensor([2 ** 31 - 1, 1 << 40], device=DEV)
+    rk, _ = kv_cache_read(kp, vp, table, big, 16)
+    assert torch.equal(rk[:, :, 0], kp[:, 0])
+    assert not kv_cache_read(kp, vp, table, big, 16, big)[0].any()
+    got = kv_cache_attention(k, kp, vp, table, big, scale=0.0)              # all that the tables reach, alike: a quarter is ones
+    assert got.eq(0.25).all()
+
+
+def test_bad_pages_are_reported_where_the_checks_are_on():
+    from torsh_b200 import _native as nv
+    from torsh_b200.ops.kv_cache import kv_cache_attention, kv_cache_read, kv_cache_write
+    q, kp, vp, ks, vs, table, start = _case(2, 20, 2, 1, 64, 16, [60, 3], E4M3)
+    bad = table.clone()
+    bad[0, 2] = kp.shape[0]
+    calls = [lambda t: kv_cache_write(q[:, :, :1], q[:, :, :1], kp, vp, t, start - 28, None, ks, vs), lambda t: kv_cache_read(kp, vp, t, start, 60, None, ks, vs),
+             lambda t: kv_cache_attention(q[:, :1], kp, vp, t, start, None, None, ks, vs), lambda t: kv_cache_attention(q, kp, vp, t, start, None, None, ks, vs)]
+    nv.check_status()
+    nv.enable_kernel_checks(True)
+    try:
+        for call in calls:
+            call(table.clamp(min=0))
+            if call is not calls[0]:
+                nv.check_status()
+            else:                                                           # the second sequence begins in front of position 0
+                with pytest.raises(nv.KernelCheckFailed):
+                    nv.check_status()
+            call(bad.clamp(min=0))
+            with pytest.raises(nv.KernelCheckFailed):
+                nv.check_status()
+        nv.check_status()
+    finally:
+        nv.enable_kernel_checks(False)
+    kv_cache_attention(q, kp, vp, bad, start, None, None, ks, vs)
+    nv.check_status()
+
+
+def test_rotary_offsets_beyond_32_bits():
+    from torsh_b200.ops.rotary import rotary, rotary_frequencies
+    N, H, D = 600_000, 32, 128                                              # 2.5e9 elements
+    q = torch.empty(N, H, D, device=DEV, dtype=BF16)
+    for i in range(0, N, 100_000):
+        q[i:i + 100_000].normal_()
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    pos = torch.arange(N, device=DEV)
+    y, _ = rotary(q, None, pos, freqs, False)
+    for i in (0, 262_000, 524_280, N - 40):
+        s = slice(i, i + 40)
+        _rotary_close(y[s], q[s], _turn64(q[s], pos[s], freqs, False, 1.0), 1.0)
+
+
+def test_captured_calls_and_calls_on_two_streams():
+    """Each operator captured and replayed over new contents, and run on two streams at once from two threads."""
+    import threading
+    from torsh_b200.ops.kv_cache import kv_cache_attention, kv_cache_read, kv_cache_write
+    from torsh_b200.ops.rotary import rotary, rotary_frequencies
+    from torsh_b200.ops.speculative import verify_draft
+    B, T, H, D, V = 3, 24, 4, 64, 500
+    freqs, _ = rotary_frequencies(D, device=DEV)
+    table = torch.arange(B * 8, device=DEV).int().view(B, 8)
+
+    def make(seed):
+        g = _gen(seed)
+        q, k, v = (torch.randn(B, T, H, D, device=DEV, generator=g).to(BF16) for _ in range(3))
+        start = torch.randint(0, 90, (B,), device=DEV, generator=g).int()
+        return [q, k, v, start, *_verify_inputs(B, T, V, torch.float32, seed)]
+
+    def step(x, pages):
+        q, k, v, start, probs, draft, tokens, u = x
+        pos = start.long()[:, None] + torch.arange(T, device=DEV)
+        q, k = rotary(q, k, pos, freqs)
+        kv_cache_write(k, v, *pages[:2], table, start, None, *pages[2:])
+        out = kv_cache_attention(q, *pages[:2], table, start, None, None, *pages[2:])
+        back = kv_cache_read(*pages[:2], table, start + T, 128, None, *pages[2:])
+        return [out, *back, *verify_draft(probs, tokens, u, draft), *verify_draft(probs, tokens, u)]
+
+    def pool():
+        return _cache(B * 8, H, 16, D, torch.int8, 0)
+
+    inputs = [make(i) for i in range(4)]
+    want = [step(x, pool()) for x in inputs]
+    held, pages = [t.clone() for t in inputs[0]], pool()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(held, pages)
+    for x, w in zip(inputs, want):
+        for p in pages:
+            p.zero_()
+        for a, b in zip(held, x):
+            a.copy_(b)
+        clean = pool()
+        for p, c in zip(pages, clean):
+            p.copy_(c)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, w))
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            pages = pool()
+            for _ in range(20):
+                for p, c in zip(pages, pool()):
+                    p.copy_(c)
+                got[i] = step(inputs[i], pages)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+def test_rotary_backward_in_a_graph():
+    from torsh_b200.ops.rotary import rotary, rotary_frequencies
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    pos = torch.arange(9, device=DEV).expand(2, 9).contiguous()
+    x = torch.randn(2, 9, 4, 64, device=DEV, generator=_gen(6)).requires_grad_()
+    dy = torch.randn_like(x)
+
+    def both():
+        yq, yk = rotary(x, x * 2, pos, freqs, False)
+        return torch.autograd.grad((yq, yk), x, (dy, dy))[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx = both()
+    dx.zero_()
+    graph.replay()
+    assert torch.equal(dx, want)
+    _rotary_close(dx, dy, 3 * _turn64(dy, pos, freqs, False, 1.0, True), 3.0)
+
+
+def test_verify_draft_of_what_is_no_probability():
+    """Infinities, and numbers outside [0, 1): whatever comes out is in range."""
+    from torsh_b200.ops.speculative import verify_draft
+    B, T, V = 6, 5, 3001
+    probs, draft, tokens, u = _verify_inputs(B, T, V, torch.float32, 3)
+    probs[0, :, 5], probs[1], draft[2] = math.inf, math.inf, math.inf
+    probs[3] = 3e38
+    u[4], u[5] = math.nan, -2.0
+    u[:2, T - 1] = 0
+    for d in (draft, None):
+        acc, path, nxt = verify_draft(probs, tokens, u, d)
+        assert ((acc >= 0) & (acc < T)).all() and ((path >= -1) & (path < T)).all() and ((nxt >= -1) & (nxt < V)).all()
+        assert torch.equal((path >= 0).sum(1), acc + 1)
