@@ -4,7 +4,14 @@
 // O += P V are tcgen05.mma products of 128 x 128 x D and 128 x D x 128 with S, P and O in TMEM. A tile's two products take 1024 clocks of
 // the tensor core and its 128 x 128 exponentials 1024 of the special-function unit, whether all rows are used or not; its keys and
 // values (64 KB in bf16, 33 KB in 8 bits, D = 128) take 2800 and 1450 clocks of the SM's share of HBM. So up to 128 rows cost what
-// the memory takes; mma.sync at 32 rows a CTA read every token rows / 32 times through L2 and was 2.5 to 8 times slower (see below).
+// the memory takes; mma.sync at 32 rows a CTA read every token rows / 32 times through L2 and was 2.5 to 8 times slower.
+//
+// Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 122 us, 4.5 TB/s. A tile
+// takes 2900 clocks, what the memory takes; the rest is the start (13 000 clocks until the first S: launch, deal, page table, first
+// copies) and the end of a unit (12 000 from the last P to the next unit's first S, in which the ring fills and then waits). 12 trees of 27
+// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 75 us. A tile takes 4300 clocks: 10 000 warp instructions (decoding,
+// scales, exponentials) at 40 % of the issue slots, no pipe above 29 %, warps waiting for loads and for one another. Measured and not kept:
+// seven decoding warps (81 us), keys' scales in the halves (82), Q a unit ahead in a second place (122 and 86).
 //
 // One CTA per SM, 512 threads:
 //   warps 0-3, 4-7  softmax, a thread per row, even tiles for the first four warps and odd ones for the others, each with a maximum, a sum
@@ -18,7 +25,7 @@
 // TMEM: S and P of even and of odd tiles 128 columns each (P takes the first half of the S it came from), then O of either.
 //
 // 8-bit scales: scores are multiplied by the key's scale in fp32. The value's goes into the halves, relative to a power of two for each
-// 32 tokens (what a loading warp has of a tile): one rounding of 2^-12 for the scale and one for the product, as P has one, where
+// 32 tokens (what a loading warp has of a tile): one rounding (2^-11 at most) for the scale and one for the product, as P has one, where
 // carrying it in P cost the softmax 32 more loads of broadcast scales a tile (3.5 us instead of 2). P of those tokens is shifted by the
 // quotient of their power of two and the largest so far (`unit`), which O is relative to.
 #include "cache_attention.cuh"

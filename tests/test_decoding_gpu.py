@@ -79,6 +79,41 @@ def test_rotary_gradient_of_a_gradient_and_of_one_output():
     _rotary_close(gd, w, _turn64(w, pos, freqs, True, 1.0), 1.0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("D,R", [(96, 34), (64, 36), (64, 32), (80, 70), (12, 6)])
+def test_rotary_leaves_the_other_columns_as_they_are(dtype, interleaved, D, R):
+    from torsh_b200.ops.rotary import rotary, rotary_frequencies
+    x = torch.randn(2, 5, 3, D, device=DEV, generator=_gen(D)).to(dtype)
+    x[..., R::3], x[..., R + 1::5] = math.inf, math.nan
+    pos = torch.arange(5, device=DEV) + 7
+    freqs, _ = rotary_frequencies(R, device=DEV)
+    y, _ = rotary(x, None, pos, freqs, interleaved, 1.25)
+    bits = torch.int16 if dtype == BF16 else torch.int32
+    assert torch.equal(y[..., R:].contiguous().view(bits), x[..., R:].contiguous().view(bits))
+    ref = _turn64(x, pos.expand(2, 5), freqs, interleaved, 1.25)
+    _rotary_close(y[..., :R], x[..., :R], ref[..., :R], 1.25)
+
+
+def test_rotary_strides_beyond_32_bits_and_heads_between_tokens():
+    """Rows so far apart that their strides do not fit 32 bits, and blocks whose rows are of several tokens and of both tensors."""
+    from torsh_b200.ops.rotary import rotary, rotary_frequencies
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    store = torch.empty((1 << 31) + 4096, dtype=BF16, device=DEV)
+    q = store.as_strided((2, 3, 64), ((1 << 31) + 8, 64, 1))
+    q.copy_(torch.randn(2, 3, 64, device=DEV, generator=_gen(4)))
+    pos = torch.tensor([3, 1000], device=DEV)
+    y, _ = rotary(q, None, pos, freqs)
+    _rotary_close(y, q, _turn64(q, pos, freqs, True, 1.0), 1.0)
+    del store, q
+    for N, hq, hk in ((3000, 3, 1), (40000, 5, 2), (5000, 70, 1)):
+        q, k = (torch.randn(N, h, 64, device=DEV, generator=_gen(N + h)).to(BF16) for h in (hq, hk))
+        pos = torch.randint(0, 5000, (N,), device=DEV, generator=_gen(2))
+        for interleaved in (True, False):
+            for x, y in zip((q, k), rotary(q, k, pos, freqs, interleaved)):
+                _rotary_close(y, x, _turn64(x, pos, freqs, interleaved, 1.0), 1.0)
+
+
 def test_rotary_strides_and_shared_positions():
     from torsh_b200.ops.rotary import rotary, rotary_frequencies
     B, T, H, D = 3, 11, 4, 64
