@@ -10,8 +10,8 @@
 //
 // Bound by memory: each row is read and written once. D / 8 lanes share a row (8 elements each, the row's largest magnitude over
 // shuffles); neighbouring groups take neighbouring heads of a token, which lie together on the contiguous side. Measured: 8 prompts of up
-// to 2048 tokens, 32 heads of 128, bf16 into e4m3, 694 MB: 127 us, 5.5 TB/s. One token of 13 sequences: 6.6 us, launch and three
-// dependent loads (start, table, row).
+// to 2048 tokens, 32 heads of 128, bf16 into e4m3, written and read back, 694 MB: 124 us, 5.6 TB/s (127 with addresses in 64 bits
+// throughout). One token of 13 sequences, written: 6.3 us, launch and three dependent loads (start, table, row).
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -25,7 +25,8 @@ constexpr int KV_THREADS = 256;
 
 struct KvArgs {
   const void* x[2];            // k, v [B, T, H, D] with strides (write)
-  long sb[2], st[2], sh[2];    // elements
+  long sb[2];                  // elements
+  int st[2], sh[2];
   void* y[2];                  // k, v [B, T, H, D] contiguous (read)
   void* pages[2];
   float* scales[2];
@@ -33,7 +34,7 @@ struct KvArgs {
   const int* start;            // [B]: position of token 0 (null: 0)
   const int* counts;           // [B]: tokens that count (null: T)
   long table_ld;
-  int B, T, H, page, pages_per_seq, num_pages;
+  int B, T, H, page, pages_per_seq, num_pages, page_rows;   // page_rows: H * page
   FastDiv by_h, by_page;
 };
 
@@ -47,7 +48,7 @@ __device__ __forceinline__ long kv_row(const KvArgs& a, int b, int t, int h) {
   if (slot >= (unsigned)a.pages_per_seq) return -1;
   const int p = a.table[b * a.table_ld + slot];
   if ((unsigned)p >= (unsigned)a.num_pages) return -1;
-  return ((long)p * a.H + h) * a.page + (pos - slot * (unsigned)a.page);
+  return (long)p * a.page_rows + (int)(h * a.page + (pos - slot * (unsigned)a.page));
 }
 
 // Largest |x| of 8 elements, as the bits of a float without its sign: a NaN counts for more than an infinity, that for more than any
@@ -116,6 +117,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvArgs a) {
   if ((int)(blockIdx.x * (PER * R) / (unsigned)a.H) >= n) return;
   Raw8<T> x[R][2];
   long row[R];
+  const T *base[2] = {(const T*)a.x[0] + b * a.sb[0] + lane * 8, (const T*)a.x[1] + b * a.sb[1] + lane * 8};
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const unsigned r = r0 + i * PER;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvArgs a) {
     row[i] = -1;
     if (t < n) {
 #pragma unroll
-      for (int z = 0; z < 2; ++z) x[i][z].load((const T*)a.x[z] + b * a.sb[z] + t * a.st[z] + h * a.sh[z] + lane * 8);
+      for (int z = 0; z < 2; ++z) x[i][z].load(base[z] + (long)t * a.st[z] + (long)h * a.sh[z]);
       row[i] = kv_row(a, b, t, h);
       if (row[i] < 0 && lane == 0) report_bad_index();
     } else {
@@ -196,6 +198,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvArgs a) {
   const int b = blockIdx.y;
   const int n = a.counts ? a.counts[b] : a.T;
   long row[R];
+  T *base[2] = {(T*)a.y[0] + (long)b * a.T * a.H * D + lane * 8, (T*)a.y[1] + (long)b * a.T * a.H * D + lane * 8};
   uint4 raw[R][2];
   float sc[R][2];
 #pragma unroll
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvArgs a) {
           else f[j] = __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3))) * sc[i][z];
         }
       }
-      T* y = (T*)a.y[z] + ((long)b * a.T * a.H + r) * D + lane * 8;
+      T* y = base[z] + (long)r * D;
       if constexpr (sizeof(T) == 2) {
         Vec16<T> v;
         v.set(f);
@@ -294,23 +297,24 @@ static int kv_call(const KvCall* c, bool write, cudaStream_t st) {
   if (c->B <= 0 || c->T <= 0) return 0;
   if (c->B > 65535 || c->H <= 0 || c->T > 0x7fffff00l || c->H > 0x7fffff00l || c->T * c->H > 0x7fffff00l)
     TB_FAIL(TB_E_TOO_LARGE, "kv cache: at most 65535 sequences and 2^31 rows a sequence in one call");
-  if (c->page <= 0 || c->page > 0x7fffff00l || c->num_pages < 0 || c->num_pages > 0x7fffffff || c->pages_per_seq < 0 || c->pages_per_seq > 0x7fffffff)
+  if (c->page <= 0 || c->page > 0x7fffff00l || c->page * c->H > 0x7fffff00l || c->num_pages < 0 || c->num_pages > 0x7fffffff || c->pages_per_seq < 0 || c->pages_per_seq > 0x7fffffff)
     TB_FAIL(TB_E_ARG, "kv cache: bad sizes");
   KvArgs a{};
   for (int z = 0; z < 2; ++z) {
-    if (write) a.x[z] = c->x[z], a.sb[z] = c->strides[3 * z], a.st[z] = c->strides[3 * z + 1], a.sh[z] = c->strides[3 * z + 2];
+    if (write) a.x[z] = c->x[z], a.sb[z] = c->strides[3 * z], a.st[z] = (int)c->strides[3 * z + 1], a.sh[z] = (int)c->strides[3 * z + 2];
     else a.y[z] = c->x[z];
     a.pages[z] = c->pages[z], a.scales[z] = c->scales[z];
   }
   a.table = c->table, a.start = c->start, a.counts = c->counts, a.table_ld = c->table_ld;
   a.B = (int)c->B, a.T = (int)c->T, a.H = (int)c->H, a.page = (int)c->page, a.pages_per_seq = (int)c->pages_per_seq, a.num_pages = (int)c->num_pages;
+  a.page_rows = a.page * a.H;
   a.by_h = FastDiv::of((unsigned)a.H), a.by_page = FastDiv::of((unsigned)a.page);
   const int D = (int)c->D, kind = (int)c->kind, dtype = (int)c->dtype;
   if (int r = kv_check(a, D, kind, dtype)) return r;
   if (!c->x[0] || !c->x[1] || (((uintptr_t)c->x[0] | (uintptr_t)c->x[1]) & 15)) TB_FAIL(TB_E_ARG, "kv cache: rows must be 16-byte aligned");
   const int N = dtype == 0 ? 8 : 4;
   for (int i = 0; write && i < 6; ++i)
-    if (c->strides[i] % N) TB_FAIL(TB_E_ARG, "kv cache: strides must be multiples of 16 bytes");
+    if (c->strides[i] % N || (i % 3 && labs(c->strides[i]) > 0x7fffffffl)) TB_FAIL(TB_E_ARG, "kv cache: strides must be multiples of 16 bytes, those of tokens and heads below 2^31");
   return dtype == 0 ? kv_dispatch<bf16>(a, D, kind, write, st) : kv_dispatch<float>(a, D, kind, write, st);
 }
 TB_EXPORT int tb_kv_write(const KvCall* c, cudaStream_t st) {

@@ -78,9 +78,9 @@ bool ints(const Tensor& t, int64_t n, int device) {
   return here(t, device) && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
 }
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
-bool rows16(const Tensor& t) {   // [., ., ., D]: every row starts on 16 bytes
+bool rows16(const Tensor& t) {   // [., ., ., D]: every row starts on 16 bytes, and a sequence's rows are not too far apart for 32 bits
   const int64_t n = 16 / t.element_size();
-  return t.stride(3) == 1 && aligned(t.const_data_ptr()) && t.stride(0) % n == 0 && t.stride(1) % n == 0 && t.stride(2) % n == 0;
+  return t.stride(1) <= 0x7fffffff && t.stride(2) <= 0x7fffffff && t.stride(3) == 1 && aligned(t.const_data_ptr()) && t.stride(0) % n == 0 && t.stride(1) % n == 0 && t.stride(2) % n == 0;
 }
 int kind_of(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kChar ? 1 : t == at::kFloat8_e4m3fn ? 2 : -1; }
 int row_type(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kFloat ? 1 : -1; }

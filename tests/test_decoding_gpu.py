@@ -245,6 +245,21 @@ def test_cache_positions_without_a_page():
     assert rk[0, :2].eq(1).all() and rk.float().sum() == 2 * 64 and torch.equal(rk, rv)
 
 
+def test_cache_rows_more_than_32_bits_apart():
+    from torsh_b200.ops.kv_cache import kv_cache_attention, kv_cache_write
+    store = torch.empty((1 << 31) + 4096, dtype=BF16, device=DEV)
+    for strides in ((4096, 1 << 31, 64, 1), (4096, 128, 1 << 31, 1)):
+        x = store.as_strided((1, 2, 2, 64), strides)
+        x.copy_(torch.randn(1, 2, 2, 64, device=DEV, generator=_gen(1)))
+        y = x.contiguous()
+        table, start = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+        pools = [_cache(1, 2, 16, 64, BF16, 0) for _ in range(2)]
+        for z, (kp, vp, _, _) in zip((x, y), pools):
+            kv_cache_write(z, z, kp, vp, table, start)
+        assert torch.equal(pools[0][0], pools[1][0]) and torch.equal(pools[0][0][0, :, :2], y[0].transpose(0, 1))
+        assert torch.equal(*(kv_cache_attention(z, *pools[0][:2], table, start) for z in (x, y)))
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def _filled(pages, H, page, D, dtype, g):
     if dtype == BF16:

@@ -70,9 +70,9 @@ def _table(page_table):
 
 
 def _rows(x):
-    """Rows that start on 16 bytes; copied where they do not."""
+    """Rows that start on 16 bytes, less than 2^31 elements apart; copied where they are not so."""
     n = 16 // x.element_size()
-    return x if x.stride(3) == 1 and not x.data_ptr() % 16 and not any(s % n for s in x.stride()[:3]) else x.clone(memory_format=torch.contiguous_format)
+    return x if max(x.stride()[1:]) < 1 << 31 and x.stride(3) == 1 and not x.data_ptr() % 16 and not any(s % n for s in x.stride()[:3]) else x.clone(memory_format=torch.contiguous_format)
 
 
 # ------------------------------------------------------------------------------------------------ the formulas in PyTorch
