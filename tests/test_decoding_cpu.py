@@ -246,6 +246,47 @@ def test_paged_cache_keeps_its_pages():
             PagedKVCache(**{**dict(num_layers=1, num_heads=1, head_dim=8, batch=1, max_len=16, page=16, device="cpu"), **bad})
 
 
+def _fed(c, tokens, seed):
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.randn(c.batch, tokens, 1, 8, generator=g) for _ in range(2))
+    c.write(0, k, v)
+    return k, v
+
+
+def test_a_place_without_a_sequence_reaches_no_other_sequence():
+    """Batched steps go on over places that were never used, and places whose sequence was released: their rows belong nowhere."""
+    c = PagedKVCache(1, 1, 8, batch=3, max_len=64, dtype=torch.float32, page=16, num_pages=4, device="cpu")
+    c.reserve([16, 16, 0])
+    _fed(c, 16, 0)
+    c.advance([16, 16, 0])
+    c.release(0)
+    c.reserve([0, 32, 0])                                   # gets the released page
+    k, v = _fed(c, 32, 1)
+    c.advance([0, 32, 0])
+    for got, want in zip(c.read(0, torch.float32), (k, v)):
+        assert torch.equal(got[1, 16:48], want[1]) and not got[[0, 2]].any()
+    q = torch.randn(3, 1, 2, 8)
+    assert not c.attend(0, q)[[0, 2]].any()
+
+
+@pytest.mark.parametrize("owner", [0, 1, 2])
+def test_keeping_a_path_leaves_other_places_alone(owner):
+    """The sequence that owns page 0 keeps its path whichever place it has, beside places that have no page."""
+    c = PagedKVCache(1, 1, 8, batch=3, max_len=32, dtype=torch.float32, page=16, num_pages=2, device="cpu")
+    c.reserve([20 if b == owner else 0 for b in range(3)])
+    assert c.page_table[owner, 0] == 0
+    k, v = _fed(c, 5, 2)
+    path = torch.tensor([[0, 2, 4, -1, -1]] * 3)
+    c.keep(path, torch.tensor([2, 2, 2]))
+    c.advance([3 if b == owner else 0 for b in range(3)])
+    for got, want in zip(c.read(0, torch.float32), (k, v)):
+        assert torch.equal(got[owner, :3], want[owner, [0, 2, 4]])
+    assert torch.equal(c.layers[0][0][0, 0, 3:5], k[owner, 3:5, 0])            # what is not on the path stays
+    none = PagedKVCache(1, 1, 8, batch=2, max_len=32, dtype=torch.float32, page=16, device="cpu")
+    none.keep(path[:2], torch.tensor([2, 2]))
+    assert not none.layers[0][0].any()
+
+
 # ------------------------------------------------------------------------------------------------ verification
 def test_verify_by_hand():
     p = torch.tensor([[[0.5, 0.25, 0.25, 0.0], [0.0, 0.5, 0.5, 0.0], [0.25, 0.25, 0.25, 0.25]]])
@@ -314,6 +355,12 @@ def test_generate_samples_and_refuses():
     for bad in (dict(temperature=-1.0), dict(draft=small, drafted=0)):
         with pytest.raises(ValueError):
             m.generate(ids, 2, **bad)
+
+
+def test_generate_for_nobody_and_nothing():
+    m = _llama()
+    for ids, n in ((torch.zeros(0, 4, dtype=torch.int64), 3), (torch.zeros(2, 0, dtype=torch.int64), 3), (torch.ones(2, 4, dtype=torch.int64), 0)):
+        assert torch.equal(m.generate(ids, n), ids)
 
 
 def test_decode_of_a_tree_gives_each_path_its_own_states():

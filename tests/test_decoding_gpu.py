@@ -884,3 +884,49 @@ def test_verify_draft_of_what_is_no_probability():
         acc, path, nxt = verify_draft(probs, tokens, u, d)
         assert ((acc >= 0) & (acc < T)).all() and ((path >= -1) & (path < T)).all() and ((nxt >= -1) & (nxt < V)).all()
         assert torch.equal((path >= 0).sum(1), acc + 1)
+
+
+def test_a_captured_step_of_a_paged_cache_goes_on():
+    """A tree step - write, attend, verify, keep, advance - captured once and replayed while the sequences grow, beside a place without one."""
+    from torsh_b200.ops.kv_cache import PagedKVCache, tree_mask_of
+    from torsh_b200.ops.speculative import verify_draft
+    B, T, H, D, V = 3, 5, 2, 64, 40
+    parents = torch.tensor([-1, 0, 0, 1, 2], device=DEV)
+    mask = tree_mask_of(parents)
+    g = _gen(9)
+    steps = [[torch.randn(B, T, H, D, device=DEV, generator=g).to(BF16) for _ in range(3)]
+             + [torch.softmax(3 * torch.randn(B, T, V, device=DEV, generator=g), -1), torch.randint(0, V, (B, T), device=DEV, generator=g), torch.rand(B, T, device=DEV, generator=g)]
+             for _ in range(12)]
+
+    def make():
+        c = PagedKVCache(1, H, D, batch=B, max_len=96, dtype=torch.int8, page=16, num_pages=12, device=DEV)
+        c.reserve([96, 0, 70])
+        return c
+
+    def step(c, x):
+        q, k, v, probs, tokens, u = x
+        c.write(0, k, v)
+        out = c.attend(0, q, mask)
+        acc, path, nxt = verify_draft(probs, tokens, u, None, parents)
+        c.keep(path, acc)
+        c.advance(acc + 1, most=T)
+        return out, acc, nxt
+
+    eager = make()
+    want = [[y.clone() for y in step(eager, x)] for x in steps]
+    assert int(eager.lengths.max()) > 2 * T                                # beyond what there was at the capture
+    held, c = [x.clone() for x in steps[0]], make()
+    table = c.page_table.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(c, held)
+    for x, w in zip(steps, want):
+        for a, b in zip(held, x):
+            a.copy_(b)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, w))
+        assert not outs[0][1].any()
+    assert torch.equal(c.lengths, eager.lengths) and torch.equal(c.page_table, table)
+    for (a, b), (sa, sb) in ((c.layers[0], c.scales[0]),):
+        (ea, eb), (esa, esb) = eager.layers[0], eager.scales[0]
+        assert torch.equal(a, ea) and torch.equal(b, eb) and torch.equal(sa, esa) and torch.equal(sb, esb)

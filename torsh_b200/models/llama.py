@@ -227,7 +227,7 @@ class LlamaModel(nn.Module):
         if draft is not None and (draft.cfg.vocab_size != self.cfg.vocab_size or drafted < 1):
             raise ValueError("generate: the draft model has the same vocabulary, and drafts at least one token")
         B, S = input_ids.shape
-        if S == 0 or max_new_tokens <= 0:
+        if B == 0 or S == 0 or max_new_tokens <= 0:
             return input_ids
         dev = input_ids.device
         room = S + max_new_tokens + (drafted if draft is not None else 0)

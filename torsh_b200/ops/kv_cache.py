@@ -314,7 +314,9 @@ class PagedKVCache:
     ``dtype`` is ``torch.bfloat16``, ``torch.int8`` or ``torch.float8_e4m3fn``. Every layer has its own pages; the table and the lengths
     are common. A step is: :meth:`reserve` room for the new tokens of the batch, for each layer :meth:`write` their keys and values and
     :meth:`attend`, then :meth:`advance` the lengths by what is kept (after a verification fewer than were written: the rest is
-    written over). The table is a device tensor that is written in place, so a step can be captured into a graph after ``reserve``.
+    written over). Table and lengths are device tensors that are written in place, so a step with ``advance(tensor, most)`` can be captured
+    into a graph and replayed while what has been reserved lasts. Places of the batch that have no sequence have no pages: what a batched
+    step writes for them is left out, and what it reads is zeros.
     """
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, batch: int, max_len: int, dtype: torch.dtype = torch.bfloat16,
@@ -332,7 +334,7 @@ class PagedKVCache:
         self.layers = [(mk(), mk()) for _ in range(num_layers)]
         sc = lambda: torch.zeros(shape[:3], device=device) if dtype in _CODES else None   # noqa: E731
         self.scales = [(sc(), sc()) for _ in range(num_layers)]
-        self.page_table = torch.zeros(batch, per, dtype=torch.int32, device=device)
+        self.page_table = torch.full((batch, per), -1, dtype=torch.int32, device=device)   # -1: no page
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.host_lengths = [0] * batch           # upper bounds: what advance() has been told on the host
         self._owned: list[list[int]] = [[] for _ in range(batch)]
@@ -363,8 +365,7 @@ class PagedKVCache:
                scale: float | None = None) -> torch.Tensor:
         """:func:`kv_cache_attention` of tokens that :meth:`write` has just written."""
         (kp, vp), (ks, vs) = self.layers[layer], self.scales[layer]
-        longest = max(self.host_lengths, default=0) + q.shape[1]
-        return kv_cache_attention(q, kp, vp, self.page_table, self.lengths, tree_mask, counts, ks, vs, scale, longest)
+        return kv_cache_attention(q, kp, vp, self.page_table, self.lengths, tree_mask, counts, ks, vs, scale)
 
     def read(self, layer: int, dtype: torch.dtype = torch.bfloat16):
         """All keys and values of a layer, ``[B, longest, H, D]``."""
@@ -375,13 +376,17 @@ class PagedKVCache:
         """Moves the accepted nodes of a tree (:func:`~torsh_b200.ops.speculative.verify_draft`) to the front of the tokens just written,
         in every layer: node ``path[b, i]`` to place ``i``, for ``i <= accepted[b]``. A chain is in place already."""
         B, T = path.shape
+        if B * T == 0 or self.layers[0][0].numel() == 0:
+            return
         i = torch.arange(T, device=path.device)
         base = self.lengths.long()[:, None]
         src, srow, ok = _slots(self.page_table, self.layers[0][0].shape[0], self.page, base + path.clamp(min=0))
         dst, drow, there = _slots(self.page_table, self.layers[0][0].shape[0], self.page, base + i)
         ok = ok & there & (i <= accepted[:, None]) & (path >= 0)
-        # places that stay as they are copy themselves: no sizes that depend on the data
+        # no sizes that depend on the data: places that stay as they are copy themselves, and those without a page repeat one that has one
         src, srow = torch.where(ok, src, dst), torch.where(ok, srow, drow)
+        some = there.flatten().int().argmax()[None]
+        src, srow, dst, drow = (torch.where(there, x, x.flatten().gather(0, some)) for x in (src, srow, dst, drow))
         for pages, scales in zip(self.layers, self.scales):
             for x in (*map(_bits, pages), *scales):
                 if x is not None:
@@ -412,5 +417,6 @@ class PagedKVCache:
         """Gives sequence ``b``'s pages back; its place takes a new sequence from position 0."""
         self._free += reversed(self._owned[b])
         self._owned[b] = []
+        self.page_table[b] = -1
         self.lengths[b] = 0
         self.host_lengths[b] = 0
