@@ -15,11 +15,11 @@
 // underflow. P in halves has eight times the bits of bf16. Scores, maxima, sums and O are fp32.
 //
 // The work of all sequences is dealt to the CTAs in equal runs of tiles (deal_tiles), so ragged batches and single long sequences
-// fill the GPU alike; a unit cut by the deal is joined by cache_attn_join_kernel.
+// fill the GPU alike; a unit cut by the deal is joined by cache_attn_join_kernel. Short units are not cut (CA_WHOLE).
 //
 // Measured (a call among others, L2 cold): 64 sequences of up to 8192 tokens, 8 heads of D = 128 in e4m3, 618 MB: 112 us, 5.5 TB/s. One
-// sequence of 131 072 tokens in int8, 277 MB: 60 us, 4.6 TB/s, of which 9 are what a call over 78 tokens takes: two launches, the deal
-// (a few dependent loads), the page table, then the data.
+// sequence of 131 072 tokens in int8, 277 MB: 60 us, 4.6 TB/s, of which 9 are two launches, the deal (a few dependent loads), the page
+// table and the joining. One of 78 tokens: 6.5 us (9.1 with its units cut).
 #include "cache_attention.cuh"
 #include "decode_calls.h"
 
@@ -28,6 +28,10 @@ namespace tb {
 constexpr int CA_WARPS = 4;
 constexpr int CA_THREADS = CA_WARPS * 32;
 constexpr int CA_TILE = 16;   // tokens of a warp's tile
+// Units stay whole while the longest has so many tiles more than a CTA's share. Measured (us, whole / cut): one sequence of 16 heads of 64,
+// 77 tokens 6.3 / 9.3, 200: 7.7 / 9.2, 400 (21 tiles more) 9.8 / 9.2, 1600: 22.7 / 10.6; 16 sequences of 8 heads of 128 in e4m3, 400 tokens
+// (18 more) 13.4 / 15.7, 800 (39 more) 19.1 / 18.2; 32 sequences of 16 heads of 64, 800 tokens (7 more) 22.4 / 27.2.
+constexpr int CA_WHOLE = 20;
 
 __device__ __forceinline__ uint32_t ca_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ca_copy16(uint32_t dst, const void* src, bool live) {
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
   float* wild = (float*)(smem + CA_WARPS * S::RING + S::ML) + warp * CA_TILE * 8;
   const uint32_t ring_u = ca_smem(ring);
 
-  const Deal deal = deal_tiles<CA_THREADS, CA_TILE, CA_WARPS>(a, scratch);
+  const Deal deal = deal_tiles<CA_THREADS, CA_TILE, CA_WARPS, CA_WHOLE>(a, scratch);
   release_join();
   zero_empty<D, CA_THREADS>(a);
   if (deal.first >= deal.last) {
@@ -558,6 +562,7 @@ __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const Ca
     const int units = a.Hkv * a.row_tiles;
     b = blockIdx.x / units, hr = blockIdx.x - b * units;
     per = a.plan[0].w;
+    if (per == 0) return;                                // no unit has been cut
   } else {
     const int4 p = a.plan[blockIdx.x];
     if (p.w == 0 || p.z == 0 || p.z > p.w) return;     // nothing; a unit's beginning; not its first cut

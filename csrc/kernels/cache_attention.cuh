@@ -68,21 +68,24 @@ __device__ __forceinline__ int block_prefix(int v, int* scratch, int& total) {
   return before + incl - v;
 }
 
-// The deal: the tiles of all units in a row, `per` of them to each CTA, so that every CTA has the same share whatever the lengths.
-// Returns the CTA's first sequence and the tiles in front of it.
+// The deal: the tiles of all units in a row, `per` of them to each CTA, so that every CTA has the same share whatever the lengths. Where
+// there are no more units than CTAs and the longest has at most WHOLE tiles more than such a share, each CTA has a unit: joining parts costs
+// 2 to 4 us, as much as those tiles. Returns the CTA's first sequence and the tiles in front of it.
 struct Deal {
-  int per, first, last;   // tiles of a CTA; this CTA's tiles are [first, last)
+  int per, first, last;   // tiles of a CTA (0: no unit is cut); this CTA's tiles are [first, last)
   int b, before;          // the sequence that tile `first` is of, and the tiles in front of that sequence
 };
 // `scratch`: 36 ints of shared memory.
-template <int THREADS, int TILE, int ROUND>
+template <int THREADS, int TILE, int ROUND, int WHOLE>
 __device__ __forceinline__ Deal deal_tiles(const CacheAttnArgs& a, int* scratch) {
   Deal d;
   const int units = a.Hkv * a.row_tiles;
   int all = 0, keep_n = 0, keep_before = 0;
+  int most = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
-    const int n = b < a.B ? (seq_len(a, b).len + TILE - 1) / TILE * units : 0;
+    const int nt = b < a.B ? (seq_len(a, b).len + TILE - 1) / TILE : 0, n = nt * units;
+    most = max(most, nt);
     int total;
     const int before = all + block_prefix<THREADS>(n, scratch, total);
     if (b0 == 0) keep_n = n, keep_before = before;
@@ -91,6 +94,16 @@ __device__ __forceinline__ Deal deal_tiles(const CacheAttnArgs& a, int* scratch)
   }
   d.per = max((all + a.grid - 1) / a.grid, 1);
   d.per = (d.per + ROUND - 1) / ROUND * ROUND;
+  if (a.before && !__syncthreads_or(most > d.per + WHOLE)) {
+    // a unit for each CTA, and nothing to join; `first` and `before` count from the unit's sequence
+    d.per = 0;
+    d.b = blockIdx.x / units;
+    d.before = 0;
+    const int nt = d.b < a.B ? (seq_len(a, d.b).len + TILE - 1) / TILE : 0;
+    d.first = ((int)blockIdx.x - d.b * units) * nt;
+    d.last = d.first + nt;
+    return d;
+  }
   d.first = min((long)blockIdx.x * d.per, (long)all);
   d.last = min((long)d.first + d.per, (long)all);
   d.b = d.before = 0;

@@ -97,7 +97,6 @@ class LlamaBlock(nn.Module):
         h, x = norm_ops.rms_norm_fork(x, self.post_attn_norm.weight, cfg.rms_eps)
         return self.down(ew.swiglu(self.gate_up(h)), residual=x)
 
-
     def step(self, x, B: int, T: int, cache, layer: int, positions, freqs, tree_mask=None, counts=None):
         """``T`` new tokens per sequence on top of ``cache`` (:class:`~torsh_b200.ops.kv_cache.PagedKVCache`), which gets their keys and values."""
         cfg, H, D = self.cfg, self.local_heads, self.cfg.head_dim
