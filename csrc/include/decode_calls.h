@@ -37,6 +37,7 @@ struct CacheAttnCall {
   long B, T, Hq, Hkv, D, page, pages_per_seq, num_pages, max_len, kind;
   int* status;
   double scale;
+  mutable long kernels;   // out: what has been launched
 };
 
 struct VerifyCall {

@@ -19,7 +19,7 @@
 //
 // Measured (a call among others, L2 cold): 64 sequences of up to 8192 tokens, 8 heads of D = 128 in e4m3, 618 MB: 112 us, 5.5 TB/s. One
 // sequence of 131 072 tokens in int8, 277 MB: 60 us, 4.6 TB/s, of which 9 are two launches, the deal (a few dependent loads), the page
-// table and the joining. One of 78 tokens: 6.5 us (9.1 with its units cut).
+// table and the joining. One of 78 tokens: 5.3 us (9.1 with its units cut, 6.5 where the table could hold more).
 #include "cache_attention.cuh"
 #include "decode_calls.h"
 
@@ -620,7 +620,9 @@ __global__ void __launch_bounds__(CJ_WARPS * 32) cache_attn_join_kernel(const Ca
 
 static long ca_units(const CacheAttnArgs& a) { return (long)a.B * a.Hkv * a.row_tiles; }
 
-int cache_attn_join(const CacheAttnArgs& a, int D, int tile, cudaStream_t st) {
+int cache_attn_join(CacheAttnArgs& a, int D, int tile, int whole, cudaStream_t st) {
+  if (a.before && (a.limit + tile - 1) / tile <= whole) return 0;   // the table is so short that no unit can have been cut: 1 us
+  a.kernels = 2;
   // one sequence cuts few units into many parts, many sequences many units into few
   const long units = ca_units(a);
   const int share = units * 8 >= a.grid ? 1 : CJ_WARPS;
@@ -646,7 +648,7 @@ static int cache_attn_launch(CacheAttnArgs& a, cudaStream_t st) {
   if (ca_units(a) > a.grid) a.before = nullptr;
   cache_attn_kernel<D, KIND, NT><<<a.grid, CA_THREADS, S::SMEM, st>>>(a);
   TB_CUDA_CHECK(cudaGetLastError());
-  return cache_attn_join(a, D, CA_TILE, st);
+  return cache_attn_join(a, D, CA_TILE, CA_WHOLE + CA_WARPS, st);
 }
 
 template <int D, int KIND>
@@ -727,6 +729,8 @@ TB_EXPORT int tb_cache_attention(const CacheAttnCall* c, cudaStream_t st) {
   a.part_ml = a.part_o + slots * a.part_rows * D;
   a.plan = (int4*)(a.part_ml + slots * a.part_rows * 2);
   a.before = (int*)(a.plan + slots / 2);               // there are at most as many sequences as units, and units as CTAs, where it is used
-  if (tc) return cache_attn_tc(a, (int)D, kind, c->status, st);
-  return D == 64 ? cache_attn_kind<64>(a, kind, nt, st) : cache_attn_kind<128>(a, kind, nt, st);
+  a.kernels = 1;
+  const int rc = tc ? cache_attn_tc(a, (int)D, kind, c->status, st) : D == 64 ? cache_attn_kind<64>(a, kind, nt, st) : cache_attn_kind<128>(a, kind, nt, st);
+  c->kernels = a.kernels;
+  return rc;
 }

@@ -27,6 +27,7 @@ struct CacheAttnArgs {
   int part_rows;               // rows of a slot of partial results
   int limit;                   // tokens of a sequence that the table can name, or fewer
   float scale_log2;
+  int kernels;                 // launches of the call
 };
 
 // Tokens that sequence b has to offer, and how many of its new ones count.
@@ -231,7 +232,7 @@ __device__ __forceinline__ void pairs_of(uint32_t t0, uint32_t t1, uint32_t (&r)
 }
 
 // Joins the units that the deal has cut; in cache_attention.cu.
-int cache_attn_join(const CacheAttnArgs& a, int D, int tile, cudaStream_t st);
+int cache_attn_join(CacheAttnArgs& a, int D, int tile, int whole, cudaStream_t st);
 // The same attention for many rows, on tcgen05; in cache_attention_sm100.cu.
 int cache_attn_tc(CacheAttnArgs& a, int D, int kind, int* status, cudaStream_t st);
 

@@ -698,12 +698,12 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
 }
 
 template <int D, int KIND>
-static int cache_attn_tc_launch(const CacheAttnArgs& a, int* status, cudaStream_t st) {
+static int cache_attn_tc_launch(CacheAttnArgs& a, int* status, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   if (int r = smem_opt_in(done, cache_attn_tc_kernel<D, KIND>, CtShape<D, KIND>::ALLOC)) return r;
   cache_attn_tc_kernel<D, KIND><<<a.grid, CT_THREADS, CtShape<D, KIND>::ALLOC, st>>>(a, status);
   TB_CUDA_CHECK(cudaGetLastError());
-  return cache_attn_join(a, D, CT_TILE, st);
+  return cache_attn_join(a, D, CT_TILE, CT_WHOLE + 1, st);
 }
 
 int cache_attn_tc(CacheAttnArgs& a, int D, int kind, int* status, cudaStream_t st) {
