@@ -647,38 +647,52 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       const float inv = all > 0.f || all != all ? 1.f / all : 0.f;   // a row that sees nothing: zeros
       const long at = (long)slot * a.part_rows + row;
       if (!whole && row < a.part_rows && group == 0) *(float2*)(a.part_ml + at * 2) = make_float2(top, all);
-      // this group's half of the columns, 16 at a time: through shared memory (Q's place), so that four lanes store 64 bytes of a row
+      // this group's half of the columns, COLS at a time: through shared memory (Q's place), so that four lanes store 64 bytes of a row
+      constexpr int COLS = D / 4, BLOCKS = COLS / 16;
       const uint32_t to0 = tmem_base + TM_O + lane_off;
-      float4* turn = (float4*)(smem + L::Q_OFF) + warp * 128;
+      float4* turn = (float4*)(smem + L::Q_OFF) + warp * 128 * BLOCKS;
 #pragma unroll 1
-      for (int c = group * (D / 2); c < (group + 1) * (D / 2); c += 16) {
+      for (int c = group * (D / 2); c < (group + 1) * (D / 2); c += COLS) {
         if (busy) {
-          uint32_t o0[16], o1[16];
-          tmem_ld16(to0 + c, o0);
-          tmem_ld16(to0 + 128 + c, o1);
-          tmem_wait_ld();
-          float y[16];
+          uint32_t o0[BLOCKS][16], o1[BLOCKS][16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            y[i] = (has0 ? __uint_as_float(o0[i]) * f0 : 0.f) + (has1 ? __uint_as_float(o1[i]) * f1 : 0.f);
-            y[i] = live ? (whole ? y[i] * inv : y[i]) : 0.f;
+          for (int k = 0; k < BLOCKS; ++k) {
+            tmem_ld16(to0 + c + k * 16, o0[k]);
+            tmem_ld16(to0 + 128 + c + k * 16, o1[k]);
           }
+          tmem_wait_ld();
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) turn[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          for (int k = 0; k < BLOCKS; ++k) {
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              y[i] = (has0 ? __uint_as_float(o0[k][i]) * f0 : 0.f) + (has1 ? __uint_as_float(o1[k][i]) * f1 : 0.f);
+              y[i] = live ? (whole ? y[i] * inv : y[i]) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) turn[k * 128 + lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          }
           __syncwarp();
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int rl = i * 8 + (lane >> 2), rr = (warp & 3) * 32 + rl, piece = lane & 3;
-          const float4 z = busy ? turn[rl * 4 + (piece ^ ((rl >> 1) & 3))] : make_float4(0.f, 0.f, 0.f, 0.f);
+          const int rl = i * 8 + (lane >> 2), rr = (warp & 3) * 32 + rl, piece = lane & 3, at4 = rl * 4 + (piece ^ ((rl >> 1) & 3));
           if (!whole) {
-            if (rr < a.part_rows) *(float4*)(a.part_o + ((long)slot * a.part_rows + rr) * D + c + piece * 4) = z;
+            if (rr < a.part_rows) {
+              float* part = a.part_o + ((long)slot * a.part_rows + rr) * D + c + piece * 4;
+#pragma unroll
+              for (int k = 0; k < BLOCKS; ++k) *(float4*)(part + k * 16) = busy ? turn[k * 128 + at4] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
           } else {
             const int r2 = (w.hr - w.h * a.row_tiles) * CT_TILE + rr, t2 = r2 / a.G;
             if (t2 < a.T) {
               bf16* op = a.out + (((long)w.b * a.T + t2) * a.Hq + w.h * a.G + r2 - t2 * a.G) * D + c + piece * 4;
-              *(uint2*)op = make_uint2(pack_bf16x2(z.x, z.y), pack_bf16x2(z.z, z.w));
+#pragma unroll
+              for (int k = 0; k < BLOCKS; ++k) {
+                const float4 z = busy ? turn[k * 128 + at4] : make_float4(0.f, 0.f, 0.f, 0.f);
+                *(uint2*)(op + k * 16) = make_uint2(pack_bf16x2(z.x, z.y), pack_bf16x2(z.z, z.w));
+              }
             }
           }
         }
