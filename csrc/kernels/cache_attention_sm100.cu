@@ -167,14 +167,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
   volatile int* abort_flag = (volatile int*)(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // the deal uses the (not yet used) place of Q
-  const Deal deal = deal_tiles<CT_THREADS, CT_TILE, 1, CT_WHOLE>(a, (int*)smem);
-  release_join();
-  zero_empty<D, CT_THREADS>(a);
-  if (deal.first >= deal.last) {
-    if (threadIdx.x == 0) a.plan[blockIdx.x] = make_int4(0, 0, 0, 0);
-    return;
-  }
+  // both on their way while the deal waits for its loads
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
       mbar_init(&v_full[i], 4);
@@ -196,6 +189,15 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
   if (warp == 12) {
     tmem_alloc(tmem_ptr, 512);
     tmem_relinquish();
+  }
+  // the deal uses the (not yet used) place of Q
+  const Deal deal = deal_tiles<CT_THREADS, CT_TILE, 1, CT_WHOLE>(a, (int*)smem);
+  release_join();
+  zero_empty<D, CT_THREADS>(a);
+  if (deal.first >= deal.last) {
+    if (threadIdx.x == 0) a.plan[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (warp == 12) tmem_dealloc(*tmem_ptr, 512);
+    return;
   }
   Walk w;
   walk_begin<CT_TILE>(a, w, deal, 0);
