@@ -313,8 +313,12 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
           if (pos0 + g >= w.s.len) vs[0] = 0.f;
           if (pos0 + g + 8 >= w.s.len) vs[1] = 0.f;
         }
-        if (__any_sync(0xffffffffu, fmaxf(vs[0], vs[1]) > unit_v)) {
-          float top = fmaxf(vs[0], vs[1]);
+        // an infinite scale makes its own values no numbers, as a NaN does, and nothing else's unit: rows that do not see them have P = 0
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if ((__float_as_uint(vs[i]) & 0x7f800000u) == 0x7f800000u) vs[i] = __int_as_float(0x7fffffff);
+        float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));   // a NaN counts for nothing
+        if (__any_sync(0xffffffffu, top > unit_v)) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
           const float up = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
@@ -670,9 +674,15 @@ constexpr int CA_MAX_OCC = 4;
 // heads of D = 128): 16 rows bf16 8 x 2000 22 / 34, 8 x 16000 72 / 106, int8 28 / 37 and 80 / 145; 24 rows (32 of this one's) bf16 40 / 34
 // and 218 / 106, int8 42 / 37 and 212 / 145. With D = 64 and 24 rows it is 26 / 28 and 84 / 86, int8 28 / 31 and 95 / 112.
 constexpr long CA_MAX_ROWS = 16;
+// More rows go here too while what this kernel could read at most (every 16 rows their own keys and values, up to the table's end) is less
+// than so many bytes: its launch is half as long. Measured (us, this one / that one): 27 tokens of 4 heads, two sequences of 8 int8 heads of
+// 128, 77 tokens (3 MB) 10.3 / 12.6, 200 (6.5 MB) 13.3 / 13.7, 800 (24 MB) 25.5 / 20.6; 20 tokens, 16 heads of 64, bf16, 77 tokens (0.8 MB)
+// 7.1 / 10.4; 64 tokens, 16 heads of 64, int8, 200 tokens (2.2 MB) 10.9 / 15.8, 800 (7.1 MB) 20.1 / 16.2.
+constexpr double CA_SMALL = 5e6;
 static long ca_slots(bool tc) { return 2l * (tc ? 1 : CA_MAX_OCC) * sm_count(); }
 // Rows of a slot of partial results: a multiple of 4, so that what follows stays aligned.
-static int ca_part_rows(long rows) { return rows > CA_MAX_ROWS ? (int)(rows < 128 ? (rows + 3) & ~3l : 128) : 8 * ca_row_blocks(rows); }
+static int ca_part_rows(long rows, bool tc) { return tc ? (int)(rows < 128 ? (rows + 3) & ~3l : 128) : 8 * ca_row_blocks(rows); }
+static long ca_workspace(long rows, int D, bool tc) { return ca_slots(tc) * ca_part_rows(rows, tc) * (D * 4 + 8) + ca_slots(tc) / 2 * (16 + 4); }
 
 }  // namespace tb
 using namespace tb;
@@ -686,8 +696,8 @@ int tb_set_check_word_cache_attention(int* word) {
 // Bytes of workspace that tb_cache_attention needs for these sizes.
 TB_EXPORT long tb_cache_attention_workspace(int B, int T, int Hq, int Hkv, int D) {
   if (ensure_device() || Hkv <= 0) return -1;
-  const long rows = (long)T * (Hq / Hkv), slots = ca_slots(rows > CA_MAX_ROWS);
-  return slots * ca_part_rows(rows) * (D * 4 + 8) + slots / 2 * (16 + 4);
+  const long rows = (long)T * (Hq / Hkv), few = ca_workspace(rows, D, false), many = ca_workspace(rows, D, true);
+  return rows > CA_MAX_ROWS && many > few ? many : few;   // both kernels can be taken beyond CA_MAX_ROWS
 }
 
 // q [B, T, Hq, D] bf16 (strides in elements, multiples of 8; 16-byte aligned), out contiguous. ws: tb_cache_attention_workspace() bytes,
@@ -714,17 +724,18 @@ TB_EXPORT int tb_cache_attention(const CacheAttnCall* c, cudaStream_t st) {
   a.mask = c->mask, a.mask_b = c->mask_b, a.mask_t = c->mask_t, a.out = (bf16*)c->out;
   a.B = (int)c->B, a.T = (int)c->T, a.Hq = (int)c->Hq, a.Hkv = (int)c->Hkv, a.G = a.Hq / a.Hkv, a.page = (int)page, a.num_pages = (int)c->num_pages;
   a.scale_log2 = (float)(c->scale * 1.4426950408889634);
-  const bool tc = rows > CA_MAX_ROWS;
+  const long held = c->pages_per_seq * page, limit = held < c->max_len ? held : c->max_len;
+  const double most = (double)c->B * c->Hkv * ((rows + 15) / 16) * limit * D * (kind == CA_BF16 ? 4 : 2);
+  const bool tc = rows > CA_MAX_ROWS && most > CA_SMALL;
   const int nt = ca_row_blocks(rows);
   const int per_tile = tc ? 128 : 8 * nt;
   a.row_tiles = (int)((rows + per_tile - 1) / per_tile);
   a.page_tiles = (int)(page / CA_TILE);
   a.page_shift = (a.page_tiles & (a.page_tiles - 1)) ? -1 : __builtin_ctz((unsigned)a.page_tiles);
-  const long held = c->pages_per_seq * page, limit = held < c->max_len ? held : c->max_len;
   a.limit = (int)limit;
   if (limit > 0x7fff0000l || (double)(limit + CA_TILE) / CA_TILE * (double)ca_units(a) > 2e9) TB_FAIL(TB_E_TOO_LARGE, "cache attention: too much for one call");
   const long slots = ca_slots(tc);
-  a.part_rows = ca_part_rows(rows);
+  a.part_rows = ca_part_rows(rows, tc);
   a.part_o = (float*)c->ws;
   a.part_ml = a.part_o + slots * a.part_rows * D;
   a.plan = (int4*)(a.part_ml + slots * a.part_rows * 2);

@@ -6,12 +6,13 @@
 // values (64 KB in bf16, 33 KB in 8 bits, D = 128) take 2800 and 1450 clocks of the SM's share of HBM. So up to 128 rows cost what
 // the memory takes; mma.sync at 32 rows a CTA read every token rows / 32 times through L2 and was 2.5 to 8 times slower.
 //
-// Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 122 us, 4.5 TB/s. A tile
-// takes 2900 clocks, what the memory takes; the rest is the start (13 000 clocks until the first S: launch, deal, page table, first
-// copies) and the end of a unit (12 000 from the last P to the next unit's first S, in which the ring fills and then waits). 12 trees of 27
-// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 75 us. A tile takes 4300 clocks: 10 000 warp instructions (decoding,
+// Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 120 us, 4.6 TB/s. A tile
+// takes 2900 clocks, what the memory takes; the rest is the start (12 000 clocks until the first S: launch, deal, page table, first
+// copies) and the end of a unit (11 000 from the last P to the next unit's first S, in which the ring fills and then waits). 12 trees of 27
+// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 78 us (75 with the values' scales rounded to halves). A tile takes 4300 clocks: 10 000 warp instructions (decoding,
 // scales, exponentials) at 40 % of the issue slots, no pipe above 29 %, warps waiting for loads and for one another. Measured and not kept:
-// seven decoding warps (81 us), keys' scales in the halves (82), Q a unit ahead in a second place (122 and 86).
+// seven decoding warps (81 us for 75), keys' scales in the halves (82, and a rounding more), Q a unit ahead in a second place (122 for 121, 86
+// for 75).
 //
 // One CTA per SM, 512 threads:
 //   warps 0-3, 4-7  softmax, a thread per row, even tiles for the first four warps and odd ones for the others, each with a maximum, a sum
@@ -25,7 +26,7 @@
 // TMEM: S and P of even and of odd tiles 128 columns each (P takes the first half of the S it came from), then O of either.
 //
 // 8-bit scales: scores are multiplied by the key's scale in fp32. The value's goes into the halves, relative to a power of two for each
-// 32 tokens (what a loading warp has of a tile): one rounding (2^-11 at most) for the scale and one for the product, as P has one, where
+// 32 tokens (what a loading warp has of a tile), as the sum of two halves: one rounding (2^-11 at most) for the product, as P has one, where
 // carrying it in P cost the softmax 32 more loads of broadcast scales a tile (3.5 us instead of 2). P of those tokens is shifted by the
 // quotient of their power of two and the largest so far (`unit`), which O is relative to.
 #include "cache_attention.cuh"
@@ -325,6 +326,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
     // halves of the warp's codes of a tile, keys as they are, values times their token's `scale` (lane: token 32 pw + lane)
     auto convert = [&](auto is_value, const uint8_t* raw, uint8_t* dst, float scale, int first_new, uint32_t& odd) {
       constexpr bool VALUE = decltype(is_value)::value;
+      const __half s_hi = __float2half_rn(scale), s_lo = __float2half_rn(scale - __half2float(s_hi));
+      const uint32_t scale_halves = (uint32_t)__half_as_ushort(s_hi) | (uint32_t)__half_as_ushort(s_lo) << 16;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -349,9 +352,10 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
           halves_of<KIND>(v.z, hi.x, hi.y);
           halves_of<KIND>(v.w, hi.z, hi.w);
           if (VALUE) {
-            const __half2 sc = __float2half2_rn(__shfl_sync(0xffffffffu, scale, tok & 31));
-            auto times = [&](uint32_t& h) {
-              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h), sc);
+            const uint32_t both = __shfl_sync(0xffffffffu, scale_halves, tok & 31), sh = __byte_perm(both, 0u, 0x1010), sl = __byte_perm(both, 0u, 0x3232);
+            const __half2 hi2 = *reinterpret_cast<const __half2*>(&sh), lo2 = *reinterpret_cast<const __half2*>(&sl);
+            auto times = [&](uint32_t& h) {   // the smaller product first: one rounding
+              const __half2 x = *reinterpret_cast<const __half2*>(&h), y = __hfma2(x, hi2, __hmul2(x, lo2));
               h = *reinterpret_cast<const uint32_t*>(&y);
             };
             times(lo.x), times(lo.y), times(lo.z), times(lo.w), times(hi.x), times(hi.y), times(hi.z), times(hi.w);

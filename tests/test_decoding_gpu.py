@@ -930,3 +930,36 @@ def test_a_captured_step_of_a_paged_cache_goes_on():
     for (a, b), (sa, sb) in ((c.layers[0], c.scales[0]),):
         (ea, eb), (esa, esb) = eager.layers[0], eager.scales[0]
         assert torch.equal(a, ea) and torch.equal(b, eb) and torch.equal(sa, esa) and torch.equal(sb, esb)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.int8, E4M3])
+@pytest.mark.parametrize("wide", [0, 5000])
+@pytest.mark.parametrize("shape", [(3, 5, 64, 2, 64, 16, [0, 0, 20]), (2, 3, 48, 2, 128, 16, [300, 41]), (2, 33, 3, 1, 64, 16, [16, 250]), (2, 6, 32, 1, 128, 16, [37, 12]),
+                                   (4, 20, 3, 3, 64, 16, [5, 0, 33, 1]), (5, 17, 4, 2, 128, 48, [127, 128, 0, 129, 1]), (1, 1, 20, 1, 64, 16, [0])])
+def test_cache_attention_of_short_sequences_in_short_and_wide_tables(dtype, wide, shape):
+    """The width of the table decides which kernel takes many rows over little: both, with rows that see nothing, counts, scales below zero,
+    and infinities and NaN in new tokens that other rows do not see."""
+    from torsh_b200.ops.kv_cache import kv_cache_attention
+    q, kp, vp, ks, vs, table, start = _case(*shape, dtype)
+    B, T, _, H, D = shape[:5]
+    table = torch.nn.functional.pad(table, (0, wide), value=-1)
+    if ks is not None:
+        ks, vs = (x * torch.where(torch.rand(x.shape, device=DEV, generator=_gen(i)) < 0.5, -1, 1) for i, x in enumerate((ks, vs)))
+    g = _gen(T)
+    counts = torch.randint(0, T + 1, (B,), device=DEV, generator=g).int()
+    counts[0] = T
+    for mask, n in ((None, None), (torch.rand(T, T, device=DEV, generator=g) < 0.3, None), (torch.rand(B, T, T, device=DEV, generator=g) < 0.5, counts)):
+        got = kv_cache_attention(q, kp, vp, table, start, mask, n, ks, vs)
+        _attention_close(got, *_attend64(q, kp, vp, ks, vs, table, start, mask, n, D ** -0.5), dtype)
+    mask = torch.eye(T, dtype=torch.bool, device=DEV)
+    ref, mass = _attend64(q, kp, vp, ks, vs, table, start, mask, None, D ** -0.5)
+    pos = int(start[0]) + T // 2                                            # only row T // 2 of sequence 0 sees it
+    p, r = int(table[0, pos // shape[5]]), pos % shape[5]
+    if dtype == BF16:
+        vp[p, :, r, 3], vp[p, :, r, D - 1], kp[p, :, r, 5] = math.inf, math.nan, math.nan
+    else:
+        vs[p, :, r], ks[p, :, r] = math.inf, math.nan
+    got = kv_cache_attention(q, kp, vp, table, start, mask, None, ks, vs)
+    assert got[0, T // 2].isnan().any()
+    got[0, T // 2] = ref[0, T // 2].to(BF16)
+    _attention_close(got, ref, mass, dtype)

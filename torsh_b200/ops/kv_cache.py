@@ -255,8 +255,8 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     places that a row does not see do not reach it. ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
     not read. Pages outside the pool read as zeros. No backward pass.
 
-    For more than 16 query rows to a head of the cache the kernel turns 8-bit values into halves relative to the largest scale of their 32
-    positions: a value whose scale is less than 2^-25 of a neighbour's counts as zero, whether or not the row sees that neighbour.
+    8-bit values are multiplied as halves relative to a largest scale, that of the positions so far or (many query rows) of their 32 positions:
+    values with scales below 2^-14 of it lose precision and below 2^-25 count as zero, whether or not the row sees that largest one.
     """
     if q.is_cuda:
         out = (nv._decode or nv.decode_calls()).kv_attention(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, max_len,
