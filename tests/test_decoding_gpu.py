@@ -963,3 +963,57 @@ def test_cache_attention_of_short_sequences_in_short_and_wide_tables(dtype, wide
     assert got[0, T // 2].isnan().any()
     got[0, T // 2] = ref[0, T // 2].to(BF16)
     _attention_close(got, ref, mass, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.int8])
+@pytest.mark.parametrize("wide", [0, 5000])
+def test_cache_attention_of_queries_that_are_no_numbers(dtype, wide):
+    """A query with an infinity or a NaN spoils its own row."""
+    from torsh_b200.ops.kv_cache import kv_cache_attention
+    q, kp, vp, ks, vs, table, start = _case(2, 9, 8, 2, 64, 16, [200, 3], dtype)
+    table = torch.nn.functional.pad(table, (0, wide), value=-1)
+    ref, mass = _attend64(q, kp, vp, ks, vs, table, start, None, None, 0.125)
+    bad = q.clone()
+    bad[0, 4, 3, 5], bad[1, 0, 0, 0], bad[1, 8, 7] = math.nan, math.inf, math.nan
+    got = kv_cache_attention(bad, kp, vp, table, start, None, None, ks, vs)
+    for at in ((0, 4, 3), (1, 0, 0), (1, 8, 7)):
+        assert got[at].isnan().any()
+        got[at] = ref[at].to(BF16)
+    _attention_close(got, ref, mass, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_cache_attention_of_many_rows_captured_and_on_several_streams(dtype):
+    import threading
+    from torsh_b200.ops.kv_cache import kv_cache_attention
+    q, kp, vp, ks, vs, table, start = _case(6, 30, 8, 4, 64, 16, [900, 3, 77, 500, 0, 1300], dtype)
+    table = torch.nn.functional.pad(table, (0, 2000), value=-1)
+    starts = [start, start // 2, start // 3, torch.zeros_like(start)]
+    want = [kv_cache_attention(q, kp, vp, table, s, None, None, ks, vs) for s in starts]
+    held, graphs = start.clone(), []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = kv_cache_attention(q, kp, vp, table, held, None, None, ks, vs)
+        graphs.append((graph, out))
+    for s, w in zip(starts, want):
+        held.copy_(s)
+        for graph, out in graphs:
+            out.zero_()
+            graph.replay()
+        assert all(torch.equal(out, w) for _, out in graphs)
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [kv_cache_attention(q, kp, vp, table, starts[i], None, None, ks, vs) for _ in range(25)]
+            torch.cuda.current_stream().synchronize()
+            got[i] = outs
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(o, w) for outs, w in zip(got, want) for o in outs)
