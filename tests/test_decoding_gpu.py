@@ -218,6 +218,21 @@ def test_cache_write_and_read(dtype, xdtype, B, T, H, D, page):
                 assert torch.equal(got[b, :n], (codes * unit).float().to(out))   # code times scale is exact in 32 bits
 
 
+@pytest.mark.parametrize("dtype", [torch.int8, E4M3])
+def test_rows_are_quantised_alike_on_every_device(dtype):
+    from torsh_b200.ops.kv_cache import kv_cache_write, quantize_rows
+    x = torch.randn(3000, 96, device=DEV, generator=_gen(2)) * torch.exp(4 * torch.randn(3000, 1, device=DEV, generator=_gen(3)))
+    here, there = quantize_rows(x, dtype), quantize_rows(x.cpu(), dtype)
+    for a, b in zip(here, there):
+        assert torch.equal(a.cpu().view(torch.int8), b.view(torch.int8))
+    rows = x[:48, :64].contiguous()                                         # and as the kernel does it
+    kp, vp, ks, vs = _cache(1, 3, 16, 64, dtype, 0)
+    kv_cache_write(rows.view(1, 16, 3, 64), rows.view(1, 16, 3, 64), kp, vp, torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV),
+                   None, ks, vs)
+    codes, scale = quantize_rows(rows, dtype)
+    assert torch.equal(kp.transpose(1, 2).reshape(48, 64).view(torch.int8), codes.view(torch.int8)) and torch.equal(ks.transpose(1, 2).reshape(48), scale)
+
+
 def test_cache_rows_that_are_not_numbers():
     from torsh_b200.ops.kv_cache import kv_cache_read, kv_cache_write
     k = torch.randn(1, 4, 2, 64, device=DEV, generator=_gen(5)).to(BF16)

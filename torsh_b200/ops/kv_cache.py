@@ -82,7 +82,7 @@ def quantize_rows(x: torch.Tensor, dtype: torch.dtype):
         return x.to(dtype), None
     big = x.float().abs().amax(-1)
     if dtype == torch.int8:
-        scale = big / 127
+        scale = big / torch.full_like(big, 127)     # by a tensor: by a number, a GPU multiplies with the rounded 1 / 127
     else:
         m, e = torch.frexp(big)
         scale = ((e.long() - 9 + (m > 0.875) + 1023) << 52).view(torch.float64).float()   # from the bits: exact on every device
