@@ -103,6 +103,8 @@ bool pages_ok(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? (T*)t.const_data_ptr() : nullptr; }
 
+// Forward-mode derivatives: a tensor that carries a tangent looks like any other, and the kernels would drop it.
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 int current() { return c10::cuda::current_device(); }
 PyObject* pair(const Tensor& a, const Tensor& b) {
@@ -191,6 +193,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (freqs.scalar_type() != at::kDouble || freqs.dim() != 1 || !freqs.is_contiguous() || 2 * freqs.numel() > std::min<int64_t>(q.size(-1), 512)) Py_RETURN_NONE;
   if (k.defined() && (!here(k, device) || k.scalar_type() != q.scalar_type() || k.dim() != dims || k.size(-1) != q.size(-1) || k.sizes().slice(0, dims - 2) != q.sizes().slice(0, dims - 2)))
     Py_RETURN_NONE;
+  if (dual(q) || dual(k) || dual(freqs)) Py_RETURN_NONE;
   const int interleaved = PyObject_IsTrue(args[4]);
   const double magnitude = PyFloat_AsDouble(args[5]);
   if (interleaved < 0 || (magnitude == -1.0 && PyErr_Occurred())) return nullptr;
@@ -221,7 +224,7 @@ PyObject* py_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!here(k, device) || !here(v, device) || k.dim() != 4 || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || row_type(k.scalar_type()) < 0) Py_RETURN_NONE;
   const int64_t B = k.size(0);
   if (!pages_ok(kp, vp, ks, vs, table, device, B) || kp.size(1) != k.size(2) || kp.size(3) != k.size(3) || !rows16(k) || !rows16(v)) Py_RETURN_NONE;
-  if (!ints(start, B, device) || (counts.defined() && !ints(counts, B, device)) || wants_grad(k) || wants_grad(v)) Py_RETURN_NONE;
+  if (!ints(start, B, device) || (counts.defined() && !ints(counts, B, device)) || wants_grad(k) || wants_grad(v) || dual(k) || dual(v)) Py_RETURN_NONE;
   if (k.numel() == 0) Py_RETURN_TRUE;
   KvCall c{};
   const Tensor* x[2] = {&k, &v};
@@ -250,6 +253,7 @@ PyObject* py_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (table.dim() != 2 || most < 0 || most > 0x7fffffff) Py_RETURN_NONE;
   const int64_t B = table.size(0);
   if (!pages_ok(kp, vp, ks, vs, table, device, B) || !ints(lengths, B, device) || (begin.defined() && !ints(begin, B, device))) Py_RETURN_NONE;
+  if (dual(kp) || dual(vp) || dual(ks) || dual(vs)) Py_RETURN_NONE;
   const bool wide = PyObject_IsTrue(args[8]) == 1;
   const auto options = kp.options().dtype(wide ? at::kFloat : at::kBFloat16);
   Tensor k = at::empty({B, most, kp.size(1), kp.size(3)}, options), v = at::empty({B, most, kp.size(1), kp.size(3)}, options);
@@ -278,6 +282,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3);
   if (!pages_ok(kp, vp, ks, vs, table, device, B) || kp.size(3) != D || kp.size(1) == 0 || Hq % kp.size(1) || !rows16(q)) Py_RETURN_NONE;
   if (!ints(start, B, device) || (counts.defined() && !ints(counts, B, device)) || wants_grad(q)) Py_RETURN_NONE;
+  if (dual(q) || dual(kp) || dual(vp) || dual(ks) || dual(vs)) Py_RETURN_NONE;
   CacheAttnCall c{};
   if (mask.defined()) {
     const int64_t m = mask.dim();

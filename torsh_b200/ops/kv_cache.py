@@ -19,6 +19,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from .. import _native as nv
 
@@ -63,6 +64,11 @@ def _int32(t):
 def _no_grad(what, *tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under no_grad()")
+
+
+def _no_tangent(what, *tensors):
+    if any(fwd.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: what is read back would not carry it")
 
 
 def _table(page_table):
@@ -130,6 +136,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     ``k`` and ``v`` are ``[B, T, H, D]``; token ``t`` of sequence ``b`` goes to position ``start[b] + t``, tokens from ``counts[b]`` on are
     left out, and so are sequences whose ``start`` is negative. Positions that the table does not reach, or to which it gives a page
     outside the pool, are skipped (and reported where the device-side index checks are on). Two sequences may share pages, but not the positions that one call writes.
+    No derivatives, of either mode: such inputs are refused.
     """
     if k.is_cuda and (nv._decode or nv.decode_calls()).kv_write(k, v, k_pages, v_pages, page_table, start, counts, k_scales, v_scales):
         return
@@ -141,6 +148,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     if k_pages.shape[1] != H or k_pages.shape[3] != D or v.device != k.device:
         raise ValueError(f"kv_cache_write: pages of {k_pages.shape[1]} heads of {k_pages.shape[3]}, rows of {H} of {D}")
     _no_grad("kv_cache_write", k, v)
+    _no_tangent("kv_cache_write", k, v)
     start = _per_sequence("kv_cache_write", "start", start, B, k.device)
     if counts is not None:
         counts = _per_sequence("kv_cache_write", "counts", counts, B, k.device)
@@ -253,7 +261,7 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     ``tree_mask[t, j]`` (bool, ``[T, T]`` or ``[B, T, T]``; :func:`tree_mask_of`) - without a mask those up to itself. ``T = 1`` is an
     ordinary decoding step. Rows from ``counts[b]`` on, and rows that see nothing, come out as zeros; infinities and NaN in
     places that a row does not see do not reach it. ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
-    not read. Pages outside the pool read as zeros. No backward pass.
+    not read. Pages outside the pool read as zeros. No backward pass; forward-mode derivatives are computed in PyTorch.
 
     8-bit values are multiplied as halves relative to a largest scale, that of the positions so far or (many query rows) of their 32 positions:
     values with scales below 2^-14 of it lose precision and below 2^-25 count as zero, whether or not the row sees that largest one.
