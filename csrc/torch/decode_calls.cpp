@@ -193,7 +193,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (freqs.scalar_type() != at::kDouble || freqs.dim() != 1 || !freqs.is_contiguous() || 2 * freqs.numel() > std::min<int64_t>(q.size(-1), 512)) Py_RETURN_NONE;
   if (k.defined() && (!here(k, device) || k.scalar_type() != q.scalar_type() || k.dim() != dims || k.size(-1) != q.size(-1) || k.sizes().slice(0, dims - 2) != q.sizes().slice(0, dims - 2)))
     Py_RETURN_NONE;
-  if (dual(q) || dual(k) || dual(freqs)) Py_RETURN_NONE;
+  if (dual(q) || dual(k) || dual(freqs) || wants_grad(freqs)) Py_RETURN_NONE;   // frequencies that learn: the kernel has no gradient for them
   const int interleaved = PyObject_IsTrue(args[4]);
   const double magnitude = PyFloat_AsDouble(args[5]);
   if (interleaved < 0 || (magnitude == -1.0 && PyErr_Occurred())) return nullptr;

@@ -118,3 +118,39 @@ def test_cache_writes_refuse_tangents():
     assert not kp.any() and not vp.any()
     kv_cache_write(k, k, kp, vp, table, start)
     assert kp[0, 0, :3].eq(1).all() and not math.isnan(float(kp.sum()))
+
+
+# ------------------------------------------------------------------------------------------------ learned frequencies
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("which", ["freqs", "all"])
+def test_rotary_gives_frequencies_their_gradient(interleaved, which):
+    """dL/df_i = sum over tokens and heads of p (dy_b y_a - dy_a y_b), against 64 bits and differences. A pair's term is two products of
+    fp32 numbers, each off by a few units; their sum over tokens in fp32 or more: 64 units of the sum of magnitudes. Freqs are fp64 and so is the last sum."""
+    from torsh_b200.ops.rotary import rotary
+    q, k, dq, dk, pos, freqs = _setup(interleaved)
+    pos = pos % 50
+    f = freqs.clone().requires_grad_()
+    a, b = (x.clone().requires_grad_(which == "all") for x in (q, k))
+    outs = rotary(a, b, pos, f, interleaved)
+    wrt = (f, a, b) if which == "all" else (f,)
+    grads = torch.autograd.grad(outs, wrt, (dq, dk))
+    want, size = torch.zeros_like(freqs), torch.zeros_like(freqs)
+    h = freqs.numel()
+    i = torch.arange(h, device=DEV)
+    ia, ib = (2 * i, 2 * i + 1) if interleaved else (i, i + h)
+    for x, dy in ((q, dq), (k, dk)):
+        y = _turn64(x, pos, freqs, interleaved)
+        p = pos.double()[..., None, None]
+        terms = p * dy.double()[..., ib] * y[..., ia], -p * dy.double()[..., ia] * y[..., ib]
+        want += sum(t.sum((0, 1, 2)) for t in terms)
+        size += sum(t.abs().sum((0, 1, 2)) for t in terms)
+    assert grads[0].dtype == torch.float64 and ((grads[0] - want).abs() <= 64 * UNIT * size).all()
+
+    def loss(fr):
+        return sum((d.double() * _turn64(x, pos, fr, interleaved)).sum() for x, d in ((q, dq), (k, dk)))
+    e = torch.zeros_like(freqs)
+    e[3] = 1e-6
+    assert abs((loss(freqs + e) - loss(freqs - e)) / 2e-6 - want[3]) <= 1e-6 * size[3] + 1e-4   # the formula itself
+    if which == "all":
+        for g, d in zip(grads[1:], (dq, dk)):
+            _close(g, _turn64(d, pos, freqs, interleaved, 1.0, True), d)

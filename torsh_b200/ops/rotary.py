@@ -80,7 +80,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     ``q`` is ``[..., Hq, D]``, ``k`` ``[..., Hk, D]`` with the same leading dimensions (``[B, T]`` or ``[tokens]``), ``positions``
     integers of those dimensions or fewer (``[T]`` serves every sequence). ``freqs`` (:func:`rotary_frequencies`) has one entry per
     pair: ``2 * len(freqs)`` columns of ``D`` turn, the rest pass through. ``interleaved`` pairs columns ``(2i, 2i + 1)``, as
-    :func:`~torsh_b200.ops.elementwise.rope` does; otherwise ``(i, i + len(freqs))``. Differentiable in ``q`` and ``k``; forward-mode derivatives are computed in PyTorch.
+    :func:`~torsh_b200.ops.elementwise.rope` does; otherwise ``(i, i + len(freqs))``. Differentiable in ``q`` and ``k``; forward-mode derivatives, and calls whose
+    ``freqs`` require a gradient, are computed in PyTorch.
     """
     if q.is_cuda:
         out = (nv._decode or nv.decode_calls()).rotary(q, k, positions, freqs, interleaved, magnitude)
