@@ -149,6 +149,19 @@ std::pair<Tensor, Tensor> turn(const Tensor& q, const Tensor& k, const Tensor& p
   launch(rotary_fn, c, q.get_device(), "tb_rotary", 1);
   return {yq, yk};
 }
+// Gradients that the kernel does not read (batched ones have no memory of their own, dual ones a tangent): the formula in PyTorch. With the GIL held.
+Tensor turn_plain(const Tensor& x, const Tensor& pos, const Tensor& freqs, bool interleaved, double magnitude, bool inverse) {
+  struct Held {
+    PyObject* p;
+    Held(PyObject* p) : p(p) {
+      if (!p) raise_set();
+    }
+    ~Held() { Py_DECREF(p); }
+  };
+  const Held module(PyImport_ImportModule("torsh_b200.ops.rotary")), px(THPVariable_Wrap(x)), pp(THPVariable_Wrap(pos)), pf(THPVariable_Wrap(freqs));
+  const Held y(PyObject_CallMethod(module.p, "_rotary_plain", "OOOOdO", px.p, pp.p, pf.p, interleaved ? Py_True : Py_False, magnitude, inverse ? Py_True : Py_False));
+  return THPVariable_Unpack(y.p);
+}
 struct RotaryFn : public torch::autograd::Function<RotaryFn> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor q, std::optional<Tensor> k, Tensor pos, Tensor freqs, bool interleaved, double magnitude, bool inverse) {
     ctx->save_for_backward({pos, freqs});
@@ -171,7 +184,9 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
     } release{gil};
     const std::optional<Tensor> dk = dy.size() > 1 ? std::optional<Tensor>(dy[1]) : std::nullopt;
     torch::autograd::variable_list d;
-    if (at::GradMode::is_enabled()) {
+    if (!plain_dense(dy[0]) || dual(dy[0]) || (dk && (!plain_dense(*dk) || dual(*dk)))) {
+      for (const Tensor& x : dy) d.push_back(turn_plain(x, saved[0], saved[1], interleaved, magnitude, !inverse));
+    } else if (at::GradMode::is_enabled()) {
       d = RotaryFn::apply(dy[0], dk, saved[0], saved[1], interleaved, magnitude, !inverse);
     } else {
       auto y = turn(dy[0], dk ? *dk : Tensor(), saved[0], saved[1], interleaved, magnitude, !inverse);

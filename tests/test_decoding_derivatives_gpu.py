@@ -154,3 +154,46 @@ def test_rotary_gives_frequencies_their_gradient(interleaved, which):
     if which == "all":
         for g, d in zip(grads[1:], (dq, dk)):
             _close(g, _turn64(d, pos, freqs, interleaved, 1.0, True), d)
+
+
+# ------------------------------------------------------------------------------------------------ batched gradients, tangents of gradients
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_batched_gradients_of_rotary(interleaved):
+    """The framework's reverse-mode Jacobian: one batched backward pass."""
+    from torsh_b200.autograd import transforms
+    from torsh_b200.ops.rotary import rotary, rotary_frequencies
+    freqs, _ = rotary_frequencies(4, device=DEV)
+    x, k, pos = torch.randn(2, 1, 6, device=DEV, generator=_gen(1)), torch.randn(2, 2, 6, device=DEV, generator=_gen(2)), torch.tensor([3, 900], device=DEV)
+    eye = torch.eye(12, device=DEV).view(12, 2, 1, 6)
+    want = torch.stack([_turn64(e, pos, freqs, interleaved) for e in eye], -1).view(2, 1, 6, 2, 1, 6)
+    for other in (None, k):                                                 # alone, and as one of two
+        _close(transforms.jacrev(lambda a: rotary(a, other, pos, freqs, interleaved)[0])(x), want, torch.ones(1))
+        with torch.no_grad():
+            _close(transforms.jacrev(lambda a: torch.enable_grad()(rotary)(a, other, pos, freqs, interleaved)[0])(x), want, torch.ones(1))
+    # both outputs, several gradients at once, differentiated again in those gradients
+    a, b = x.clone().requires_grad_(), k.clone().requires_grad_()
+    outs = rotary(a, b, pos, freqs, interleaved, 1.25)
+    da, db = (torch.randn(3, *y.shape, device=DEV, generator=_gen(4)).requires_grad_() for y in outs)
+    ga, gb = torch.autograd.grad(outs, (a, b), (da, db), is_grads_batched=True, create_graph=True)
+    for i in range(3):
+        for g, d in ((ga, da), (gb, db)):
+            _close(g[i].detach(), _turn64(d[i].detach(), pos, freqs, interleaved, 1.25, True), d.detach(), 1.25)
+    w = torch.randn_like(ga)
+    (gg,) = torch.autograd.grad((ga * w).sum(), da)
+    for i in range(3):
+        _close(gg[i], _turn64(w[i], pos, freqs, interleaved, 1.25), w, 1.25)
+
+
+def test_gradients_that_carry_tangents():
+    """Reverse mode first, forward mode through its backward pass."""
+    from torsh_b200.ops.rotary import rotary
+    q, k, dq, dk, pos, freqs = _setup(True)
+    a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+    outs = rotary(a, b, pos, freqs)
+    t = torch.randn_like(dq)
+    with fwd.dual_level():
+        ga, gb = torch.autograd.grad(outs, (a, b), (fwd.make_dual(dq, t), dk))
+        ga = fwd.unpack_dual(ga)
+    _close(ga.primal, _turn64(dq, pos, freqs, True, 1.0, True), dq)
+    _close(ga.tangent, _turn64(t, pos, freqs, True, 1.0, True), t)
+    _close(gb, _turn64(dk, pos, freqs, True, 1.0, True), dk)

@@ -69,7 +69,7 @@ def _rotary_plain(x, positions, freqs, interleaved, magnitude, inverse):
     r, rest = xf[..., :rot], xf[..., rot:]
     a, b = (r[..., 0::2], r[..., 1::2]) if interleaved else (r[..., :rot // 2], r[..., rot // 2:])
     u, w = a * cos - b * sin, a * sin + b * cos
-    turned = torch.stack([u, w], -1).flatten(-2) if interleaved else torch.cat([u, w], -1)
+    turned = torch.stack([u, w], -1).reshape(r.shape) if interleaved else torch.cat([u, w], -1)
     return torch.cat([turned, rest], -1).to(x.dtype)
 
 
