@@ -1,0 +1,53 @@
+"""A paged cache whose batch has places without a sequence, and lengths that the host knows only as upper bounds."""
+import pytest
+import torch
+
+from torsh_b200.ops.kv_cache import PagedKVCache
+
+
+def _cache(batch=2, max_len=64, num_pages=None, **kw):
+    return PagedKVCache(1, 1, 8, batch=batch, max_len=max_len, dtype=torch.float32, page=16, num_pages=num_pages, device="cpu", **kw)
+
+
+def _rows(batch, T, seed):
+    g = torch.Generator().manual_seed(seed)
+    return tuple(torch.randn(batch, T, h, 8, generator=g) for h in (2, 1, 1))
+
+
+@pytest.mark.parametrize("form", ["tensor", "bounded", "int", "list"])
+@pytest.mark.parametrize("used", [False, True])
+def test_a_place_without_a_sequence_stays_empty(form, used):
+    """Steps of a batch advance every place; those without a sequence (never used, or released) neither grow, nor get pages, nor stop the
+    others, and the sequence that comes to such a place begins at position 0."""
+    c = _cache(num_pages=5)
+    if used:
+        c.reserve([4, 20])
+        c.write(0, *_rows(2, 20, 9)[1:])
+        c.advance([0, 20])
+        c.release(1)
+    free, steps = len(c._free), 60
+    for i in range(steps):
+        c.reserve([1, 0])
+        q, k, v = _rows(2, 1, i)
+        c.write(0, k, v)
+        assert not c.attend(0, q)[1].any()
+        one = torch.ones(2, dtype=torch.int64)
+        if form == "bounded":
+            c.advance(one, most=1)
+        else:
+            c.advance({"tensor": one, "int": 1, "list": [1, 1]}[form])
+    assert c.lengths.tolist() == [steps, 0] and not (c.page_table[1] >= 0).any()
+    assert len(c._free) + 4 == 5 >= free and c.read(0, torch.float32)[0].shape[1] == steps
+    # a sequence comes
+    fresh = _cache(batch=1)
+    c.reserve([0, 3])
+    fresh.reserve(3)
+    q, k, v = _rows(2, 3, 77)
+    c.write(0, k, v)
+    fresh.write(0, k[1:], v[1:])
+    # the batch is as wide as its longest sequence: sums of 8 and 3 products (and zeros) below 8, perhaps in another order, 16 units of 2^-24 * 8
+    torch.testing.assert_close(c.attend(0, q)[1:], fresh.attend(0, q[1:]), rtol=0, atol=2.0 ** -17)
+    assert torch.equal(c.attend(0, q)[1, 0], v[1, 0].expand(2, 8))          # the first token sees itself alone
+    c.advance(torch.tensor([0, 3]))
+    assert c.lengths.tolist() == [steps, 3] and c.host_lengths == [steps, 3]
+    assert torch.equal(c.read(0, torch.float32)[0][1, :3], k[1])

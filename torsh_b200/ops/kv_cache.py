@@ -348,9 +348,14 @@ class PagedKVCache:
         self._owned: list[list[int]] = [[] for _ in range(batch)]
         self._free = list(range(num_pages - 1, -1, -1))
 
+    def _bounds(self) -> list[int]:
+        """``host_lengths`` without what batched steps have added to places that have no pages, whose lengths are 0."""
+        return [n if own else 0 for n, own in zip(self.host_lengths, self._owned)]
+
     def reserve(self, tokens) -> None:
         """Room for ``tokens`` (an int, or one per sequence) more tokens of every sequence. Raises where the pool or ``max_len`` has none."""
         tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
+        self.host_lengths = self._bounds()
         need = [max(0, -(-(n + t) // self.page) - len(own)) for n, t, own in zip(self.host_lengths, tokens, self._owned)]
         for n, t in zip(self.host_lengths, tokens):
             if n + t > self.max_len:
@@ -378,7 +383,7 @@ class PagedKVCache:
     def read(self, layer: int, dtype: torch.dtype = torch.bfloat16):
         """All keys and values of a layer, ``[B, longest, H, D]``."""
         (kp, vp), (ks, vs) = self.layers[layer], self.scales[layer]
-        return kv_cache_read(kp, vp, self.page_table, self.lengths, max(self.host_lengths, default=0), None, ks, vs, dtype)
+        return kv_cache_read(kp, vp, self.page_table, self.lengths, max(self._bounds(), default=0), None, ks, vs, dtype)
 
     def keep(self, path: torch.Tensor, accepted: torch.Tensor) -> None:
         """Moves the accepted nodes of a tree (:func:`~torsh_b200.ops.speculative.verify_draft`) to the front of the tokens just written,
@@ -401,23 +406,25 @@ class PagedKVCache:
                     x[dst, :, drow] = x[src, :, srow]
 
     def advance(self, tokens, most: int | None = None) -> None:
-        """The last ``tokens`` that were written belong to their sequences now: an int, one per sequence, or a device vector of at most ``most``."""
+        """The last ``tokens`` that were written belong to their sequences now: an int, one per sequence, or a device vector of at most ``most``.
+        Places without a sequence stay empty, whatever they are given."""
+        taken = (self.page_table >= 0).any(1)
         if isinstance(tokens, torch.Tensor):
-            self.lengths += tokens.to(torch.int32)
+            self.lengths += torch.where(taken, tokens.to(torch.int32), 0)
             if most is None:
                 self.host_lengths = self.lengths.tolist()
             else:
                 self.host_lengths = [n + most for n in self.host_lengths]
             return
         tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
-        self.lengths += torch.tensor(tokens, dtype=torch.int32, device=self.lengths.device)
-        self.host_lengths = [n + t for n, t in zip(self.host_lengths, tokens)]
+        self.lengths += torch.where(taken, torch.tensor(tokens, dtype=torch.int32, device=self.lengths.device), 0)
+        self.host_lengths = [n + t if own else 0 for n, t, own in zip(self.host_lengths, tokens, self._owned)]
 
     def truncate(self, lengths) -> None:
         """Shortens the sequences to ``lengths`` (one per sequence): what lies behind is written over. Their pages stay theirs."""
         lengths = [int(n) for n in lengths]
-        if len(lengths) != self.batch or any(not 0 <= n <= was for n, was in zip(lengths, self.host_lengths)):
-            raise ValueError(f"PagedKVCache: lengths {lengths} of sequences that have {self.host_lengths}")
+        if len(lengths) != self.batch or any(not 0 <= n <= was for n, was in zip(lengths, self._bounds())):
+            raise ValueError(f"PagedKVCache: lengths {lengths} of sequences that have {self._bounds()}")
         self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
         self.host_lengths = lengths
 
