@@ -51,3 +51,26 @@ def test_a_place_without_a_sequence_stays_empty(form, used):
     c.advance(torch.tensor([0, 3]))
     assert c.lengths.tolist() == [steps, 3] and c.host_lengths == [steps, 3]
     assert torch.equal(c.read(0, torch.float32)[0][1, :3], k[1])
+
+
+def test_truncating_never_lengthens():
+    """After a bounded advance the host has upper bounds: a length between what a sequence has and that bound leaves it as it is."""
+    c = _cache()
+    c.reserve([20, 20])
+    q, k, v = _rows(2, 5, 1)
+    c.write(0, k, v)
+    c.advance(torch.tensor([1, 4]), most=5)
+    c.truncate([5, 3])
+    assert c.lengths.tolist() == [1, 3] and all(n >= m for n, m in zip(c.host_lengths, [1, 3]))
+    # the next token sees what was accepted, and itself
+    q, k2, v2 = _rows(2, 1, 2)
+    c.write(0, k2, v2)
+    got = c.attend(0, q)
+    for b, n in enumerate((1, 3)):
+        kk, vv = torch.cat([k[b, :n, 0], k2[b, :, 0]]), torch.cat([v[b, :n, 0], v2[b, :, 0]])
+        torch.testing.assert_close(got[b, 0], torch.softmax(q[b, 0] @ kk.T / 8 ** 0.5, -1) @ vv)
+    for bad in ([6, 0], [-1, 0], [1], [1, 1, 1]):
+        with pytest.raises(ValueError):
+            c.truncate(bad)
+    c.truncate([0, 2])
+    assert c.lengths.tolist() == [0, 2]

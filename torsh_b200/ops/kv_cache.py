@@ -421,11 +421,13 @@ class PagedKVCache:
         self.host_lengths = [n + t if own else 0 for n, t, own in zip(self.host_lengths, tokens, self._owned)]
 
     def truncate(self, lengths) -> None:
-        """Shortens the sequences to ``lengths`` (one per sequence): what lies behind is written over. Their pages stay theirs."""
+        """Shortens the sequences to ``lengths`` (one per sequence; shorter ones stay as they are): what lies behind is written over. Their pages
+        stay theirs."""
         lengths = [int(n) for n in lengths]
         if len(lengths) != self.batch or any(not 0 <= n <= was for n, was in zip(lengths, self._bounds())):
             raise ValueError(f"PagedKVCache: lengths {lengths} of sequences that have {self._bounds()}")
-        self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        # the host may know upper bounds only: nothing gets longer
+        self.lengths.copy_(torch.minimum(self.lengths, torch.tensor(lengths, dtype=torch.int32, device=self.lengths.device)))
         self.host_lengths = lengths
 
     def release(self, b: int) -> None:
