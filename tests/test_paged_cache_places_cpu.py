@@ -74,3 +74,28 @@ def test_truncating_never_lengthens():
             c.truncate(bad)
     c.truncate([0, 2])
     assert c.lengths.tolist() == [0, 2]
+
+
+def test_upper_bounds_refuse_nothing_that_there_is_room_for():
+    """Steps that keep one token of five: the bounds pass max_len, and what the pool has, long before the sequences do."""
+    c = _cache(batch=1, num_pages=4)
+    for i in range(59):
+        c.reserve(5)
+        q, k, v = _rows(1, 5, i)
+        c.write(0, k, v)
+        c.advance(torch.tensor([1]), most=5)
+    assert c.lengths.tolist() == [59] and 59 <= c.host_lengths[0] <= 64
+    for i in range(59):
+        assert torch.equal(c.read(0, torch.float32)[0][0, i], _rows(1, 5, i)[1][0, 0])
+    c.reserve(5)
+    for n in (6, 1000):
+        with pytest.raises(ValueError):
+            c.reserve(n)
+    two = _cache(num_pages=4)
+    two.reserve(30)
+    two.advance(torch.tensor([1, 1]), most=30)
+    two.reserve(30)
+    with pytest.raises(RuntimeError):
+        two.reserve([40, 0])
+    two.reserve([0, 31])
+    assert len(two._free) == 0 and two.lengths.tolist() == [1, 1]

@@ -323,7 +323,8 @@ class PagedKVCache:
     are common. A step is: :meth:`reserve` room for the new tokens of the batch, for each layer :meth:`write` their keys and values and
     :meth:`attend`, then :meth:`advance` the lengths by what is kept (after a verification fewer than were written: the rest is
     written over). Table and lengths are device tensors that are written in place, so a step with ``advance(tensor, most)`` can be captured
-    into a graph and replayed while what has been reserved lasts. Places of the batch that have no sequence have no pages: what a batched
+    into a graph and replayed while what has been reserved lasts; after one, :meth:`reserve`, :meth:`read` and :meth:`truncate` ask the device for the
+    lengths. Places of the batch that have no sequence have no pages: what a batched
     step writes for them is left out, and what it reads is zeros.
     """
 
@@ -345,21 +346,31 @@ class PagedKVCache:
         self.page_table = torch.full((batch, per), -1, dtype=torch.int32, device=device)   # -1: no page
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.host_lengths = [0] * batch           # upper bounds: what advance() has been told on the host
+        self._replayed = False                    # an advance() has been captured: only the device knows how often it has run
         self._owned: list[list[int]] = [[] for _ in range(batch)]
         self._free = list(range(num_pages - 1, -1, -1))
 
-    def _bounds(self) -> list[int]:
-        """``host_lengths`` without what batched steps have added to places that have no pages, whose lengths are 0."""
+    def _capturing(self) -> bool:
+        return self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
+
+    def _bounds(self, exact: bool = False) -> list[int]:
+        """``host_lengths``, brought up to date from the device where replays may have changed them (or where asked to), without what batched
+        steps have added to places that have no pages, whose lengths are 0."""
+        if (exact or self._replayed) and not self._capturing():
+            self.host_lengths = self.lengths.tolist()
         return [n if own else 0 for n, own in zip(self.host_lengths, self._owned)]
 
     def reserve(self, tokens) -> None:
         """Room for ``tokens`` (an int, or one per sequence) more tokens of every sequence. Raises where the pool or ``max_len`` has none."""
         tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
-        self.host_lengths = self._bounds()
-        need = [max(0, -(-(n + t) // self.page) - len(own)) for n, t, own in zip(self.host_lengths, tokens, self._owned)]
-        for n, t in zip(self.host_lengths, tokens):
-            if n + t > self.max_len:
-                raise ValueError(f"PagedKVCache: {n + t} tokens in a sequence, room for {self.max_len}")
+        for exact in (False, True):               # upper bounds first: what does not fit them is asked of the device
+            self.host_lengths = self._bounds(exact)
+            need = [max(0, -(-(n + t) // self.page) - len(own)) for n, t, own in zip(self.host_lengths, tokens, self._owned)]
+            longest = max((n + t for n, t in zip(self.host_lengths, tokens)), default=0)
+            if longest <= self.max_len and sum(need) <= len(self._free):
+                break
+        if longest > self.max_len:
+            raise ValueError(f"PagedKVCache: {longest} tokens in a sequence, room for {self.max_len}")
         if sum(need) > len(self._free):
             raise RuntimeError(f"PagedKVCache: {sum(need)} pages wanted, {len(self._free)} free")
         for b, n in enumerate(need):
@@ -415,6 +426,7 @@ class PagedKVCache:
                 self.host_lengths = self.lengths.tolist()
             else:
                 self.host_lengths = [n + most for n in self.host_lengths]
+            self._replayed = self._replayed or self._capturing()
             return
         tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
         self.lengths += torch.where(taken, torch.tensor(tokens, dtype=torch.int32, device=self.lengths.device), 0)
