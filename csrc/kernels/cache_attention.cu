@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
     if (more) {
       const long next_row = row_of(a, next, ld.h);
       const int live = next_row < 0 ? 0 : min(ld.s.len - ld.tile * CA_TILE, CA_TILE);
-      if (next_row < 0 && lane == 0) report_bad_index();
+      if (next_row < 0 && lane == 0 && !vacant_place(a.table + (long)ld.b * a.table_ld, next.page)) report_bad_index();
       const long row = max(next_row, 0l);
       const uint8_t* kp = (const uint8_t*)a.k_pages + row * S::ROW + lane * 16;
       const uint8_t* vp = (const uint8_t*)a.v_pages + row * S::ROW + lane * 16;

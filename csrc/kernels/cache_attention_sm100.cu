@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       for (int i = 0; i < 2; ++i) {
         const bool there = pos0 + (pw * 2 + i) * 16 < w.s.len;
         rows[i] = there ? row_of(a, next[i], w.h) : -1;
-        if (there && rows[i] < 0 && lane == 0) report_bad_index();
+        if (there && rows[i] < 0 && lane == 0 && !vacant_place(a.table + (long)w.b * a.table_ld, next[i].page)) report_bad_index();
       }
       if (HALVES) {
         const int pos = pos0 + pw * 32 + lane;

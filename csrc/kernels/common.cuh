@@ -101,6 +101,8 @@ __device__ __forceinline__ void report_bad_index() {
   int* w = d_check_word;
   if (w) atomicCAS(w, 0, TB_ERR_BAD_INDEX);
 }
+// A row of a page table whose first entry is -1 belongs to a place of the batch that has no sequence: a page -1 there (`p`) is no bad index.
+__device__ __forceinline__ bool vacant_place(const int* table_row, int p) { return p == -1 && table_row[0] == -1; }
 // Host: point this translation unit's check word at `word` (null switches the reports off).
 static inline cudaError_t set_check_word_this_tu(int* word) {
   return cudaMemcpyToSymbol(d_check_word, &word, sizeof(word));

@@ -38,7 +38,9 @@ struct KvArgs {
   FastDiv by_h, by_page;
 };
 
-// Address of a row in the pages, in rows; -1 where the position is outside the table or the table names no page of the pool.
+// Address of a row in the pages, in rows; -1 where the position is outside the table or the table names no page of the pool, KV_VACANT
+// where that is because the place has no sequence.
+constexpr long KV_VACANT = -3;
 __device__ __forceinline__ long kv_row(const KvArgs& a, int b, int t, int h) {
   const int first = a.start ? a.start[b] : 0;
   if (first < 0) return -1;
@@ -47,7 +49,7 @@ __device__ __forceinline__ long kv_row(const KvArgs& a, int b, int t, int h) {
   const unsigned slot = a.by_page.div(pos);
   if (slot >= (unsigned)a.pages_per_seq) return -1;
   const int p = a.table[b * a.table_ld + slot];
-  if ((unsigned)p >= (unsigned)a.num_pages) return -1;
+  if ((unsigned)p >= (unsigned)a.num_pages) return vacant_place(a.table + b * a.table_ld, p) ? KV_VACANT : -1;
   return (long)p * a.page_rows + (int)(h * a.page + (pos - slot * (unsigned)a.page));
 }
 
@@ -127,7 +129,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvArgs a) {
 #pragma unroll
       for (int z = 0; z < 2; ++z) x[i][z].load(base[z] + (long)t * a.st[z] + (long)h * a.sh[z]);
       row[i] = kv_row(a, b, t, h);
-      if (row[i] < 0 && lane == 0) report_bad_index();
+      if (row[i] == -1 && lane == 0) report_bad_index();
     } else {
 #pragma unroll
       for (int z = 0; z < 2; ++z) x[i][z].clear();

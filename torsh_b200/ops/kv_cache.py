@@ -135,7 +135,8 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
 
     ``k`` and ``v`` are ``[B, T, H, D]``; token ``t`` of sequence ``b`` goes to position ``start[b] + t``, tokens from ``counts[b]`` on are
     left out, and so are sequences whose ``start`` is negative. Positions that the table does not reach, or to which it gives a page
-    outside the pool, are skipped (and reported where the device-side index checks are on). Two sequences may share pages, but not the positions that one call writes.
+    outside the pool, are skipped (and reported where the device-side index checks are on, but for pages -1 of a sequence whose first page is -1: a
+    place of the batch without a sequence). Two sequences may share pages, but not the positions that one call writes.
     No derivatives, of either mode: such inputs are refused.
     """
     if k.is_cuda and (nv._decode or nv.decode_calls()).kv_write(k, v, k_pages, v_pages, page_table, start, counts, k_scales, v_scales):
