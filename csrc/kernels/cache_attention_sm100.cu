@@ -378,14 +378,15 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[kst]);
-        // a scale that is no number, of a new token, is for the rows that see it (ct_odd_values)
-        const bool wild = (__float_as_uint(vs) & 0x7f800000u) == 0x7f800000u && pw * 32 + lane >= first_new;
+        // a scale that is no finite number leaves none among its token's values: a new token's are for the rows that see it (ct_odd_values),
+        // a context's become NaN here. Neither counts for the unit, which an infinity would take out of range for all
+        const bool odd_scale = (__float_as_uint(vs) & 0x7f800000u) == 0x7f800000u, wild = odd_scale && pw * 32 + lane >= first_new;
         if (wild) odd = 1u << lane;
-        const float big = warp_max(wild ? 0.f : fabsf(vs));
+        const float big = warp_max(odd_scale ? 0.f : fabsf(vs));
         const uint32_t bits = __float_as_uint(vs);
         const int unit = min(max((int)((__float_as_uint(big) + 0x7fffffu) >> 23) - 127, CT_UNIT), 127);
-        const int ex = (int)((bits >> 23) & 255u) - unit;             // of the scale relative to the unit, at most 127; a context's NaN stays one
-        const float rel = wild || ex < 127 - 25 ? 0.f : ex > 127 ? vs : __uint_as_float((bits & 0x807fffffu) | (uint32_t)ex << 23);
+        const int ex = (int)((bits >> 23) & 255u) - unit;             // of the scale relative to the unit, at most 127
+        const float rel = wild ? 0.f : odd_scale ? __int_as_float(0x7fffffff) : ex < 127 - 25 ? 0.f : __uint_as_float((bits & 0x807fffffu) | (uint32_t)ex << 23);
         mbar_wait(&v_empty[vst], ((n / VST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
         ((float*)side)[pw * 32 + lane] = ks;
         if (lane == 0) ((int*)(side + L::SCALES))[pw] = unit;

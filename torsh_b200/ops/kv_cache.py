@@ -261,7 +261,7 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     already, follow at positions ``start[b] ..``. A new token sees all of the context, and the new tokens ``j`` with
     ``tree_mask[t, j]`` (bool, ``[T, T]`` or ``[B, T, T]``; :func:`tree_mask_of`) - without a mask those up to itself. ``T = 1`` is an
     ordinary decoding step. Rows from ``counts[b]`` on, and rows that see nothing, come out as zeros; infinities and NaN in
-    places that a row does not see do not reach it. ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
+    places that a row does not see do not reach it (a value scale that is no finite number leaves none among its token's values). ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
     not read. Pages outside the pool read as zeros. No backward pass; forward-mode derivatives are computed in PyTorch.
 
     8-bit values are multiplied as halves relative to a largest scale, that of the positions so far or (many query rows) of their 32 positions:
