@@ -196,7 +196,6 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
     // Q as the second operand: lane (g, c) holds row g; 8-bit keys give lane c the D / 4 neighbouring columns from c D / 4 on
     uint32_t qf[NT][D / 16][2];
     float qs[NT][2];     // of rows 2c, 2c + 1, as the scores have them
-    float s0[NT][2];     // what their scores begin with: int8 keys go in as 1152 + code (one instruction less per two), which is taken off here
     int tt[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -204,7 +203,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
       const int t = r / a.G;
       const bool live = t < w.s.count;
       const bf16* qp = a.q + w.b * a.qb + (long)t * a.qt + (long)(h * a.G + r - t * a.G) * a.qh;
-      float mine = a.scale_log2, all = 0.f;
+      float mine = a.scale_log2;
       if (!HALVES) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -232,20 +231,11 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
           for (int z = 0; z < 2; ++z) {
             const uint32_t v = qf[n][kk][z];
             qf[n][kk][z] = pack2<true>(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down);
-            if (KIND == CA_INT8) {
-              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][kk][z]));
-              all += y.x + y.y;
-            }
           }
-        if (KIND == CA_INT8) {
-          all += __shfl_xor_sync(0xffffffffu, all, 1);
-          all += __shfl_xor_sync(0xffffffffu, all, 2);
-        }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         qs[n][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
-        s0[n][e] = KIND == CA_INT8 ? -1152.f * __shfl_sync(0xffffffffu, all, (2 * c + e) * 4) : 0.f;
         tt[n][e] = min(__shfl_sync(0xffffffffu, t, (2 * c + e) * 4), a.T);
       }
     }
@@ -274,7 +264,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = s0[n][e & 1];
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
       if (!HALVES) {
         const int tok = lane & 15;
         const uint32_t ka = ca_smem(kt) + tok * S::ROW;
@@ -295,8 +285,8 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4) {
             uint32_t kf[4];
-            halves_of<KIND, false>(w0[k4], kf[0], kf[2]);
-            halves_of<KIND, false>(w1[k4], kf[1], kf[3]);
+            halves_of<KIND>(w0[k4], kf[0], kf[2]);
+            halves_of<KIND>(w1[k4], kf[1], kf[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma16816<HALVES>(sc[n], kf, qf[n][q * 4 + k4][0], qf[n][q * 4 + k4][1]);
           }

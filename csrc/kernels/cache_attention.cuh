@@ -197,14 +197,12 @@ __device__ __forceinline__ bool sees(const CacheAttnArgs& a, int b, int t, int p
   return a.mask ? a.mask[b * a.mask_b + t * a.mask_t + j] != 0 : j <= t;
 }
 
-// Two 8-bit codes (the low 16 bits of v) as two halves. int8 without EXACT: 1152 more than the code.
-template <int KIND, bool EXACT = true>
+// Two 8-bit codes (the low 16 bits of v) as two halves.
+template <int KIND>
 __device__ __forceinline__ uint32_t half2_of(uint32_t v) {
   uint32_t r;
   if (KIND == CA_E4M3) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)v));
-  } else if (!EXACT) {
-    r = v;
   } else {   // v holds the codes + 128: 0x6400 + u is the half 1024 + u
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v), __half2half2(__ushort_as_half(0x6480)));
     r = *reinterpret_cast<const uint32_t*>(&h);
@@ -212,15 +210,15 @@ __device__ __forceinline__ uint32_t half2_of(uint32_t v) {
   return r;
 }
 // Four codes as halves: r0 = (code 0, code 1), r1 = (code 2, code 3).
-template <int KIND, bool EXACT = true>
+template <int KIND>
 __device__ __forceinline__ void halves_of(uint32_t w, uint32_t& r0, uint32_t& r1) {
   if (KIND == CA_E4M3) {
     r0 = half2_of<KIND>(w);
     r1 = half2_of<KIND>(w >> 16);
   } else {
     w ^= 0x80808080u;
-    r0 = half2_of<KIND, EXACT>(__byte_perm(w, 0x64646464u, 0x4140));
-    r1 = half2_of<KIND, EXACT>(__byte_perm(w, 0x64646464u, 0x4342));
+    r0 = half2_of<KIND>(__byte_perm(w, 0x64646464u, 0x4140));
+    r1 = half2_of<KIND>(__byte_perm(w, 0x64646464u, 0x4342));
   }
 }
 // Codes of two tokens (words of four columns each) as halves (token 0, token 1) of each column.
