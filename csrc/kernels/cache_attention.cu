@@ -10,9 +10,10 @@
 // clocks of the SM's share of HBM; their products take 32 clocks of the tensor pipe for 8 rows), and mma.sync takes its operands
 // from registers, which is where the 8-bit codes are decoded.
 //
-// 8-bit codes are multiplied as halves: int8 and e4m3 are exact there, q is brought into the half's range by a power of two per row,
-// P carries the value's scale (relative to a running power of two, the largest scale so far) and an offset of 2^8 against
-// underflow. P in halves has eight times the bits of bf16. Scores, maxima, sums and O are fp32.
+// 8-bit codes are multiplied as halves: int8 and e4m3 are exact there, q is brought into the half's range by a power of two per row, and
+// P carries the value's scale v: P = 2^(x + log2 v - M + 8), M the largest x + log2 v that the row sees, so that halves have room for
+// what counts in this row, whatever other scales there are (tokens that it does not see, or hardly attends to). The softmax's sum is
+// that of P / v. P in halves has eight times the bits of bf16. Scores, maxima, sums and O are fp32.
 //
 // The work of all sequences is dealt to the CTAs in equal runs of tiles (deal_tiles), so ragged batches and single long sequences
 // fill the GPU alike; a unit cut by the deal is joined by cache_attn_join_kernel. Short units are not cut (CA_WHOLE).
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
       }
     }
 
-    float o[MB][NT][4], mx[NT][2], sum[NT][2], unit_v = 0.f;   // unit_v: the power of two that O's values are relative to
+    float o[MB][NT][4], mx[NT][2], sum[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -294,36 +295,19 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
       }
 
       const bool edge = pos0 + CA_TILE > min(w.s.start, w.s.len);   // new tokens in it, or the end of the sequence
-      float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+      float ks[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f}, reach[2] = {0.f, 0.f}, inv[2] = {1.f, 1.f}, sign[2] = {1.f, 1.f};
       if (HALVES) {
         const float* scales = (const float*)(vt + S::TILE_BYTES);
         ks[0] = scales[g], ks[1] = scales[g + 8];
-        vs[0] = scales[CA_TILE + g], vs[1] = scales[CA_TILE + g + 8];
-        if (edge) {
-          if (pos0 + g >= w.s.len) vs[0] = 0.f;
-          if (pos0 + g + 8 >= w.s.len) vs[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float vs = scales[CA_TILE + g + 8 * i];
+          const bool none = no_scale(vs), odd = odd_scale(vs);
+          sign[i] = odd ? __int_as_float(0x7fffffff) : none ? 0.f : vs < 0.f ? -1.f : 1.f;
+          lv[i] = none || odd ? 0.f : log2f(fabsf(vs));
+          reach[i] = none ? CA_NONE : lv[i];
+          inv[i] = exp2f(-lv[i] - CA_DOWN);
         }
-        // an infinite scale makes its own values no numbers, as a NaN does, and nothing else's unit: rows that do not see them have P = 0
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if ((__float_as_uint(vs[i]) & 0x7f800000u) == 0x7f800000u) vs[i] = __int_as_float(0x7fffffff);
-        float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));   // a NaN counts for nothing
-        if (__any_sync(0xffffffffu, top > unit_v)) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          const float up = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
-          const float f = unit_v / up;
-#pragma unroll
-          for (int j = 0; j < MB; ++j)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[j][n][e] *= f;
-          unit_v = up;
-        }
-        const float inv = unit_v > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(unit_v)) : 0.f;
-        vs[0] *= inv;
-        vs[1] *= inv;
       }
 
       // the maximum that P is relative to moves only when a score is 2^6 above it: P stays below 2^6 (2^14 with the halves' offset)
@@ -335,7 +319,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
           float x = sc[n][e] * qs[n][e & 1];
           if (HALVES) x *= ks[e >> 1];
           if (edge && !(tt[n][e & 1] < a.T && sees(a, w.b, tt[n][e & 1], pos0 + g + (e >> 1) * 8, w.s))) x = -INFINITY;
-          over |= x > mx[n][e & 1] + 6.f;
+          over |= x + reach[e >> 1] > mx[n][e & 1] + 6.f;
           sc[n][e] = x;
         }
       if (__any_sync(0xffffffffu, over)) {
@@ -343,7 +327,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float top = fmaxf(sc[n][r], sc[n][2 + r]);
+            float top = fmaxf(sc[n][r] + reach[0], sc[n][2 + r] + reach[1]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             const float now = fmaxf(mx[n][r], top);
@@ -360,9 +344,11 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
         const float ref[2] = {(mx[n][0] == -INFINITY ? 0.f : mx[n][0]) - OFFSET, (mx[n][1] == -INFINITY ? 0.f : mx[n][1]) - OFFSET};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float p = exp2f(sc[n][e] - ref[e & 1]);
-          sum[n][e & 1] += p;
-          if (HALVES) p = sc[n][e] == -INFINITY ? 0.f : p * vs[e >> 1];
+          float x = sc[n][e] - ref[e & 1];
+          if (HALVES) x += lv[e >> 1];
+          float p = exp2f(x);
+          sum[n][e & 1] += HALVES ? p * inv[e >> 1] : p;
+          if (HALVES) p = sc[n][e] == -INFINITY ? 0.f : p * sign[e >> 1];
           sc[n][e] = p;
         }
         pf[n][0] = transpose8(pack2<HALVES>(sc[n][0], sc[n][1]));
@@ -482,7 +468,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
           const float2 y = *(const float2*)(ml + (v * S::ROWS + row) * 2);
           all += y.y * exp2f(y.x - ref);
         }
-        const float f = exp2f(mx[n][r] - ref) * (HALVES ? unit_v : 1.f);
+        const float f = exp2f(mx[n][r] - ref) * (HALVES ? exp2f(-CA_DOWN) : 1.f);
 #pragma unroll
         for (int j = 0; j < MB; ++j) o[j][n][r] *= f, o[j][n][2 + r] *= f;
         norm[n][r] = all > 0.f || all != all ? 1.f / all : 0.f;   // a row that sees nothing: zeros

@@ -9,8 +9,9 @@
 // Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 120 us, 4.6 TB/s. A tile
 // takes 2900 clocks, what the memory takes; the rest is the start (12 000 clocks until the first S: launch, deal, page table, first
 // copies) and the end of a unit (11 000 from the last P to the next unit's first S, in which the ring fills and then waits). 12 trees of 27
-// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 78 us (75 with the values' scales rounded to halves). A tile takes 4300 clocks: 10 000 warp instructions (decoding,
-// scales, exponentials) at 40 % of the issue slots, no pipe above 29 %, warps waiting for loads and for one another. Measured and not kept:
+// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 87 us; 78 while values went into the halves times their scales relative to the largest
+// of 32 tokens, which lost what a row sees beside a larger scale that it does not see. The softmax reads three numbers of each token (key's scale, log2 v,
+// 1 / v) out of shared memory, 16 bytes for each lane at a time, where it read one. Measured and not kept:
 // seven decoding warps (81 us for 75), keys' scales in the halves (82, and a rounding more), Q a unit ahead in a second place (122 for 121, 86
 // for 75).
 //
@@ -25,10 +26,11 @@
 //   warp 12    issues the products (warps 13-15: none; 512 threads take no more of the SM than 416, for 128 registers each)
 // TMEM: S and P of even and of odd tiles 128 columns each (P takes the first half of the S it came from), then O of either.
 //
-// 8-bit scales: scores are multiplied by the key's scale in fp32. The value's goes into the halves, relative to a power of two for each
-// 32 tokens (what a loading warp has of a tile), as the sum of two halves: one rounding (2^-11 at most) for the product, as P has one, where
-// carrying it in P cost the softmax 32 more loads of broadcast scales a tile (3.5 us instead of 2). P of those tokens is shifted by the
-// quotient of their power of two and the largest so far (`unit`), which O is relative to.
+// 8-bit scales: scores are multiplied by the key's scale in fp32, and P carries the value's, v: P = 2^(x + log2 v - M + 14), M the largest
+// x + log2 v that the row sees, so that halves have room for what counts in this row, whatever other scales there are (tokens that it does
+// not see, or hardly attends to). The softmax's sum is that of P / v. The first pass over a tile's scores takes log2 v in, the second takes
+// 1 / v, which the group works out in the place of the keys' scales in between (two barriers; shared memory has no room for both). Values
+// are multiplied as the codes that they are; signs of scales, and zeros, go into their halves.
 #include "cache_attention.cuh"
 #include "sm100.cuh"
 
@@ -41,7 +43,6 @@ constexpr int CT_TILE = 128;
 // Units stay whole while the longest has so many tiles more than a CTA's share. Measured (us, whole / cut): 2 trees of 27 in int8, 8 heads of
 // the cache, 200 tokens (one tile more) 16.6 / 19.9, 400 (three) 21.2 / 20.1; 16 tokens of one sequence, bf16, 300 tokens (two) 16.5 / 14.2.
 constexpr int CT_WHOLE = 1;
-constexpr int CT_UNIT = -80;   // log2 of the smallest power of two that values are relative to: sums times its inverse stay in range
 
 template <int D, int KIND> struct CtShape {
   static constexpr bool HALVES = KIND != CA_BF16;
@@ -52,10 +53,10 @@ template <int D, int KIND> struct CtShape {
   static constexpr int RAW = HALVES ? 2 * CT_TILE * D : 0;
   static constexpr int RAWS = HALVES ? 2 : 0;
   static constexpr int Q_OFF = 0, K_OFF = TILE, V_OFF = K_OFF + KST * TILE, RAW_OFF = V_OFF + VST * TILE;
-  // per value stage: scales of keys, the four loading warps' powers of two, and their tokens with odd values
-  static constexpr int SIDE_OFF = RAW_OFF + RAWS * RAW, SCALES = HALVES ? CT_TILE * 4 : 0, SIDE = SCALES + 32;
-  static constexpr int TOP_OFF = SIDE_OFF + VST * SIDE;             // largest |q| of either half of a row
-  static constexpr int BAR_OFF = TOP_OFF + (HALVES ? 2 * CT_TILE * 4 : 0);
+  // per value stage: scales of keys, logarithms of those of values, and the four loading warps' tokens with odd values
+  static constexpr int SIDE_OFF = RAW_OFF + RAWS * RAW, SCALES = HALVES ? 2 * CT_TILE * 4 : 0, SIDE = SCALES + 16;
+  static constexpr int TOP_OFF = SIDE_OFF + VST * SIDE;             // exponent of the largest |q| of either half of a row
+  static constexpr int BAR_OFF = TOP_OFF + (HALVES ? 2 * CT_TILE : 0);
   // k_full[2], k_empty[2], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done[2], side_full[2], q_full
   static constexpr int NBARS = 21;
   static constexpr int ALLOC = BAR_OFF + NBARS * 8 + 8;
@@ -92,7 +93,7 @@ __device__ __forceinline__ void ct_odd_values(const CacheAttnArgs& a, uint32_t t
       const int pos = pos0 + w * 32 + __ffs(rest) - 1;
       const long row = row_of(a, page_ref(a, b, pos), h);
       const bool mine = live && row >= 0 && sees(a, b, t, pos, s);
-      const bool wild = KIND != CA_BF16 && row >= 0 && (__float_as_uint(__ldg(a.v_scales + row + (pos & 15))) & 0x7f800000u) == 0x7f800000u;
+      const bool wild = KIND != CA_BF16 && row >= 0 && odd_scale(__ldg(a.v_scales + row + (pos & 15)));
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
@@ -257,9 +258,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
     const int pw = warp - 8;
     const uint32_t smem_base = smem_u32(smem);
     constexpr int N = L::PIECE / 512;             // 16-byte copies of a lane for a piece of keys or values
-    // of the tile last asked for: the scales of token 32 pw + lane, and the first token that is a new one (CT_TILE: none)
+    // of the tile last asked for: the scales of token 32 pw + lane, the first token that is a new one (CT_TILE: none), its position and its sequence's end
     float ks = 0.f, vs = 0.f;
-    int first_new = CT_TILE;
+    int first_new = CT_TILE, tile_pos = 0, seq_end = 0;
     PageRef next[2];
     auto seek = [&]() {
 #pragma unroll
@@ -299,6 +300,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
     auto ask = [&](int n) {
       const int pos0 = w.tile * CT_TILE;
       first_new = pos0 + CT_TILE > min(w.s.start, w.s.len) ? max(w.s.start - pos0, 0) : CT_TILE;
+      tile_pos = pos0, seq_end = w.s.len;
       long rows[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -323,11 +325,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       if (++w.tile >= w.end) walk_next<CT_TILE>(a, w, 0);
       if (n + 1 < total) seek();
     };
-    // halves of the warp's codes of a tile, keys as they are, values times their token's `scale` (lane: token 32 pw + lane)
-    auto convert = [&](auto is_value, const uint8_t* raw, uint8_t* dst, float scale, int first_new, uint32_t& odd) {
+    // halves of the warp's codes of a tile. Values of tokens in `none` become zeros, those of tokens in `minus` change their sign
+    auto convert = [&](auto is_value, const uint8_t* raw, uint8_t* dst, uint32_t none, uint32_t minus, int first_new, uint32_t& odd) {
       constexpr bool VALUE = decltype(is_value)::value;
-      const __half s_hi = __float2half_rn(scale), s_lo = __float2half_rn(scale - __half2float(s_hi));
-      const uint32_t scale_halves = (uint32_t)__half_as_ushort(s_hi) | (uint32_t)__half_as_ushort(s_lo) << 16;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -351,21 +351,17 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
           halves_of<KIND>(v.y, lo.z, lo.w);
           halves_of<KIND>(v.z, hi.x, hi.y);
           halves_of<KIND>(v.w, hi.z, hi.w);
-          if (VALUE) {
-            const uint32_t both = __shfl_sync(0xffffffffu, scale_halves, tok & 31), sh = __byte_perm(both, 0u, 0x1010), sl = __byte_perm(both, 0u, 0x3232);
-            const __half2 hi2 = *reinterpret_cast<const __half2*>(&sh), lo2 = *reinterpret_cast<const __half2*>(&sl);
-            auto times = [&](uint32_t& h) {   // the smaller product first: one rounding
-              const __half2 x = *reinterpret_cast<const __half2*>(&h), y = __hfma2(x, hi2, __hmul2(x, lo2));
-              h = *reinterpret_cast<const uint32_t*>(&y);
-            };
-            times(lo.x), times(lo.y), times(lo.z), times(lo.w), times(hi.x), times(hi.y), times(hi.z), times(hi.w);
+          if (VALUE && (none | minus)) {
+            const uint32_t keep = (none >> (tok & 31)) & 1u ? 0u : 0xffffffffu, turn = (minus >> (tok & 31)) & 1u ? 0x80008000u : 0u;
+            lo.x = (lo.x & keep) ^ turn, lo.y = (lo.y & keep) ^ turn, lo.z = (lo.z & keep) ^ turn, lo.w = (lo.w & keep) ^ turn;
+            hi.x = (hi.x & keep) ^ turn, hi.y = (hi.y & keep) ^ turn, hi.z = (hi.z & keep) ^ turn, hi.w = (hi.w & keep) ^ turn;
           }
           *(uint4*)(dst + ct_at(tok, 2 * q)) = lo;
           *(uint4*)(dst + ct_at(tok, 2 * q + 1)) = hi;
         }
     };
     // tile n, whose copies have arrived: its halves, its odd values; then it is the products'
-    auto hand_on = [&](int n, float ks, float vs, int first_new) {
+    auto hand_on = [&](int n, float ks, float vs, int first_new, int last_tile, int last_len) {
       const int kst = n % KST, vst = n % VST;
       uint8_t* vt = smem + L::V_OFF + vst * L::TILE;
       uint8_t* side = smem + L::SIDE_OFF + vst * L::SIDE;
@@ -374,25 +370,22 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       if (HALVES) {
         const uint8_t* raw = smem + L::RAW_OFF + (n & 1) * L::RAW;
         mbar_wait(&k_empty[kst], ((n / KST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
-        convert(std::false_type{}, raw, smem + L::K_OFF + kst * L::TILE, 0.f, 0, odd);
+        convert(std::false_type{}, raw, smem + L::K_OFF + kst * L::TILE, 0u, 0u, 0, odd);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[kst]);
         // a scale that is no finite number leaves none among its token's values: a new token's are for the rows that see it (ct_odd_values),
-        // a context's become NaN here. Neither counts for the unit, which an infinity would take out of range for all
-        const bool odd_scale = (__float_as_uint(vs) & 0x7f800000u) == 0x7f800000u, wild = odd_scale && pw * 32 + lane >= first_new;
+        // a context's are NaN by their logarithm. What lies behind the end is not seen
+        const bool there = last_tile + pw * 32 + lane < last_len, infinite = there && odd_scale(vs), wild = infinite && pw * 32 + lane >= first_new;
+        const uint32_t minus = __ballot_sync(0xffffffffu, vs < 0.f), none = __ballot_sync(0xffffffffu, wild || (there && no_scale(vs)));
         if (wild) odd = 1u << lane;
-        const float big = warp_max(odd_scale ? 0.f : fabsf(vs));
-        const uint32_t bits = __float_as_uint(vs);
-        const int unit = min(max((int)((__float_as_uint(big) + 0x7fffffu) >> 23) - 127, CT_UNIT), 127);
-        const int ex = (int)((bits >> 23) & 255u) - unit;             // of the scale relative to the unit, at most 127
-        const float rel = wild ? 0.f : odd_scale ? __int_as_float(0x7fffffff) : ex < 127 - 25 ? 0.f : __uint_as_float((bits & 0x807fffffu) | (uint32_t)ex << 23);
+        const float lv = !there ? 0.f : (none >> lane) & 1u ? CA_NONE : infinite ? __int_as_float(0x7fffffff) : log2f(fabsf(vs));
         mbar_wait(&v_empty[vst], ((n / VST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
         ((float*)side)[pw * 32 + lane] = ks;
-        if (lane == 0) ((int*)(side + L::SCALES))[pw] = unit;
+        ((float*)side)[CT_TILE + pw * 32 + lane] = lv;
         __syncwarp();
         if (lane == 0) mbar_arrive(&side_full[vst]);                  // the softmax does not wait for the values
-        convert(std::true_type{}, raw + CT_TILE * D, vt, rel, first_new, odd);
+        convert(std::true_type{}, raw + CT_TILE * D, vt, none, minus, first_new, odd);
       } else {
         if (edge) {
 #pragma unroll 1
@@ -415,7 +408,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
       }
       if (edge) odd = __reduce_or_sync(0xffffffffu, odd);
-      if (lane == 0) ((uint32_t*)(side + L::SCALES + 16))[pw] = odd;
+      if (lane == 0) ((uint32_t*)(side + L::SCALES))[pw] = odd;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -427,7 +420,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
     // Tile n is asked for before tile n - 1 is handed on; what that waits for are tiles n - 2 and older.
     for (int n = 0; n <= total; ++n) {
       const float last_ks = ks, last_vs = vs;
-      const int last_new = first_new;
+      const int last_new = first_new, last_pos = tile_pos, last_end = seq_end;
       if (n < total) {
         ask(n);
       } else {
@@ -436,7 +429,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       }
       if (n >= 1) {
         ct_wait<2>();
-        hand_on(n - 1, last_ks, last_vs, last_new);
+        hand_on(n - 1, last_ks, last_vs, last_new, last_pos, last_end);
       }
     }
     ct_wait<0>();
@@ -464,11 +457,10 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
           for (int i = 0; i < D / 16; ++i)
             big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(bf16_lo(v[i].x)), fabsf(bf16_hi(v[i].x))), fmaxf(fabsf(bf16_lo(v[i].y)), fabsf(bf16_hi(v[i].y)))),
                                    fmaxf(fmaxf(fabsf(bf16_lo(v[i].z)), fabsf(bf16_hi(v[i].z))), fmaxf(fabsf(bf16_lo(v[i].w)), fabsf(bf16_hi(v[i].w))))));
-          float* tops = (float*)(smem + L::TOP_OFF);
-          tops[group * 128 + row] = big;
+          uint8_t* tops = smem + L::TOP_OFF;
+          tops[group * 128 + row] = (uint8_t)(__float_as_uint(big) >> 23);
           asm volatile("bar.sync 1, 256;" ::: "memory");
-          big = fmaxf(big, tops[(group ^ 1) * 128 + row]);
-          const uint32_t ex = __float_as_uint(big) >> 23;
+          const uint32_t ex = max(__float_as_uint(big) >> 23, (uint32_t)tops[(group ^ 1) * 128 + row]);
           const bool plain = ex == 0 || ex > 253;
           const float down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
           if (!plain) f *= __uint_as_float(ex << 23);
@@ -480,16 +472,15 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
             v[i].w = ct_pack<true>(bf16_lo(v[i].w) * down, bf16_hi(v[i].w) * down);
           }
         }
-        f = fmaxf(f, 1e-30f);   // -inf (not seen) times a factor of zero would be no number
+        if (!HALVES) f = fmaxf(f, 1e-30f);   // -inf (not seen) times a factor of zero would be no number
         if (!HALVES) asm volatile("bar.sync 1, 256;" ::: "memory");   // the last unit's output has left Q's place (8 bits: the barrier above)
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) *(uint4*)(smem + L::Q_OFF + ct_at(row, group * (D / 16) + i)) = v[i];
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // P = 2^(x f - m f + OFFSET + shift), x the score (times the key's scale), shift that of the value's 32 tokens; l sums it unshifted
+      // P = 2^(x f - m f), x the score; of 8-bit caches 2^(y - m + OFFSET), y = x f + log2 v
       float m = -INFINITY, l = 0.f;
-      int unit = HALVES ? CT_UNIT : 0;
       uint32_t odd[4] = {0u, 0u, 0u, 0u};
       int odd_pos = 0;
       bool any_tile = false;
@@ -502,10 +493,12 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         if (edge && live) ct_visible(a, w.b, t, pos0, w.s, vis_lo, vis_hi);
         if (HALVES) mbar_wait(&side_full[st], (n / VST) & 1, abort_flag, status, TB_ERR_WAIT_FULL);
         // S of this tile; O += P V of the tile before last has finished, or its place would not have been S's
+        const float inverse = HALVES ? exp2f(-((const float*)side)[CT_TILE + row] - CA_DOWN) : 0.f;
         mbar_wait(&s_full[group], (n >> 1) & 1, abort_flag, status, TB_ERR_WAIT_TMEM_FULL);
         tc_fence_after();
         float alpha = 1.f;
         bool grow = false;
+        const float2 f2 = make_float2(f, f);
         // Two passes over S, 64 columns at a time: the maximum, then P over the columns that have been read
         if (busy) {
           uint32_t v[2][32];
@@ -520,9 +513,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
               for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                  const float4 k4 = *(const float4*)(side + ((half * 2 + c) * 32 + i) * 4);
-                  const float2 x = __fmul2_rn(make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), make_float2(k4.x, k4.y));
-                  const float2 y = __fmul2_rn(make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), make_float2(k4.z, k4.w));
+                  const float4 k4 = *(const float4*)(side + ((half * 2 + c) * 32 + i) * 4), l4 = *(const float4*)(side + (CT_TILE + (half * 2 + c) * 32 + i) * 4);
+                  const float2 x = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), make_float2(k4.x, k4.y)), f2, make_float2(l4.x, l4.y));
+                  const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), make_float2(k4.z, k4.w)), f2, make_float2(l4.z, l4.w));
                   v[c][i] = __float_as_uint(x.x), v[c][i + 1] = __float_as_uint(x.y), v[c][i + 2] = __float_as_uint(y.x), v[c][i + 3] = __float_as_uint(y.y);
                 }
             }
@@ -550,28 +543,25 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
               }
           }
           now = fmaxf(now, also);
-          int now_unit = unit, units[4];
-          if (HALVES) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              units[c] = ((const int*)(side + L::SCALES))[c];
-              now_unit = max(now_unit, units[c]);
-            }
-            tmem_wait_st();
-          } else if (edge) {
-            tmem_wait_st();
-          }
-          grow = now > m || now_unit > unit;
+          if (HALVES || edge) tmem_wait_st();
+          grow = now > m;
           // O of no tile yet, or of tiles that the row saw nothing of, is zero (or not there): any finite factor does
           if (grow) {
-            const float less = m == -INFINITY ? 1.f : exp2f((m - now) * f);
-            alpha = HALVES ? less * exp2f((float)(unit - now_unit)) : less;
-            l *= less;
+            alpha = m == -INFINITY ? 1.f : exp2f(HALVES ? m - now : (m - now) * f);
+            l *= alpha;
           }
           m = now;
-          unit = now_unit;
-          const float ref = (m == -INFINITY ? 0.f : m * f) - OFFSET;
-          const float2 f2 = make_float2(f, f);
+        }
+        float* inv = (float*)side;
+        if (HALVES) {   // the keys' scales have been read by all: 1 / v in their place
+          asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
+          inv[row] = inverse;
+          asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
+        }
+        if (busy) {
+          uint32_t v[2][32];
+          const float ref = (m == -INFINITY ? 0.f : HALVES ? m : m * f) - OFFSET;
+          const float2 r2 = make_float2(-ref, -ref);
 #pragma unroll 1
           for (int half = 0; half < 2; ++half) {
             tmem_ld32(ts + half * 64, v[0]);
@@ -579,23 +569,27 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const float shift = HALVES ? (float)max((half ? units[2 + c] : units[c]) - unit, -100) : 0.f;
-              const float2 r2 = make_float2(shift - ref, shift - ref);
               float2 l2 = make_float2(0.f, 0.f), l3 = l2;
               uint32_t pk[16];
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
-                const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), f2, r2);
-                const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), f2, r2);
+                const float2 s01 = make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), s23 = make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3]));
+                const float2 x = HALVES ? __fadd2_rn(s01, r2) : __ffma2_rn(s01, f2, r2);
+                const float2 y = HALVES ? __fadd2_rn(s23, r2) : __ffma2_rn(s23, f2, r2);
                 const float2 e = make_float2(exp2f(x.x), exp2f(x.y)), g = make_float2(exp2f(y.x), exp2f(y.y));
-                l2 = __fadd2_rn(l2, e);
-                l3 = __fadd2_rn(l3, g);
+                if (HALVES) {
+                  const float4 i4 = *(const float4*)(inv + (half * 2 + c) * 32 + i);
+                  l2 = __ffma2_rn(e, make_float2(i4.x, i4.y), l2);
+                  l3 = __ffma2_rn(g, make_float2(i4.z, i4.w), l3);
+                } else {
+                  l2 = __fadd2_rn(l2, e);
+                  l3 = __fadd2_rn(l3, g);
+                }
                 pk[i / 2] = ct_pack<HALVES>(e.x, e.y);
                 pk[i / 2 + 1] = ct_pack<HALVES>(g.x, g.y);
               }
               tmem_st16(tp + (half * 2 + c) * 16, pk);
-              const float sum = (l2.x + l2.y) + (l3.x + l3.y);
-              l += HALVES ? sum * exp2f(-shift) : sum;
+              l += (l2.x + l2.y) + (l3.x + l3.y);
             }
           }
           if (odd[0] | odd[1] | odd[2] | odd[3]) ct_odd_values<D, KIND>(a, to, odd, w.b, w.h, min(t, a.T - 1), live, odd_pos, w.s);
@@ -617,7 +611,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
         if (edge) mbar_wait(&v_full[st], (n / VST) & 1, abort_flag, status, TB_ERR_WAIT_FULL);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) odd[i] = edge ? ((const uint32_t*)(side + L::SCALES + 16))[i] : 0u;
+        for (int i = 0; i < 4; ++i) odd[i] = edge ? ((const uint32_t*)(side + L::SCALES))[i] : 0u;
         odd_pos = pos0;
         any_tile = true;
         tmem_wait_st();
@@ -633,8 +627,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
           ct_odd_values<D, KIND>(a, to, odd, w.b, w.h, min(t, a.T - 1), live, odd_pos, w.s);
         }
       }
-      const float mine_r = m == -INFINITY ? m : m * f + (float)unit;
-      if (HALVES) l *= exp2f(-(float)unit);             // relative to the same power of two as O
+      const float mine_r = HALVES || m == -INFINITY ? m : m * f;
       // all products of the unit have read Q when both groups are here
       tc_fence_before();
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -646,7 +639,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       const float f_mine = exp2f(mine_r - ref), f_other = exp2f(other.x - ref);
       const float all = l * f_mine + other.y * f_other;
       // a group that has had no tile, or whose tiles the row saw nothing of, has nothing in its O
-      const float f0 = group ? f_other : f_mine, f1 = group ? f_mine : f_other;
+      constexpr float DOWN = HALVES ? 1.f / (float)(1 << (int)CA_DOWN) : 1.f;
+      const float f0 = (group ? f_other : f_mine) * DOWN, f1 = (group ? f_mine : f_other) * DOWN;
       const bool has0 = (group ? other.y : l) != 0.f, has1 = (group ? l : other.y) != 0.f;
       asm volatile("bar.sync 1, 256;" ::: "memory");   // read, before the next Q overwrites it
       const bool whole = w.head == 0 && w.end == w.nt;

@@ -264,8 +264,9 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     places that a row does not see do not reach it (a value scale that is no finite number leaves none among its token's values). ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
     not read. Pages outside the pool read as zeros. No backward pass; forward-mode derivatives are computed in PyTorch.
 
-    8-bit values are multiplied as halves relative to a largest scale, that of the positions so far or (many query rows) of their 32 positions:
-    values with scales below 2^-14 of it lose precision and below 2^-25 count as zero, whether or not the row sees that largest one.
+    Probabilities are rounded to bf16 over bf16 pages. Over 8-bit pages they are rounded to halves, times the scale of their value and relative to
+    the largest such product that the row sees: a scale that a row does not see, or hardly attends to, takes nothing from the others. Scales of
+    ``v_scales`` from 2^122 on count as infinite, those below 2^-96 as zero.
     """
     if q.is_cuda:
         out = (nv._decode or nv.decode_calls()).kv_attention(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, max_len,
