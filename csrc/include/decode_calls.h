@@ -1,7 +1,12 @@
 // Arguments of the decoding operators' launchers (csrc/kernels/rotary.cu, kv_cache.cu, cache_attention.cu, verify_draft.cu) as records of
-// 8-byte fields: the Python wrappers pack them with struct, csrc/torch/decode_calls.cpp fills them in.
+// 8-byte fields, filled in by csrc/torch/decode_calls.cpp. Launchers and that module are built apart from one another: the build gives both
+// a number for this file's text, and the module refuses a library that has another one.
 #pragma once
 #include <stdint.h>
+
+#ifndef TB_DECODE_LAYOUT   // torsh_b200/_build.py gives it; a file that is compiled by hand has none to compare
+#define TB_DECODE_LAYOUT 0
+#endif
 
 struct RotaryCall {
   const void *q, *k;

@@ -208,6 +208,9 @@ static int rotary_launch(RotaryArgs& a, bool half, bool vec, cudaStream_t st) {
 }  // namespace tb
 using namespace tb;
 
+// Which text of decode_calls.h the launchers of this library have been built with.
+TB_EXPORT uint64_t tb_decode_layout() { return TB_DECODE_LAYOUT; }
+
 // q [tokens, hq, D], k [tokens, hk, D] (hk = 0: none) with strides in elements, columns contiguous; yq, yk contiguous.
 TB_EXPORT int tb_rotary(const RotaryCall* c, cudaStream_t st) {
   TB_ENSURE_DEVICE();

@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
+#include <torch/version.h>
 
 #include "decode_calls.h"
 
@@ -381,18 +382,21 @@ PyObject* py_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // bind(module torsh_b200._native, addresses of: tb_set_device, tb_last_error, tb_rotary, tb_kv_write, tb_kv_read, tb_cache_attention,
-//      tb_cache_attention_workspace, tb_verify_draft)
+//      tb_cache_attention_workspace, tb_verify_draft, tb_decode_layout)
 PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 9 || !PyModule_Check(args[0])) {
-    PyErr_SetString(PyExc_TypeError, "bind: a module and eight addresses");
+  constexpr int ADDRESSES = 9;
+  if (n != 1 + ADDRESSES || !PyModule_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "bind: a module and nine addresses");
     return nullptr;
   }
-  void* at[8];
-  for (int i = 0; i < 8; ++i)
+  void* at[ADDRESSES];
+  for (int i = 0; i < ADDRESSES; ++i)
     if (!(at[i] = PyLong_AsVoidPtr(args[i + 1]))) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "bind: null address");
   PyObject* dict = PyModule_GetDict(args[0]);
   PyObject* error = PyDict_GetItemString(dict, "NativeError");
   if (!error) return PyErr_Format(PyExc_ValueError, "bind: no NativeError");
+  if (((uint64_t (*)())at[8])() != TB_DECODE_LAYOUT)
+    return PyErr_Format(error, "_decode_calls.so and libtorsh_b200_cuda.so have been built with different records: run `python -m torsh_b200._build`");
   key_bound = PyUnicode_InternFromString("_bound_device");
   key_count = PyUnicode_InternFromString("launch_count");
   native_error = Py_NewRef(error);
@@ -420,4 +424,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decode_calls", "Calls of the deco
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__decode_calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__decode_calls() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -62,6 +62,12 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(r.stdout + r.stderr, flush=True)
 
 
+def _decode_layout() -> str:
+    """The number of ``decode_calls.h`` that its launchers and the extension module compare."""
+    import hashlib
+    return "-DTB_DECODE_LAYOUT=0x" + hashlib.sha256((CSRC / "include" / "decode_calls.h").read_bytes()).hexdigest()[:15]
+
+
 def build_cuda(verbose: bool = False, ptxas_info: bool = False) -> Path:
     nvcc = _nvcc()
     srcs = sorted((CSRC / "kernels").glob("*.cu"))
@@ -74,7 +80,7 @@ def build_cuda(verbose: bool = False, ptxas_info: bool = False) -> Path:
         o = OBJDIR / (s.stem + ".cu.o")
         objs.append(o)
         if _newer(s, o, hdrs):
-            cmd = [nvcc, *NVCC_FLAGS, "-I", str(CSRC / "include"), "-I", str(CSRC / "kernels"), "-c", str(s), "-o", str(o)]
+            cmd = [nvcc, *NVCC_FLAGS, _decode_layout(), "-I", str(CSRC / "include"), "-I", str(CSRC / "kernels"), "-c", str(s), "-o", str(o)]
             if ptxas_info:
                 cmd[1:1] = ["-Xptxas", "-v"]
             jobs.append(cmd)
@@ -110,16 +116,19 @@ def build_torch(verbose: bool = False) -> Path:
     import sysconfig
 
     import torch
-    src, out = CSRC / "torch" / "decode_calls.cpp", LIBDIR / "_decode_calls.so"
+    src, out, stamp = CSRC / "torch" / "decode_calls.cpp", LIBDIR / "_decode_calls.so", OBJDIR / "decode_calls.txt"
+    OBJDIR.mkdir(parents=True, exist_ok=True)
     LIBDIR.mkdir(parents=True, exist_ok=True)
-    if _newer(src, out, [CSRC / "include" / "decode_calls.h"]):
+    made_for = f"{torch.__version__} {sys.version} {_decode_layout()}"       # an extension module is no good for another of these
+    if _newer(src, out, [CSRC / "include" / "decode_calls.h"]) or not stamp.exists() or stamp.read_text() != made_for:
         base = Path(torch.__file__).resolve().parent
         cuda = Path(_nvcc()).resolve().parent.parent / "include"
         inc = [CSRC / "include", base / "include", base / "include" / "torch" / "csrc" / "api" / "include", cuda, sysconfig.get_paths()["include"]]
         cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
-        _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", _decode_layout(), f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
               *(f"-isystem{p}" if i else f"-I{p}" for i, p in enumerate(inc)), str(src), "-o", str(out), f"-L{base / 'lib'}", "-lc10", "-lc10_cuda",
               "-ltorch_cpu", "-ltorch", "-ltorch_python"], verbose)
+        stamp.write_text(made_for)
     return out
 
 

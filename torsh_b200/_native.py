@@ -90,9 +90,11 @@ def decode_calls():
                 spec = importlib.util.spec_from_file_location("torsh_b200._decode_calls", path)
                 mod = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(mod)
+                if mod.torch_version != torch.__version__.split("+")[0]:
+                    raise NativeError(f"{path} has been built with PyTorch {mod.torch_version}, not {torch.__version__}: run `python -m torsh_b200._build`")
                 mod.bind(sys.modules[__name__], *(c_void_p.from_address(ctypes.addressof(getattr(lib, f))).value for f in (
                     "tb_set_device", "tb_last_error", "tb_rotary", "tb_kv_write", "tb_kv_read", "tb_cache_attention",
-                    "tb_cache_attention_workspace", "tb_verify_draft")))
+                    "tb_cache_attention_workspace", "tb_verify_draft", "tb_decode_layout")))
                 _decode = mod
     return _decode
 
