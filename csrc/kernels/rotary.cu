@@ -21,8 +21,7 @@ namespace tb {
 constexpr int ROT_THREADS = 256;
 constexpr int ROT_MAX_PAIRS = 256;   // R <= 512
 constexpr int ROT_MAX_TOKENS = 8;    // tokens of a block
-constexpr int ROT_ANGLES = 1024;     // pairs of a block, over its tokens
-constexpr int ROT_TABLE = ROT_ANGLES + 8 * ROT_MAX_TOKENS;
+constexpr int ROT_ANGLES = 1024;     // pairs of a block, over its tokens: the places of its table
 
 struct RotaryArgs {
   const void* x[2];      // q, k: [tokens, heads, D] with strides
@@ -62,7 +61,7 @@ template <typename T, bool HALF>
 __global__ void __launch_bounds__(ROT_THREADS, HALF ? 5 : 4) rotary_vec_kernel(const RotaryArgs a) {
   constexpr int N = Vec16<T>::N;
   constexpr int U = HALF ? 2 : 4;      // rows in flight
-  __shared__ float2 tab[ROT_TABLE];
+  __shared__ float2 tab[ROT_ANGLES];
   constexpr int K = HALF ? N : N / 2;
   const int half = a.R >> 1, D = a.D;
   const RotTable place{K, half / K};
@@ -142,7 +141,7 @@ __global__ void __launch_bounds__(ROT_THREADS, HALF ? 5 : 4) rotary_vec_kernel(c
 // Head sizes, pairings and addresses that 16-byte vectors do not fit: one pair (or one column that passes through) at a time.
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_scalar_kernel(const RotaryArgs a) {
-  __shared__ float2 tab[ROT_TABLE];
+  __shared__ float2 tab[ROT_ANGLES];
   const int half = a.R >> 1, D = a.D;
   const long t0 = (long)blockIdx.x * a.per_block;
   const int nt = (int)min((long)a.per_block, a.tokens - t0);
