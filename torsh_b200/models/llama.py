@@ -211,7 +211,8 @@ class LlamaModel(nn.Module):
         logits = lin_ops.linear(h, self.lm_head, None)[:, : self.cfg.vocab_size].float()
         if temperature == 0:
             return torch.zeros_like(logits).scatter_(1, logits.argmax(-1, keepdim=True), 1.0)
-        return torch.softmax(logits / temperature, -1)
+        # the largest first: a small temperature takes the others out of range, and infinity less infinity is no number
+        return torch.softmax((logits - logits.amax(-1, keepdim=True)) / max(temperature, torch.finfo(torch.float32).tiny), -1)
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 0.0, draft: "LlamaModel | None" = None, drafted: int = 4,
@@ -220,8 +221,9 @@ class LlamaModel(nn.Module):
 
         With ``draft`` (a smaller model over the same vocabulary) each round drafts ``drafted`` tokens and verifies them in one pass of this
         model (:func:`~torsh_b200.ops.speculative.verify_draft`): the tokens are distributed as without it, and the same at temperature 0
-        up to the rounding of sums over different numbers of rows."""
-        if temperature < 0:
+        up to the rounding of sums over different numbers of rows. Raises where this model's probabilities are no numbers; a draft's that are none
+        are never accepted."""
+        if not temperature >= 0:
             raise ValueError("generate: temperature is not negative")
         if draft is not None and (draft.cfg.vocab_size != self.cfg.vocab_size or drafted < 1):
             raise ValueError("generate: the draft model has the same vocabulary, and drafts at least one token")
@@ -249,14 +251,16 @@ class LlamaModel(nn.Module):
                 for _ in range(drafted):            # one token more than is drafted: its keys are needed where all are accepted
                     p = draft._probs(draft.decode(tokens[:, -1:], c), temperature)
                     c.advance(1)
-                    nxt = spec_ops.verify_draft(p[:, None], tokens[:, -1:], rand(B, 1))[2]
+                    nxt = spec_ops.verify_draft(p[:, None], tokens[:, -1:], rand(B, 1))[2].clamp(min=0)   # none: a token that is refused below
                     tokens, q = torch.cat([tokens, nxt[:, None]], 1), q + [p]
                 draft.decode(tokens[:, -1:], c)
                 c.advance(1)
             caches[0].reserve(T)
             probs = self._probs(self.decode(tokens, caches[0]), temperature).view(B, T, -1)
             taken, _, nxt = spec_ops.verify_draft(probs, tokens, rand(B, T), torch.stack(q, 1) if q else None)
-            took = taken.tolist()
+            took, follow = taken.tolist(), nxt.tolist()
+            if min(follow) < 0:
+                raise RuntimeError("generate: the model's probabilities are no numbers")
             caches[0].advance([n + 1 for n in took])
             for b, (n, more) in enumerate(zip(took, torch.cat([tokens[:, 1:], nxt[:, None]], 1).tolist())):
                 done[b] += more[:n] + more[-1:]
