@@ -99,3 +99,14 @@ def test_upper_bounds_refuse_nothing_that_there_is_room_for():
         two.reserve([40, 0])
     two.reserve([0, 31])
     assert len(two._free) == 0 and two.lengths.tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("bad", [[1], [1, 1, 1], []])
+def test_tokens_of_other_batches_are_refused(bad):
+    """A list that is too short reserved for the places that it had, and said nothing of the others."""
+    c = _cache()
+    c.reserve([5, 5])
+    for call in (c.reserve, c.advance):
+        with pytest.raises(ValueError):
+            call(bad)
+    assert c.lengths.tolist() == [0, 0] == c.host_lengths and len(c._free) == 6

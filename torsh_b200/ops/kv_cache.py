@@ -321,7 +321,8 @@ def tree_mask_of(parents: torch.Tensor) -> torch.Tensor:
 class PagedKVCache:
     """Pages of one or more layers, the sequences that own them, and the calls on them.
 
-    ``dtype`` is ``torch.bfloat16``, ``torch.int8`` or ``torch.float8_e4m3fn``. Every layer has its own pages; the table and the lengths
+    ``dtype`` is ``torch.bfloat16``, ``torch.int8`` or ``torch.float8_e4m3fn``. Heads of 64 or 128 columns, and queries in bf16, take the kernels;
+    other heads and types run in PyTorch, which gathers a context in fp32 and waits for the device, so that such steps cannot be captured. Every layer has its own pages; the table and the lengths
     are common. A step is: :meth:`reserve` room for the new tokens of the batch, for each layer :meth:`write` their keys and values and
     :meth:`attend`, then :meth:`advance` the lengths by what is kept (after a verification fewer than were written: the rest is
     written over). Table and lengths are device tensors that are written in place, so a step with ``advance(tensor, most)`` can be captured
@@ -352,6 +353,12 @@ class PagedKVCache:
         self._owned: list[list[int]] = [[] for _ in range(batch)]
         self._free = list(range(num_pages - 1, -1, -1))
 
+    def _per_place(self, tokens) -> list[int]:
+        tokens = [tokens] * self.batch if isinstance(tokens, int) else [int(t) for t in tokens]
+        if len(tokens) != self.batch:
+            raise ValueError(f"PagedKVCache: tokens {tokens} for {self.batch} sequences")
+        return tokens
+
     def _capturing(self) -> bool:
         return self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
 
@@ -364,7 +371,7 @@ class PagedKVCache:
 
     def reserve(self, tokens) -> None:
         """Room for ``tokens`` (an int, or one per sequence) more tokens of every sequence. Raises where the pool or ``max_len`` has none."""
-        tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
+        tokens = self._per_place(tokens)
         for exact in (False, True):               # upper bounds first: what does not fit them is asked of the device
             self.host_lengths = self._bounds(exact)
             need = [max(0, -(-(n + t) // self.page) - len(own)) for n, t, own in zip(self.host_lengths, tokens, self._owned)]
@@ -430,7 +437,7 @@ class PagedKVCache:
                 self.host_lengths = [n + most for n in self.host_lengths]
             self._replayed = self._replayed or self._capturing()
             return
-        tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
+        tokens = self._per_place(tokens)
         self.lengths += torch.where(taken, torch.tensor(tokens, dtype=torch.int32, device=self.lengths.device), 0)
         self.host_lengths = [n + t if own else 0 for n, t, own in zip(self.host_lengths, tokens, self._owned)]
 
