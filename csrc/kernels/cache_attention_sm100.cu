@@ -9,9 +9,9 @@
 // Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 120 us, 4.6 TB/s. A tile
 // takes 2900 clocks, what the memory takes; the rest is the start (12 000 clocks until the first S: launch, deal, page table, first
 // copies) and the end of a unit (11 000 from the last P to the next unit's first S, in which the ring fills and then waits). 12 trees of 27
-// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 87 us; 78 while values went into the halves times their scales relative to the largest
-// of 32 tokens, which lost what a row sees beside a larger scale that it does not see. The softmax reads three numbers of each token (key's scale, log2 v,
-// 1 / v) out of shared memory, 16 bytes for each lane at a time, where it read one. Measured and not kept:
+// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 83 us; 78 while values went into the halves times their scales relative to the largest
+// of 32 tokens, which lost what a row sees beside a larger scale that it does not see; 87 with a logarithm for each score. A tile takes some 4500 clocks: 10 000
+// warp instructions (decoding, scales, exponentials) at 40 % of the issue slots, no pipe above 29 %, warps waiting for loads and for one another. Measured and not kept:
 // seven decoding warps (81 us for 75), keys' scales in the halves (82, and a rounding more), Q a unit ahead in a second place (122 for 121, 86
 // for 75).
 //
@@ -28,9 +28,8 @@
 //
 // 8-bit scales: scores are multiplied by the key's scale in fp32, and P carries the value's, v: P = 2^(x + log2 v - M + 14), M the largest
 // x + log2 v that the row sees, so that halves have room for what counts in this row, whatever other scales there are (tokens that it does
-// not see, or hardly attends to). The softmax's sum is that of P / v. The first pass over a tile's scores takes log2 v in, the second takes
-// 1 / v, which the group works out in the place of the keys' scales in between (two barriers; shared memory has no room for both). Values
-// are multiplied as the codes that they are; signs of scales, and zeros, go into their halves.
+// not see, or hardly attends to). The softmax's sum is that of P / v. For 32 tokens (what a loading warp has of a tile) whose scales are within
+// 2^6 of one another, M takes the largest score with the largest scale; otherwise a logarithm for each score.
 #include "cache_attention.cuh"
 #include "sm100.cuh"
 
@@ -43,6 +42,7 @@ constexpr int CT_TILE = 128;
 // Units stay whole while the longest has so many tiles more than a CTA's share. Measured (us, whole / cut): 2 trees of 27 in int8, 8 heads of
 // the cache, 200 tokens (one tile more) 16.6 / 19.9, 400 (three) 21.2 / 20.1; 16 tokens of one sequence, bf16, 300 tokens (two) 16.5 / 14.2.
 constexpr int CT_WHOLE = 1;
+constexpr uint32_t CT_WIDE = 6;   // so many powers of two between 32 scales of values are taken for one
 
 template <int D, int KIND> struct CtShape {
   static constexpr bool HALVES = KIND != CA_BF16;
@@ -53,8 +53,9 @@ template <int D, int KIND> struct CtShape {
   static constexpr int RAW = HALVES ? 2 * CT_TILE * D : 0;
   static constexpr int RAWS = HALVES ? 2 : 0;
   static constexpr int Q_OFF = 0, K_OFF = TILE, V_OFF = K_OFF + KST * TILE, RAW_OFF = V_OFF + VST * TILE;
-  // per value stage: scales of keys, logarithms of those of values, and the four loading warps' tokens with odd values
-  static constexpr int SIDE_OFF = RAW_OFF + RAWS * RAW, SCALES = HALVES ? 2 * CT_TILE * 4 : 0, SIDE = SCALES + 16;
+  // per value stage: scales of keys, scales of values times 2^CA_DOWN, and of each loading warp's tokens log2 of the values' largest scale, and
+  // which have odd values
+  static constexpr int SIDE_OFF = RAW_OFF + RAWS * RAW, SCALES = HALVES ? 2 * CT_TILE * 4 + 16 : 0, SIDE = SCALES + 16;
   static constexpr int TOP_OFF = SIDE_OFF + VST * SIDE;             // exponent of the largest |q| of either half of a row
   static constexpr int BAR_OFF = TOP_OFF + (HALVES ? 2 * CT_TILE : 0);
   // k_full[2], k_empty[2], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done[2], side_full[2], q_full
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
   constexpr bool HALVES = L::HALVES;
   constexpr int KST = L::KST, VST = L::VST, KCH = D / 64;
   constexpr uint32_t TM_S = 0, TM_O = 256;   // + 128 for odd tiles
-  constexpr float OFFSET = HALVES ? 14.f : 0.f;
+  constexpr float OFFSET = HALVES ? 14.f - CA_DOWN : 0.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = (uint64_t*)(smem + L::BAR_OFF);
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 8, *s_full = bars + 12, *p_full = bars + 14, *pv_done = bars + 16, *side_full = bars + 18, *q_full = bars + 20;
@@ -325,8 +326,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       if (++w.tile >= w.end) walk_next<CT_TILE>(a, w, 0);
       if (n + 1 < total) seek();
     };
-    // halves of the warp's codes of a tile. Values of tokens in `none` become zeros, those of tokens in `minus` change their sign
-    auto convert = [&](auto is_value, const uint8_t* raw, uint8_t* dst, uint32_t none, uint32_t minus, int first_new, uint32_t& odd) {
+    // halves of the warp's codes of a tile
+    auto convert = [&](auto is_value, const uint8_t* raw, uint8_t* dst, int first_new, uint32_t& odd) {
       constexpr bool VALUE = decltype(is_value)::value;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -351,11 +352,6 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
           halves_of<KIND>(v.y, lo.z, lo.w);
           halves_of<KIND>(v.z, hi.x, hi.y);
           halves_of<KIND>(v.w, hi.z, hi.w);
-          if (VALUE && (none | minus)) {
-            const uint32_t keep = (none >> (tok & 31)) & 1u ? 0u : 0xffffffffu, turn = (minus >> (tok & 31)) & 1u ? 0x80008000u : 0u;
-            lo.x = (lo.x & keep) ^ turn, lo.y = (lo.y & keep) ^ turn, lo.z = (lo.z & keep) ^ turn, lo.w = (lo.w & keep) ^ turn;
-            hi.x = (hi.x & keep) ^ turn, hi.y = (hi.y & keep) ^ turn, hi.z = (hi.z & keep) ^ turn, hi.w = (hi.w & keep) ^ turn;
-          }
           *(uint4*)(dst + ct_at(tok, 2 * q)) = lo;
           *(uint4*)(dst + ct_at(tok, 2 * q + 1)) = hi;
         }
@@ -370,22 +366,27 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       if (HALVES) {
         const uint8_t* raw = smem + L::RAW_OFF + (n & 1) * L::RAW;
         mbar_wait(&k_empty[kst], ((n / KST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
-        convert(std::false_type{}, raw, smem + L::K_OFF + kst * L::TILE, 0u, 0u, 0, odd);
+        convert(std::false_type{}, raw, smem + L::K_OFF + kst * L::TILE, 0, odd);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[kst]);
         // a scale that is no finite number leaves none among its token's values: a new token's are for the rows that see it (ct_odd_values),
-        // a context's are NaN by their logarithm. What lies behind the end is not seen
+        // a context's are NaN by their scale. What lies behind the end is not seen
         const bool there = last_tile + pw * 32 + lane < last_len, infinite = there && odd_scale(vs), wild = infinite && pw * 32 + lane >= first_new;
-        const uint32_t minus = __ballot_sync(0xffffffffu, vs < 0.f), none = __ballot_sync(0xffffffffu, wild || (there && no_scale(vs)));
+        const bool zero = wild || (there && no_scale(vs)), plain = there && !infinite && !zero;
         if (wild) odd = 1u << lane;
-        const float lv = !there ? 0.f : (none >> lane) & 1u ? CA_NONE : infinite ? __int_as_float(0x7fffffff) : log2f(fabsf(vs));
+        const uint32_t size = __float_as_uint(vs) & 0x7fffffffu;
+        const uint32_t most = __reduce_max_sync(0xffffffffu, plain ? size : 0u), least = __reduce_min_sync(0xffffffffu, plain ? size : 0xffffffffu);
+        float top = most ? log2f(__uint_as_float(most)) : CA_NONE;
+        if (__any_sync(0xffffffffu, zero)) top = fmaxf(top, CA_NONE);
+        if (most && (most >> 23) - (least >> 23) > CT_WIDE) top = __int_as_float(0x7fffffff);
         mbar_wait(&v_empty[vst], ((n / VST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
         ((float*)side)[pw * 32 + lane] = ks;
-        ((float*)side)[CT_TILE + pw * 32 + lane] = lv;
+        ((float*)side)[CT_TILE + pw * 32 + lane] = zero ? 0.f : infinite ? __int_as_float(0x7fffffff) : vs * (float)(1 << (int)CA_DOWN);
+        if (lane == 0) ((float*)side)[2 * CT_TILE + pw] = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(&side_full[vst]);                  // the softmax does not wait for the values
-        convert(std::true_type{}, raw + CT_TILE * D, vt, none, minus, first_new, odd);
+        convert(std::true_type{}, raw + CT_TILE * D, vt, first_new, odd);
       } else {
         if (edge) {
 #pragma unroll 1
@@ -472,14 +473,14 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
             v[i].w = ct_pack<true>(bf16_lo(v[i].w) * down, bf16_hi(v[i].w) * down);
           }
         }
-        if (!HALVES) f = fmaxf(f, 1e-30f);   // -inf (not seen) times a factor of zero would be no number
+        f = fmaxf(f, 1e-30f);   // -inf (not seen) times a factor of zero would be no number
         if (!HALVES) asm volatile("bar.sync 1, 256;" ::: "memory");   // the last unit's output has left Q's place (8 bits: the barrier above)
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) *(uint4*)(smem + L::Q_OFF + ct_at(row, group * (D / 16) + i)) = v[i];
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // P = 2^(x f - m f), x the score; of 8-bit caches 2^(y - m + OFFSET), y = x f + log2 v
+      // P = 2^(x f - m f), x the score; of 8-bit caches 2^(x f - m + OFFSET) v, m the largest x f + log2 v. l sums it without v
       float m = -INFINITY, l = 0.f;
       uint32_t odd[4] = {0u, 0u, 0u, 0u};
       int odd_pos = 0;
@@ -493,7 +494,6 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         if (edge && live) ct_visible(a, w.b, t, pos0, w.s, vis_lo, vis_hi);
         if (HALVES) mbar_wait(&side_full[st], (n / VST) & 1, abort_flag, status, TB_ERR_WAIT_FULL);
         // S of this tile; O += P V of the tile before last has finished, or its place would not have been S's
-        const float inverse = HALVES ? exp2f(-((const float*)side)[CT_TILE + row] - CA_DOWN) : 0.f;
         mbar_wait(&s_full[group], (n >> 1) & 1, abort_flag, status, TB_ERR_WAIT_TMEM_FULL);
         tc_fence_after();
         float alpha = 1.f;
@@ -513,9 +513,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
               for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                  const float4 k4 = *(const float4*)(side + ((half * 2 + c) * 32 + i) * 4), l4 = *(const float4*)(side + (CT_TILE + (half * 2 + c) * 32 + i) * 4);
-                  const float2 x = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), make_float2(k4.x, k4.y)), f2, make_float2(l4.x, l4.y));
-                  const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), make_float2(k4.z, k4.w)), f2, make_float2(l4.z, l4.w));
+                  const float4 k4 = *(const float4*)(side + ((half * 2 + c) * 32 + i) * 4);
+                  const float2 x = __fmul2_rn(make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), make_float2(k4.x, k4.y));
+                  const float2 y = __fmul2_rn(make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), make_float2(k4.z, k4.w));
                   v[c][i] = __float_as_uint(x.x), v[c][i + 1] = __float_as_uint(x.y), v[c][i + 2] = __float_as_uint(y.x), v[c][i + 3] = __float_as_uint(y.y);
                 }
             }
@@ -535,14 +535,36 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
               }
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c) {
+              if (HALVES) {
+                const float top = ((const float*)side)[2 * CT_TILE + half * 2 + c];
+                if ((__float_as_uint(top) & 0x7fffffffu) > 0x7f800000u) {
+                  const float* scales = (const float*)side + CT_TILE + (half * 2 + c) * 32;
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                now = fmaxf(now, fmaxf(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])));
-                also = fmaxf(also, fmaxf(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])));
+                  for (int i = 0; i < 32; ++i) {
+                    const float s = fabsf(scales[i]);
+                    now = fmaxf(now, fmaf(__uint_as_float(v[c][i]), f, s == 0.f ? CA_NONE : log2f(s) - CA_DOWN));
+                  }
+                  continue;
+                }
+                also = -INFINITY;
+                float here = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  here = fmaxf(here, fmaxf(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])));
+                  also = fmaxf(also, fmaxf(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])));
+                }
+                now = fmaxf(now, fmaf(fmaxf(here, also), f, top));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  now = fmaxf(now, fmaxf(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])));
+                  also = fmaxf(also, fmaxf(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])));
+                }
               }
+            }
           }
-          now = fmaxf(now, also);
+          if (!HALVES) now = fmaxf(now, also);
           if (HALVES || edge) tmem_wait_st();
           grow = now > m;
           // O of no tile yet, or of tiles that the row saw nothing of, is zero (or not there): any finite factor does
@@ -551,15 +573,6 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
             l *= alpha;
           }
           m = now;
-        }
-        float* inv = (float*)side;
-        if (HALVES) {   // the keys' scales have been read by all: 1 / v in their place
-          asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
-          inv[row] = inverse;
-          asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
-        }
-        if (busy) {
-          uint32_t v[2][32];
           const float ref = (m == -INFINITY ? 0.f : HALVES ? m : m * f) - OFFSET;
           const float2 r2 = make_float2(-ref, -ref);
 #pragma unroll 1
@@ -574,16 +587,13 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const float2 s01 = make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), s23 = make_float2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3]));
-                const float2 x = HALVES ? __fadd2_rn(s01, r2) : __ffma2_rn(s01, f2, r2);
-                const float2 y = HALVES ? __fadd2_rn(s23, r2) : __ffma2_rn(s23, f2, r2);
-                const float2 e = make_float2(exp2f(x.x), exp2f(x.y)), g = make_float2(exp2f(y.x), exp2f(y.y));
+                const float2 x = __ffma2_rn(s01, f2, r2), y = __ffma2_rn(s23, f2, r2);
+                float2 e = make_float2(exp2f(x.x), exp2f(x.y)), g = make_float2(exp2f(y.x), exp2f(y.y));
+                l2 = __fadd2_rn(l2, e);
+                l3 = __fadd2_rn(l3, g);
                 if (HALVES) {
-                  const float4 i4 = *(const float4*)(inv + (half * 2 + c) * 32 + i);
-                  l2 = __ffma2_rn(e, make_float2(i4.x, i4.y), l2);
-                  l3 = __ffma2_rn(g, make_float2(i4.z, i4.w), l3);
-                } else {
-                  l2 = __fadd2_rn(l2, e);
-                  l3 = __fadd2_rn(l3, g);
+                  const float4 v4 = *(const float4*)(side + (CT_TILE + (half * 2 + c) * 32 + i) * 4);
+                  e = __fmul2_rn(e, make_float2(v4.x, v4.y)), g = __fmul2_rn(g, make_float2(v4.z, v4.w));
                 }
                 pk[i / 2] = ct_pack<HALVES>(e.x, e.y);
                 pk[i / 2 + 1] = ct_pack<HALVES>(g.x, g.y);
