@@ -36,3 +36,13 @@ def test_generate_at_next_to_no_temperature(temperature):
     for bad in (-1.0, math.nan):
         with pytest.raises(ValueError):
             m.generate(ids, 2, bad)
+
+
+def test_other_temperatures_keep_their_probabilities_to_the_bit():
+    m = _llama()
+    h = torch.randn(7, 32)
+    logits = h @ m.lm_head.T
+    for t in (0.3, 0.8, 1.0, 2.5):
+        assert torch.equal(m._probs(h, t), torch.softmax(torch.nn.functional.linear(h, m.lm_head)[:, :50] / t, -1))
+    for t in (1e-38, 1e-45, 5e-324):
+        assert torch.equal(m._probs(h, t).argmax(-1), logits[:, :50].argmax(-1)) and torch.equal(m._probs(h, t).amax(-1), torch.ones(7))

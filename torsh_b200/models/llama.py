@@ -211,8 +211,10 @@ class LlamaModel(nn.Module):
         logits = lin_ops.linear(h, self.lm_head, None)[:, : self.cfg.vocab_size].float()
         if temperature == 0:
             return torch.zeros_like(logits).scatter_(1, logits.argmax(-1, keepdim=True), 1.0)
-        # the largest first: a small temperature takes the others out of range, and infinity less infinity is no number
-        return torch.softmax((logits - logits.amax(-1, keepdim=True)) / max(temperature, torch.finfo(torch.float32).tiny), -1)
+        warm = logits / temperature
+        # where that is out of range, from the largest on: infinity less infinity is no number
+        cold = (logits - logits.amax(-1, keepdim=True)) / max(temperature, torch.finfo(torch.float32).tiny)
+        return torch.softmax(torch.where(warm.amax(-1, keepdim=True).isfinite(), warm, cold), -1)
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 0.0, draft: "LlamaModel | None" = None, drafted: int = 4,
