@@ -110,3 +110,20 @@ def test_tokens_of_other_batches_are_refused(bad):
         with pytest.raises(ValueError):
             call(bad)
     assert c.lengths.tolist() == [0, 0] == c.host_lengths and len(c._free) == 6
+
+
+def test_a_place_whose_table_names_others_pages_has_a_length():
+    """A caller's own table (here a prefix that two places share) counts as a sequence."""
+    c = _cache()
+    c.reserve([20, 0])
+    c.page_table[1] = c.page_table[0]
+    q, k, v = _rows(2, 20, 3)
+    c.write(0, k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1))
+    for tokens in (5, [5, 5], torch.tensor([5, 5])):
+        c.advance(tokens)
+    c.advance(torch.tensor([5, 5]), most=5)
+    assert c.lengths.tolist() == [20, 20] == c.host_lengths
+    rk, rv = c.read(0, torch.float32)
+    assert torch.equal(rk, k[:1].expand(2, -1, -1, -1)) and torch.equal(rv, v[:1].expand(2, -1, -1, -1))
+    c.truncate([20, 7])
+    assert c.lengths.tolist() == [20, 7]

@@ -363,19 +363,24 @@ class PagedKVCache:
         return self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
 
     def _bounds(self, exact: bool = False) -> list[int]:
-        """``host_lengths``, brought up to date from the device where replays may have changed them (or where asked to), without what batched
-        steps have added to places that have no pages, whose lengths are 0."""
+        """``host_lengths``, brought up to date from the device where asked to, and where replays may have changed them."""
         if (exact or self._replayed) and not self._capturing():
             self.host_lengths = self.lengths.tolist()
-        return [n if own else 0 for n, own in zip(self.host_lengths, self._owned)]
+        return self.host_lengths
+
+    def _ghosts(self, tokens=None) -> bool:
+        """Whether a place has a length on the host without pages of its own: a batched step has counted it (then the device has 0), or its table
+        names others' pages. ``tokens``: only places that are to get some."""
+        return any(n and not own and (tokens is None or tokens[b]) for b, (n, own) in enumerate(zip(self.host_lengths, self._owned)))
 
     def reserve(self, tokens) -> None:
         """Room for ``tokens`` (an int, or one per sequence) more tokens of every sequence. Raises where the pool or ``max_len`` has none."""
         tokens = self._per_place(tokens)
-        for exact in (False, True):               # upper bounds first: what does not fit them is asked of the device
-            self.host_lengths = self._bounds(exact)
-            need = [max(0, -(-(n + t) // self.page) - len(own)) for n, t, own in zip(self.host_lengths, tokens, self._owned)]
-            longest = max((n + t for n, t in zip(self.host_lengths, tokens)), default=0)
+        for exact in (self._ghosts(tokens), True):   # upper bounds first: what does not fit them is asked of the device
+            # places without pages that get no tokens need none
+            ends = [n + t if t or own else 0 for n, t, own in zip(self._bounds(exact), tokens, self._owned)]
+            need = [max(0, -(-end // self.page) - len(own)) for end, own in zip(ends, self._owned)]
+            longest = max(ends, default=0)
             if longest <= self.max_len and sum(need) <= len(self._free):
                 break
         if longest > self.max_len:
@@ -403,7 +408,7 @@ class PagedKVCache:
     def read(self, layer: int, dtype: torch.dtype = torch.bfloat16):
         """All keys and values of a layer, ``[B, longest, H, D]``."""
         (kp, vp), (ks, vs) = self.layers[layer], self.scales[layer]
-        return kv_cache_read(kp, vp, self.page_table, self.lengths, max(self._bounds(), default=0), None, ks, vs, dtype)
+        return kv_cache_read(kp, vp, self.page_table, self.lengths, max(self._bounds(self._ghosts()), default=0), None, ks, vs, dtype)
 
     def keep(self, path: torch.Tensor, accepted: torch.Tensor) -> None:
         """Moves the accepted nodes of a tree (:func:`~torsh_b200.ops.speculative.verify_draft`) to the front of the tokens just written,
@@ -439,14 +444,15 @@ class PagedKVCache:
             return
         tokens = self._per_place(tokens)
         self.lengths += torch.where(taken, torch.tensor(tokens, dtype=torch.int32, device=self.lengths.device), 0)
-        self.host_lengths = [n + t if own else 0 for n, t, own in zip(self.host_lengths, tokens, self._owned)]
+        self.host_lengths = [n + t for n, t in zip(self.host_lengths, tokens)]
 
     def truncate(self, lengths) -> None:
         """Shortens the sequences to ``lengths`` (one per sequence; shorter ones stay as they are): what lies behind is written over. Their pages
         stay theirs."""
         lengths = [int(n) for n in lengths]
-        if len(lengths) != self.batch or any(not 0 <= n <= was for n, was in zip(lengths, self._bounds())):
-            raise ValueError(f"PagedKVCache: lengths {lengths} of sequences that have {self._bounds()}")
+        have = self._bounds(self._ghosts())
+        if len(lengths) != self.batch or any(not 0 <= n <= was for n, was in zip(lengths, have)):
+            raise ValueError(f"PagedKVCache: lengths {lengths} of sequences that have {have}")
         # the host may know upper bounds only: nothing gets longer
         self.lengths.copy_(torch.minimum(self.lengths, torch.tensor(lengths, dtype=torch.int32, device=self.lengths.device)))
         self.host_lengths = lengths
