@@ -18,8 +18,8 @@
 // The work of all sequences is dealt to the CTAs in equal runs of tiles (deal_tiles), so ragged batches and single long sequences
 // fill the GPU alike; a unit cut by the deal is joined by cache_attn_join_kernel. Short units are not cut (CA_WHOLE).
 //
-// Measured (a call among others, L2 cold): 64 sequences of up to 8192 tokens, 8 heads of D = 128 in e4m3, 618 MB: 112 us, 5.5 TB/s. One
-// sequence of 131 072 tokens in int8, 277 MB: 60 us, 4.6 TB/s, of which 9 are two launches, the deal (a few dependent loads), the page
+// Measured (a call among others, L2 cold): 64 sequences of up to 8192 tokens, 8 heads of D = 128 in e4m3, 618 MB: 113 us, 5.5 TB/s. One
+// sequence of 131 072 tokens in int8, 277 MB: 61 us, 4.6 TB/s, of which 9 are two launches, the deal (a few dependent loads), the page
 // table and the joining. One of 78 tokens: 5.3 us (9.1 with its units cut, 6.5 where the table could hold more).
 #include "cache_attention.cuh"
 #include "decode_calls.h"

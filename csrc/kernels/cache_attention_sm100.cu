@@ -6,12 +6,12 @@
 // values (64 KB in bf16, 33 KB in 8 bits, D = 128) take 2800 and 1450 clocks of the SM's share of HBM. So up to 128 rows cost what
 // the memory takes; mma.sync at 32 rows a CTA read every token rows / 32 times through L2 and was 2.5 to 8 times slower.
 //
-// Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 120 us, 4.6 TB/s. A tile
+// Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 120 to 122 us, 4.5 TB/s. A tile
 // takes 2900 clocks, what the memory takes; the rest is the start (12 000 clocks until the first S: launch, deal, page table, first
 // copies) and the end of a unit (11 000 from the last P to the next unit's first S, in which the ring fills and then waits). 12 trees of 27
-// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 83 us; 78 while values went into the halves times their scales relative to the largest
-// of 32 tokens, which lost what a row sees beside a larger scale that it does not see; 87 with a logarithm for each score. A tile takes some 4500 clocks: 10 000
-// warp instructions (decoding, scales, exponentials) at 40 % of the issue slots, no pipe above 29 %, warps waiting for loads and for one another. Measured and not kept:
+// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 83 us, 33 % of the issue slots, no pipe above 23 %: warps wait for loads and for one another (a
+// tile took 4300 clocks, 10 000 warp instructions, when it was 78 us with the values' scales in their halves relative to the largest of 32
+// tokens, which lost what a row sees beside a larger scale that it does not see). Measured and not kept: a logarithm for each score (87),
 // seven decoding warps (81 us for 75), keys' scales in the halves (82, and a rounding more), Q a unit ahead in a second place (122 for 121, 86
 // for 75).
 //

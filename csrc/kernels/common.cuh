@@ -72,7 +72,8 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
   return warp_max(r);
 }
 
-// Quotients by a number that the host knows: a multiplication instead of a division, for numerators below 2^31.
+// Quotients by a number that the host knows: a multiplication instead of a division, for numerators below 2^31 (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994).
 struct FastDiv {
   unsigned d, m, s;
   __host__ static FastDiv of(unsigned d) {

@@ -10,8 +10,8 @@
 //
 // Bound by memory: each row is read and written once. D / 8 lanes share a row (8 elements each, the row's largest magnitude over
 // shuffles); neighbouring groups take neighbouring heads of a token, which lie together on the contiguous side. Measured: 8 prompts of up
-// to 2048 tokens, 32 heads of 128, bf16 into e4m3, written and read back, 694 MB: 124 us, 5.6 TB/s (127 with addresses in 64 bits
-// throughout). One token of 13 sequences: 6.3 us, two launches of three dependent loads each (start, table, row).
+// to 2048 tokens, 32 heads of 128, bf16 into e4m3, written and read back, 694 MB: 124 to 128 us, 5.4 to 5.6 TB/s (127 with addresses in 64 bits
+// throughout, where it took 124). One token of 13 sequences: 6.2 to 6.5 us, two launches of three dependent loads each (start, table, row).
 #include <cuda_fp8.h>
 
 #include "common.cuh"

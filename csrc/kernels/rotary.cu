@@ -4,11 +4,13 @@
 //
 // over the first R of D columns; pairs are (2i, 2i+1) or (i, i + R/2), columns from R on pass through. The backward pass is
 // the same map with sin negated. Position and frequency meet in 64 bits: p * f / 2pi is reduced to a fraction of a turn
-// before it is rounded to fp32 (p * f rounded to fp32 first is off by 0.06 rad at p = 10^6), then sincospif.
+// before it is rounded to fp32 (p * f rounded to fp32 first is off by 0.06 rad at p = 10^6), then sincospif: the fraction's
+// rounding (1e-7 radians) and that of sincospif are what fp32 rows show, 4.8e-8 of a row's size where angles in 64 bits leave 3.5e-8. Turning by what the
+// fraction drops as well takes 21.4 us for 19.8 in the second case below.
 //
 // Bound by memory: x is read and y written once. The angles of a token are worked out once per block into shared memory:
 // R/2 sine/cosine pairs for every (Hq + Hk) D elements, while the block's loads are on their way. Measured, forward and backward: 8192
-// tokens of 64 heads of 128 in bf16, 537 MB: 90 us, 6 TB/s; 4593 tokens of 20 heads of 64 in fp32, half of each turned, 94 MB: 20 us. What is
+// tokens of 64 heads of 128 in bf16, 537 MB: 92 us, 5.8 TB/s; 4593 tokens of 20 heads of 64 in fp32, half of each turned, 94 MB: 20 us. What is
 // issued for a row counts (0.78 instructions a clock of each scheduler when it took 98): a vector turns or passes through as a whole,
 // addresses are offsets from the block's first token. Sines kept in registers from row to row (a branch a row): 100; twice the rows in
 // flight: 110.

@@ -264,7 +264,8 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     places that a row does not see do not reach it (a value scale that is no finite number leaves none among its token's values). ``scale`` is ``1 / sqrt(D)`` unless given; positions from ``max_len`` on, if given, are
     not read. Pages outside the pool read as zeros. No backward pass; forward-mode derivatives are computed in PyTorch.
 
-    Probabilities are rounded to bf16 over bf16 pages. Over 8-bit pages they are rounded to halves, times the scale of their value and relative to
+    Probabilities are rounded to bf16 over bf16 pages. Over 8-bit pages queries are multiplied as halves relative to a power of two near the
+    row's largest column (columns below 2^-16 of it lose bits, below 2^-25 they count as zero), and probabilities are rounded to halves, times the scale of their value and relative to
     the largest such product that the row sees: a scale that a row does not see, or hardly attends to, takes nothing from the others. Scales of
     ``v_scales`` from 2^122 on count as infinite, those below 2^-96 as zero.
     """
@@ -321,9 +322,9 @@ def tree_mask_of(parents: torch.Tensor) -> torch.Tensor:
 class PagedKVCache:
     """Pages of one or more layers, the sequences that own them, and the calls on them.
 
-    ``dtype`` is ``torch.bfloat16``, ``torch.int8`` or ``torch.float8_e4m3fn``. Heads of 64 or 128 columns, and queries in bf16, take the kernels;
-    other heads and types run in PyTorch, which gathers a context in fp32 and waits for the device, so that such steps cannot be captured. Every layer has its own pages; the table and the lengths
-    are common. A step is: :meth:`reserve` room for the new tokens of the batch, for each layer :meth:`write` their keys and values and
+    ``dtype`` is ``torch.bfloat16``, ``torch.int8`` or ``torch.float8_e4m3fn``. Heads of 64 or 128 columns, and queries in bf16, take the
+    kernels; other heads and types run in PyTorch, which gathers a context in fp32 and waits for the device, so that such steps cannot be
+    captured. Every layer has its own pages; the table and the lengths are common. A step is: :meth:`reserve` room for the new tokens of the batch, for each layer :meth:`write` their keys and values and
     :meth:`attend`, then :meth:`advance` the lengths by what is kept (after a verification fewer than were written: the rest is
     written over). Table and lengths are device tensors that are written in place, so a step with ``advance(tensor, most)`` can be captured
     into a graph and replayed while what has been reserved lasts; after one, :meth:`reserve`, :meth:`read` and :meth:`truncate` ask the device for the
