@@ -11,14 +11,14 @@
 // from registers, which is where the 8-bit codes are decoded.
 //
 // 8-bit codes are multiplied as halves: int8 and e4m3 are exact there, q is brought into the half's range by a power of two per row, and
-// P carries the value's scale v: P = 2^(x + log2 v - M + 8), M the largest x + log2 v that the row sees, so that halves have room for
-// what counts in this row, whatever other scales there are (tokens that it does not see, or hardly attends to). The softmax's sum is
+// P carries the value's scale v: P = 2^(x - M + 8) v, M the largest x + log2 v that the row sees (with the power of two above v), so that halves have room
+// for what counts in this row, whatever other scales there are (tokens that it does not see, or hardly attends to). The softmax's sum is
 // that of P / v. P in halves has eight times the bits of bf16. Scores, maxima, sums and O are fp32.
 //
 // The work of all sequences is dealt to the CTAs in equal runs of tiles (deal_tiles), so ragged batches and single long sequences
 // fill the GPU alike; a unit cut by the deal is joined by cache_attn_join_kernel. Short units are not cut (CA_WHOLE).
 //
-// Measured (a call among others, L2 cold): 64 sequences of up to 8192 tokens, 8 heads of D = 128 in e4m3, 618 MB: 113 us, 5.5 TB/s. One
+// Measured (a call among others, L2 cold): 64 sequences of up to 8192 tokens, 8 heads of D = 128 in e4m3, 618 MB: 112 us, 5.5 TB/s. One
 // sequence of 131 072 tokens in int8, 277 MB: 61 us, 4.6 TB/s, of which 9 are two launches, the deal (a few dependent loads), the page
 // table and the joining. One of 78 tokens: 5.3 us (9.1 with its units cut, 6.5 where the table could hold more).
 #include "cache_attention.cuh"
@@ -295,18 +295,17 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
       }
 
       const bool edge = pos0 + CA_TILE > min(w.s.start, w.s.len);   // new tokens in it, or the end of the sequence
-      float ks[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f}, reach[2] = {0.f, 0.f}, inv[2] = {1.f, 1.f}, sign[2] = {1.f, 1.f};
+      float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f}, reach[2] = {0.f, 0.f};
       if (HALVES) {
         const float* scales = (const float*)(vt + S::TILE_BYTES);
         ks[0] = scales[g], ks[1] = scales[g + 8];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float vs = scales[CA_TILE + g + 8 * i];
-          const bool none = no_scale(vs), odd = odd_scale(vs);
-          sign[i] = odd ? __int_as_float(0x7fffffff) : none ? 0.f : vs < 0.f ? -1.f : 1.f;
-          lv[i] = none || odd ? 0.f : log2f(fabsf(vs));
-          reach[i] = none ? CA_NONE : lv[i];
-          inv[i] = exp2f(-lv[i] - CA_DOWN);
+          const float v = scales[CA_TILE + g + 8 * i];
+          const uint32_t ex = (__float_as_uint(v) & 0x7fffffffu) >> 23;
+          vs[i] = odd_scale(v) ? __int_as_float(0x7fffffff) : no_scale(v) ? 0.f : v;
+          // log2 of the power of two above v: the exponent as a float, by the bits of 2^23 + ex
+          reach[i] = no_scale(v) ? CA_NONE : __uint_as_float(0x4b000000u | ex) - (8388608.f + 126.f);
         }
       }
 
@@ -344,11 +343,9 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
         const float ref[2] = {(mx[n][0] == -INFINITY ? 0.f : mx[n][0]) - OFFSET, (mx[n][1] == -INFINITY ? 0.f : mx[n][1]) - OFFSET};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = sc[n][e] - ref[e & 1];
-          if (HALVES) x += lv[e >> 1];
-          float p = exp2f(x);
-          sum[n][e & 1] += HALVES ? p * inv[e >> 1] : p;
-          if (HALVES) p = sc[n][e] == -INFINITY ? 0.f : p * sign[e >> 1];
+          float p = exp2f(sc[n][e] - ref[e & 1]);
+          sum[n][e & 1] += p;
+          if (HALVES) p = sc[n][e] == -INFINITY ? 0.f : p * vs[e >> 1];
           sc[n][e] = p;
         }
         pf[n][0] = transpose8(pack2<HALVES>(sc[n][0], sc[n][1]));
@@ -468,7 +465,7 @@ __global__ void __launch_bounds__(CA_THREADS, (CaShape<D, KIND, NT>::OCC)) cache
           const float2 y = *(const float2*)(ml + (v * S::ROWS + row) * 2);
           all += y.y * exp2f(y.x - ref);
         }
-        const float f = exp2f(mx[n][r] - ref) * (HALVES ? exp2f(-CA_DOWN) : 1.f);
+        const float f = exp2f(mx[n][r] - ref);
 #pragma unroll
         for (int j = 0; j < MB; ++j) o[j][n][r] *= f, o[j][n][2 + r] *= f;
         norm[n][r] = all > 0.f || all != all ? 1.f / all : 0.f;   // a row that sees nothing: zeros

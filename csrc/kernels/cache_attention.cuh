@@ -197,13 +197,12 @@ __device__ __forceinline__ bool sees(const CacheAttnArgs& a, int b, int t, int p
   return a.mask ? a.mask[b * a.mask_b + t * a.mask_t + j] != 0 : j <= t;
 }
 
-// Scales of 8-bit values, v. Those from 2^122 on (pages hold none above 2^121) count as infinite. Those below 2^-96 count as none: their tokens'
-// values are zeros, and the maximum of x + log2 v takes them for 2^CA_NONE, which moves it little beside scales of 2^-80 and more, and keeps
-// their share of the sum in range beside scales up to 2^40. Sums are those of P / v times 2^-CA_DOWN, and so is O at a unit's end: P is at
-// most 2^14, so that 1 / v and the sums of 2^21 tokens are in fp32's range for each of these scales.
-constexpr float CA_DOWN = 4.f, CA_NONE = -60.f;
+// Scales of 8-bit values, v. Those from 2^122 on (pages hold none above 2^121) count as infinite. Those below 2^-92 count as none: their tokens'
+// values are zeros, and the maximum of x + log2 v takes them for 2^CA_NONE, which moves it little beside scales of 2^-80 and more. The sum is
+// that of P / v, P at most 2^14: in fp32's range for 2^21 tokens of the smallest scale, and for shares of 2^-18 and more beside one of 2^115.
+constexpr float CA_NONE = -60.f;
 __device__ __forceinline__ bool odd_scale(float v) { return (__float_as_uint(v) & 0x7fffffffu) >= 0x7c800000u; }
-__device__ __forceinline__ bool no_scale(float v) { return (__float_as_uint(v) & 0x7fffffffu) < 0x0f800000u; }
+__device__ __forceinline__ bool no_scale(float v) { return (__float_as_uint(v) & 0x7fffffffu) < 0x11800000u; }
 
 // Two 8-bit codes (the low 16 bits of v) as two halves.
 template <int KIND>

@@ -9,7 +9,7 @@
 // Measured (a call among others, L2 cold): 8 trees of 48 tokens, 32 heads of D = 128 over 4096 tokens of bf16, 549 MB: 120 to 122 us, 4.5 TB/s. A tile
 // takes 2900 clocks, what the memory takes; the rest is the start (12 000 clocks until the first S: launch, deal, page table, first
 // copies) and the end of a unit (11 000 from the last P to the next unit's first S, in which the ring fills and then waits). 12 trees of 27
-// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 83 us, 33 % of the issue slots, no pipe above 23 %: warps wait for loads and for one another (a
+// tokens, 32 heads over 8, ragged up to 6000 tokens of int8, 95 MB: 81 us, 33 % of the issue slots, no pipe above 23 %: warps wait for loads and for one another (a
 // tile took 4300 clocks, 10 000 warp instructions, when it was 78 us with the values' scales in their halves relative to the largest of 32
 // tokens, which lost what a row sees beside a larger scale that it does not see). Measured and not kept: a logarithm for each score (87),
 // seven decoding warps (81 us for 75), keys' scales in the halves (82, and a rounding more), Q a unit ahead in a second place (122 for 121, 86
@@ -53,8 +53,7 @@ template <int D, int KIND> struct CtShape {
   static constexpr int RAW = HALVES ? 2 * CT_TILE * D : 0;
   static constexpr int RAWS = HALVES ? 2 : 0;
   static constexpr int Q_OFF = 0, K_OFF = TILE, V_OFF = K_OFF + KST * TILE, RAW_OFF = V_OFF + VST * TILE;
-  // per value stage: scales of keys, scales of values times 2^CA_DOWN, and of each loading warp's tokens log2 of the values' largest scale, and
-  // which have odd values
+  // per value stage: scales of keys and of values, and of each loading warp's tokens log2 of the values' largest scale, and which have odd values
   static constexpr int SIDE_OFF = RAW_OFF + RAWS * RAW, SCALES = HALVES ? 2 * CT_TILE * 4 + 16 : 0, SIDE = SCALES + 16;
   static constexpr int TOP_OFF = SIDE_OFF + VST * SIDE;             // exponent of the largest |q| of either half of a row
   static constexpr int BAR_OFF = TOP_OFF + (HALVES ? 2 * CT_TILE : 0);
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
   constexpr bool HALVES = L::HALVES;
   constexpr int KST = L::KST, VST = L::VST, KCH = D / 64;
   constexpr uint32_t TM_S = 0, TM_O = 256;   // + 128 for odd tiles
-  constexpr float OFFSET = HALVES ? 14.f - CA_DOWN : 0.f;
+  constexpr float OFFSET = HALVES ? 14.f : 0.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = (uint64_t*)(smem + L::BAR_OFF);
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 8, *s_full = bars + 12, *p_full = bars + 14, *pv_done = bars + 16, *side_full = bars + 18, *q_full = bars + 20;
@@ -382,7 +381,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
         if (most && (most >> 23) - (least >> 23) > CT_WIDE) top = __int_as_float(0x7fffffff);
         mbar_wait(&v_empty[vst], ((n / VST) & 1) ^ 1, abort_flag, status, TB_ERR_WAIT_EMPTY);
         ((float*)side)[pw * 32 + lane] = ks;
-        ((float*)side)[CT_TILE + pw * 32 + lane] = zero ? 0.f : infinite ? __int_as_float(0x7fffffff) : vs * (float)(1 << (int)CA_DOWN);
+        ((float*)side)[CT_TILE + pw * 32 + lane] = zero ? 0.f : infinite ? __int_as_float(0x7fffffff) : vs;
         if (lane == 0) ((float*)side)[2 * CT_TILE + pw] = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(&side_full[vst]);                  // the softmax does not wait for the values
@@ -543,7 +542,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
 #pragma unroll
                   for (int i = 0; i < 32; ++i) {
                     const float s = fabsf(scales[i]);
-                    now = fmaxf(now, fmaf(__uint_as_float(v[c][i]), f, s == 0.f ? CA_NONE : log2f(s) - CA_DOWN));
+                    now = fmaxf(now, fmaf(__uint_as_float(v[c][i]), f, s == 0.f ? CA_NONE : log2f(s)));
                   }
                   continue;
                 }
@@ -649,8 +648,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) cache_attn_tc_kernel(const __gr
       const float f_mine = exp2f(mine_r - ref), f_other = exp2f(other.x - ref);
       const float all = l * f_mine + other.y * f_other;
       // a group that has had no tile, or whose tiles the row saw nothing of, has nothing in its O
-      constexpr float DOWN = HALVES ? 1.f / (float)(1 << (int)CA_DOWN) : 1.f;
-      const float f0 = (group ? f_other : f_mine) * DOWN, f1 = (group ? f_mine : f_other) * DOWN;
+      const float f0 = group ? f_other : f_mine, f1 = group ? f_mine : f_other;
       const bool has0 = (group ? other.y : l) != 0.f, has1 = (group ? l : other.y) != 0.f;
       asm volatile("bar.sync 1, 256;" ::: "memory");   // read, before the next Q overwrites it
       const bool whole = w.head == 0 && w.end == w.nt;

@@ -267,7 +267,7 @@ def kv_cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     Probabilities are rounded to bf16 over bf16 pages. Over 8-bit pages queries are multiplied as halves relative to a power of two near the
     row's largest column (columns below 2^-16 of it lose bits, below 2^-25 they count as zero), and probabilities are rounded to halves, times the scale of their value and relative to
     the largest such product that the row sees: a scale that a row does not see, or hardly attends to, takes nothing from the others. Scales of
-    ``v_scales`` from 2^122 on count as infinite, those below 2^-96 as zero.
+    ``v_scales`` from 2^122 on count as infinite, those below 2^-92 as zero.
     """
     if q.is_cuda:
         out = (nv._decode or nv.decode_calls()).kv_attention(q, k_pages, v_pages, page_table, start, tree_mask, counts, k_scales, v_scales, scale, max_len,
