@@ -126,3 +126,31 @@ def test_scales_at_the_ends_of_what_pages_hold(dtype, size, shape, wide):
     ref, mass = _attend64(q, kp, vp, ks, vs, table, start, mask, None, D ** -0.5)
     _close(got, ref, mass, *_weight(q, kp, ks, vs, table, start, mask, D ** -0.5, H, page))
     assert not kv_cache_attention(q, kp, vp, table, start, mask, None, ks, torch.zeros_like(vs)).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, E4M3])
+@pytest.mark.parametrize("shape,wide", SHAPES)
+def test_scales_beyond_the_ends_are_none_and_infinite(dtype, shape, wide):
+    """As documented: 2^122 and more is no finite number to the rows that see it, and nothing to the others; less than 2^-92 is zero."""
+    from torsh_b200.ops.kv_cache import kv_cache_attention
+    q, kp, vp, ks, vs, table, start = _case(*shape, dtype)
+    B, T, Hq, H, D, page = shape[:6]
+    table = torch.nn.functional.pad(table, (0, wide), value=-1)
+    mask = _random_tree(T, 5)
+    call = lambda: kv_cache_attention(q, kp, vp, table, start, mask, None, ks, vs)   # noqa: E731
+    at = [(int(table[b, (int(start[b]) + 1) // page]), (int(start[b]) + 1) % page) for b in range(B)]   # token 1 of the new ones
+    for p, r in at:
+        vs[p, :, r] = 2.0 ** -93
+    small = call()
+    for p, r in at:
+        vs[p, :, r] = 0
+    assert torch.equal(small, call())
+    ref, mass = _attend64(q, kp, vp, ks, vs, table, start, mask, None, D ** -0.5)
+    for scale in (2.0 ** 122, -2.0 ** 127):
+        for p, r in at:
+            vs[p, :, r] = scale
+        got = call()
+        seen = mask[:, 1]
+        assert not torch.isfinite(got[:, seen]).any()
+        got[:, seen] = ref[:, seen].to(got.dtype)
+        _close(got, ref, mass, *_weight(q, kp, ks, torch.where(vs.abs() >= 2.0 ** 122, 0.0, vs), table, start, mask, D ** -0.5, H, page))
